@@ -10,6 +10,10 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libmia_hip.so")
+# No packed-fp32 instructions (v_pk_add/mul/fma_f32): hipcc forms them by itself from ordinary float code at -O3, and some
+# of their forms have given wrong results now and then, without an error. The host pass warns that it does not know the
+# feature, which is harmless.
+HIPFLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 SOURCES = ["runtime.hip", "gemm.hip", "dwconv.hip", "pointwise.hip", "head.hip", "preprocess.hip", "optim.hip", "seg.hip", "metrics.hip", "augment.hip"]
 
 
@@ -34,7 +38,7 @@ def _stale() -> bool:
     t = os.path.getmtime(LIB)
     # the public header too: _lib.py derives every ctypes prototype from it, so a library older than the header
     # could be called with the wrong argument list
-    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", "mia_hip.h")]
+    deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", "mia_hip.h"), __file__]
     return any(os.path.getmtime(d) > t for d in deps)
 
 
@@ -52,9 +56,9 @@ def build(force: bool = False, verbose: bool = True) -> str:
         obj = os.path.join(HERE, "build", src.replace(".hip", ".o"))
         objs.append(obj)
         if (not force) and os.path.exists(obj) and os.path.getmtime(obj) > max(
-                os.path.getmtime(path), os.path.getmtime(os.path.join(CSRC, "common.h"))):
+                os.path.getmtime(path), os.path.getmtime(os.path.join(CSRC, "common.h")), os.path.getmtime(__file__)):
             continue
-        cmd = [hipcc, "--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-c", path, "-o", obj]
+        cmd = [hipcc, *HIPFLAGS, "-c", path, "-o", obj]
         if verbose:
             print(" ".join(cmd), flush=True)
         procs.append((src, subprocess.Popen(cmd)))

@@ -35,8 +35,8 @@ struct DwParams {
     int gx, ncb;  // matrix-core kernels: 1-D grid of gx tile walkers x ncb channel blocks (see dw_decode_block)
 };
 
-// Four channels as two explicit 2-vectors (f22): each 2-vector op is one packed-f32 instruction on a naturally
-// paired register couple. (Left to itself the vectoriser pairs values across taps and spends a move per packed FMA.)
+// Four channels as two explicit 2-vectors (f22) on naturally paired register couples (the library is built without the
+// packed-f32 instructions: two scalar FMAs each).
 __device__ __forceinline__ void fma22(f22& acc, const f22& a, const f22& b) {
     acc.lo = a.lo * b.lo + acc.lo;
     acc.hi = a.hi * b.hi + acc.hi;
@@ -1027,7 +1027,7 @@ __global__ __launch_bounds__(256, 2) void dwconv_bwd_lin_s2_kernel(DwParams p, D
 // A thread owns KR tap rows of one 4-channel vector (KR*K accumulators). KR = 1 keeps the register footprint small for
 // the 5x5 kernels (the K tap rows of a channel vector are K different threads reading the same staged tiles); KR = K
 // for 3x3: the four gradient vectors of a patch are read and unpacked once for all nine taps instead of once per tap
-// row, and the patch walk's address arithmetic is paid once instead of three times (per 72 packed FMAs: 22 LDS reads
+// row, and the patch walk's address arithmetic is paid once instead of three times (per 72 two-channel FMAs: 22 LDS reads
 // instead of 30, 88 unpack instructions instead of 120).
 // SW (stride 1 with a prologue): the operands change roles. dW[t] = sum_q dY(q) * a(q + t - PAD) is also
 // sum_p a(p) * dY(p - t + PAD): the activated tensor is staged as the CENTRE tile and the gradient as the window with
