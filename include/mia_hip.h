@@ -305,6 +305,24 @@ int mia_adamw_step(int n_tensors, const void* const* params, const void* const* 
                    const void* const* exp_avg_sq, const long long* sizes, double lr, double beta1, double beta2,
                    double eps, double weight_decay, int step, double grad_scale, const float* dev_hyper,
                    void* stream);
+/* The same step on clipped gradients: every gradient is also multiplied by norm_and_factor[1] (DEVICE memory, written by
+ * mia_grad_norm earlier on the stream); the gradients themselves are left as they are. */
+int mia_adamw_step_clipped(int n_tensors, const void* const* params, const void* const* grads,
+                           const void* const* exp_avg, const void* const* exp_avg_sq, const long long* sizes, double lr,
+                           double beta1, double beta2, double eps, double weight_decay, int step, double grad_scale,
+                           const float* dev_hyper, const float* norm_and_factor, void* stream);
+/* Global gradient norm and clipping. The reference does not clip; the arithmetic is torch.nn.utils.clip_grad_norm_'s:
+ * norm = sqrt(sum over all tensors of g*g), factor = min(1, max_norm / (norm + 1e-6)), a NaN norm giving a NaN factor.
+ * grads: HOST array of DEVICE pointers (each tensor dense, aligned to its elements only); dtypes: host array of
+ * MIA_F32 / MIA_BF16, NULL = all fp32; sizes: host array of element counts. Squares are summed in double in a fixed order.
+ * ws: mia_grad_norm_ws_doubles(n_tensors, sizes) doubles of scratch. norm_and_factor: 2 floats in DEVICE memory. */
+long long mia_grad_norm_ws_doubles(int n_tensors, const long long* sizes);
+/* norm_and_factor = {|grad_scale| * norm, factor for that norm}; the gradients are only read. */
+int mia_grad_norm(int n_tensors, const void* const* grads, const int* dtypes, const long long* sizes, double grad_scale,
+                  double max_norm, double* ws, long long ws_doubles, float* norm_and_factor, void* stream);
+/* The same, and g *= factor in place (nothing is written when factor is 1). */
+int mia_grad_clip(int n_tensors, const void* const* grads, const int* dtypes, const long long* sizes, double max_norm,
+                  double* ws, long long ws_doubles, float* norm_and_factor, void* stream);
 /* Stores n (<= 64) 32-bit words, passed by value in the launch, to device memory dst. No counterpart in the
  * reference: it refreshes the per-step words a replayed graph reads (seed_offset, dev_hyper) without a host buffer
  * that must stay untouched until an asynchronous copy has run. */

@@ -5,18 +5,123 @@ which the reference builds at train.py:193-197 and finetune.py:232-248, so LR sc
 (ReduceLROnPlateau, train.py:199-201) and optimizer checkpoints (train.py:440) keep working."""
 import ctypes
 import math
+from array import array
 
 import torch
 
 from ._lib import lib
-from .ops import Side, WeightEpoch, _stream
+from .ops import _DT, Side, WeightEpoch, _p, _stream
+
+
+def _grad_table(grads):
+    """Host tables of a list of gradients for mia_grad_norm / mia_grad_clip -> (count, addresses, dtypes, sizes, device);
+    the arrays have to outlive the call that reads them. dtypes is None when all are fp32."""
+    devices = {g.get_device() for g in grads}
+    if len(devices) != 1 or min(devices) < 0:
+        raise RuntimeError("gradient norm and clipping need their tensors on one MI355X device; there is no CPU path")
+    kinds = {g.dtype for g in grads}
+    if not kinds <= _DT.keys():
+        raise TypeError(f"gradients are fp32 or bf16 (got {', '.join(sorted(str(k) for k in kinds))})")
+    if any(g.is_sparse for g in grads):
+        raise TypeError("gradients are dense tensors")
+    dtypes = None if kinds == {torch.float32} else array("i", [_DT[g.dtype] for g in grads])
+    return (len(grads), array("Q", [g.data_ptr() for g in grads]), dtypes, array("q", [g.numel() for g in grads]),
+            grads[0].device)
+
+
+def _dense(g):
+    """Whether the elements fill one run of memory in some order: a norm and a scaling need no more than that."""
+    if g.is_contiguous():
+        return True
+    run = 1
+    for stride, size in sorted((st, n) for st, n in zip(g.stride(), g.shape) if n != 1):
+        if stride != run:
+            return False
+        run *= size
+    return True
+
+
+def _addr(a):
+    return a.buffer_info()[0] if a is not None else None
+
+
+def _norm_ws(n, sizes, device):
+    nws = lib().mia_grad_norm_ws_doubles(n, _addr(sizes))
+    return torch.empty((nws,), dtype=torch.float64, device=device), nws
+
+
+def _check_max_norm(max_norm):
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"max_norm must not be negative (got {max_norm})")
+    return max_norm
+
+
+@torch.no_grad()
+def grad_norm(grads):
+    """Norm of all elements of the tensors together (fp32 or bf16, any mix, dense), as a 0-d fp32 device tensor: one pass,
+    squares summed in double in a fixed order, nothing read back to the host."""
+    grads = [g if _dense(g) else g.contiguous() for g in grads]
+    if not grads:
+        return torch.zeros(())
+    n, ptrs, dtypes, sizes, device = _grad_table(grads)
+    with torch.cuda.device(device):
+        ws, nws = _norm_ws(n, sizes, device)
+        out = torch.empty((2,), dtype=torch.float32, device=device)
+        lib().mia_grad_norm(n, _addr(ptrs), _addr(dtypes), _addr(sizes), 1.0, 0.0, _p(ws), nws, _p(out), _stream())
+    return out[0]
+
+
+@torch.no_grad()
+def clip_grads_(grads, max_norm):
+    """Scales the tensors in place so that their global norm is at most max_norm and returns the norm they had (0-d fp32
+    device tensor): g *= min(1, max_norm / (norm + 1e-6)), as torch.nn.utils.clip_grad_norm_ does. No host
+    synchronisation; the tensors must not overlap; may be captured into a HIP graph. A norm that is infinite or NaN makes the gradients zero, NaN or
+    both, as there: look at the returned norm where that can happen."""
+    max_norm = _check_max_norm(max_norm)
+    grads = list(grads)
+    if not grads:
+        return torch.zeros(())
+    for g in grads:
+        if not _dense(g):
+            raise ValueError(f"clip_grads_ scales in place and needs dense tensors (got strides {g.stride()} for {tuple(g.shape)})")
+    n, ptrs, dtypes, sizes, device = _grad_table(grads)
+    if len(set(ptrs)) != n and len({a for a, k in zip(ptrs, sizes) if k}) != sum(1 for k in sizes if k):
+        raise ValueError("a tensor is listed twice: it would be scaled twice")
+    with torch.cuda.device(device):
+        ws, nws = _norm_ws(n, sizes, device)
+        out = torch.empty((2,), dtype=torch.float32, device=device)
+        lib().mia_grad_clip(n, _addr(ptrs), _addr(dtypes), _addr(sizes), max_norm, _p(ws), nws, _p(out), _stream())
+    return out[0]
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm):
+    """clip_grads_ over the .grad of the parameters that have one (a single tensor counts as a list of one), ordered after
+    the weight gradients that may still run on the second stream. The drop-in for torch.nn.utils.clip_grad_norm_ with the
+    2-norm; an AdamW built with max_grad_norm clips by itself and never writes the gradients."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    Side.sync()
+    params = [p for p in parameters if p.grad is not None]
+    for p in params:
+        if not _dense(p.grad):
+            p.grad = p.grad.contiguous()
+    return clip_grads_([p.grad for p in params], max_norm)
 
 
 class AdamW(torch.optim.Optimizer):
-    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+    """max_grad_norm: every step first scales the gradients of ALL groups to that global norm at most (grad_norm holds the
+    norm they had, a device scalar). The factor stays on the device and is applied as the update reads the gradients, which
+    are left as they are. It belongs to the optimizer, not to its state: checkpoints keep torch's layout. In a captured
+    step it is the value at the capture."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, max_grad_norm=None):
         if lr < 0 or eps < 0 or not 0 <= betas[0] < 1 or not 0 <= betas[1] < 1 or weight_decay < 0:
             raise ValueError("invalid AdamW hyper-parameter")
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+        self.max_grad_norm = _check_max_norm(max_grad_norm) if max_grad_norm is not None else None
+        self.grad_norm = None
         self._tables = {}
         # per-parameter step counts as Python ints. torch.optim.AdamW increments one CPU tensor per parameter and
         # step (several hundred tiny host ops); here the parameters that share a count share ONE state["step"] tensor,
@@ -79,6 +184,7 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         Side.sync()     # weight gradients still running on the side stream are ordered before the update
         WeightEpoch.bump()      # the kernel rewrites the parameters through their raw pointers
+        launches = []
         for gi, group in enumerate(self.param_groups):
             ps = [p for p in group["params"] if p.grad is not None]
             if not ps:
@@ -102,27 +208,48 @@ class AdamW(torch.optim.Optimizer):
                 k += 1
                 self._pstep[p] = k
                 by_step.setdefault(k, []).append(p)
-            b1, b2 = group["betas"]
             # parameters that joined later (unfrozen for fine-tuning) carry their own step count, as in torch: one
             # launch per distinct count (a single launch in the usual case)
             for si, (k, plist) in enumerate(sorted(by_step.items())):
                 shared = torch.tensor(float(k))
                 for p in plist:
                     self.state[p]["step"] = shared
-                n, tp, tg, tm, tv, sizes = self._table((gi, si), plist)
-                dev_hyper = None
-                if self._capture is not None:
-                    ptr, max_rows, rows = self._capture
-                    if len(rows) >= max_rows:
-                        raise RuntimeError("too many distinct (group, step count) launches for one captured step")
-                    if grad_scale != 1.0:
-                        raise RuntimeError("grad_scale cannot be captured")
-                    dev_hyper = ptr + 16 * len(rows)
-                    rows.append((gi, plist))
-                lib().mia_adamw_step(n, tp, tg, tm, tv, sizes, float(group["lr"]), float(b1), float(b2),
-                                     float(group["eps"]), float(group["weight_decay"]), k, float(grad_scale), dev_hyper,
-                                     _stream())
+                launches.append((gi, group, k, plist, self._table((gi, si), plist)))
+        clip = self._clip_factor([tab for *_, tab in launches], grad_scale) if self.max_grad_norm is not None and launches else None
+        for gi, group, k, plist, (n, tp, tg, tm, tv, sizes) in launches:
+            b1, b2 = group["betas"]
+            dev_hyper = None
+            if self._capture is not None:
+                ptr, max_rows, rows = self._capture
+                if len(rows) >= max_rows:
+                    raise RuntimeError("too many distinct (group, step count) launches for one captured step")
+                if grad_scale != 1.0:
+                    raise RuntimeError("grad_scale cannot be captured")
+                dev_hyper = ptr + 16 * len(rows)
+                rows.append((gi, plist))
+            args = (n, tp, tg, tm, tv, sizes, float(group["lr"]), float(b1), float(b2), float(group["eps"]),
+                    float(group["weight_decay"]), k, float(grad_scale), dev_hyper)
+            if clip is None:
+                lib().mia_adamw_step(*args, _stream())
+            else:
+                lib().mia_adamw_step_clipped(*args, _p(clip), _stream())
         return loss
+
+    def _clip_factor(self, tables, grad_scale):
+        """{norm, factor} on the device, over the gradients of every launch of the step."""
+        if len(tables) == 1:
+            n, _, tg, _, _, sizes = tables[0]
+        else:
+            n = sum(t[0] for t in tables)
+            tg = (ctypes.c_void_p * n)(*[a for t in tables for a in t[2]])
+            sizes = (ctypes.c_longlong * n)(*[a for t in tables for a in t[5]])
+        device = next(p for g in self.param_groups for p in g["params"] if p.grad is not None).device
+        nws = lib().mia_grad_norm_ws_doubles(n, sizes)
+        ws = torch.empty((nws,), dtype=torch.float64, device=device)
+        out = torch.empty((2,), dtype=torch.float32, device=device)
+        lib().mia_grad_norm(n, tg, None, sizes, float(grad_scale), self.max_grad_norm, _p(ws), nws, _p(out), _stream())
+        self.grad_norm = out[0]
+        return out
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)
