@@ -220,6 +220,36 @@ int mia_attention_bwd(int dtype, const void* qkv, const float* P, const void* do
                       int C, int heads, float pdrop, unsigned long long seed, const unsigned long long* seed_offset,
                       void* dqkv, void* stream);
 
+/* ---- attention with a learned relative position bias (no counterpart in the reference, whose attention over the tokens of
+ *      the feature map, model.py:153-163, knows no positions) -----------------------------------------------------------
+ * s_ij = scale q_i.k_j + table[bucket(pos_j - pos_i)][head]; P = softmax over the keys that exist; out = P v. Tokens are
+ * the positions of an height x width map in row order (a sequence: height 1; several rows: width <= 1024); key j is token j,
+ * query i token q_start + i. Offset (dy, dx) has the number (dy + height-1)(2 width-1) + dx + width-1.
+ * bias[heads][(2 height-1)(2 width-1)] = table[bucket[offset]][head] / scale: made once per table, read by both calls below. */
+int mia_relpos_bias(const float* table, const int* bucket, int height, int width, int heads, float scale, float* bias,
+                    void* stream);
+/* q [B][Lq][heads][D], k, v [B][Lk][heads][D] with element strides {batch, token, head} of q, k, v in that order (HOST array of
+ * 9; every row starts at a multiple of 16 bytes), D a multiple of 8 up to 128. key_mask (nullable): [B][Lk] bytes, 0 = the key
+ * does not exist; a query without keys gives zeros. Dropout as in mia_attention_fwd, on element ((b*heads+h)*Lq+i)*Lk+j.
+ * out: [B][Lq][heads][D] contiguous; stat (nullable): [B][heads][Lq][2], kept for the backward pass (the row's maximum and the
+ * log2 of its sum of exponentials, +inf for a row without keys). ws: mia_relpos_fwd_ws_floats floats (0: none; few queries against many keys
+ * are split over the keys and joined). */
+int mia_relpos_fwd(int dtype, const void* q, const void* k, const void* v, const long long* strides, int B, int heads, int Lq,
+                   int Lk, int D, const float* bias, int height, int width, int q_start, const uint8_t* key_mask, float scale,
+                   float pdrop, unsigned long long seed, const unsigned long long* seed_offset, float* ws,
+                   long long ws_floats, void* out, float* stat, void* stream);
+long long mia_relpos_fwd_ws_floats(int dtype, int B, int heads, int Lq, int Lk, int D);
+/* dout, out: [B][Lq][heads][D] contiguous; dq, dk, dv with their own strides (HOST array of 9); dtable [buckets][heads]
+ * (nullable: not wanted), for which order lists the offsets sorted by bucket and start[buckets + 1] where each bucket's
+ * begin in it. Nothing is added atomically across waves: the same bits every time. */
+int mia_relpos_bwd(int dtype, const void* q, const void* k, const void* v, const long long* strides, const void* dout,
+                   const void* out, const float* stat, int B, int heads, int Lq, int Lk, int D, const float* bias, int height,
+                   int width, int q_start, const uint8_t* key_mask, float scale, float pdrop, unsigned long long seed,
+                   const unsigned long long* seed_offset, const int* order, const int* start, int buckets, float* ws,
+                   long long ws_floats, void* dq, void* dk, void* dv, const long long* grad_strides, float* dtable,
+                   void* stream);
+long long mia_relpos_bwd_ws_floats(int dtype, int B, int heads, int Lq, int Lk, int D, int height, int width, int want_bias);
+
 /* ---- classifier front end: AdaptiveAvgPool2d(1) -> Flatten -> [LayerNorm] -> Dropout (model.py:134-137, :309-311)
  * in_part [B][S][C]: per-image channel sums over H*W (mia_img_colsum). gamma/beta NULL = no LayerNorm. */
 int mia_pool_ln_dropout_fwd(const float* in_part, int B, int S, int HW, int C, const float* gamma, const float* beta,

@@ -3,7 +3,7 @@ csrc/blocknorm.hip."""
 import torch
 
 from ._lib import lib
-from .ops import _DT, _p, _stream
+from .ops import _DT, _p, _stream, on_device
 
 _KINDS = {None: 0, "rms": 1, "layer": 2}
 
@@ -21,7 +21,7 @@ class GatedResidualNormFn(torch.autograd.Function):
         keep = any(ctx.needs_input_grad)
         stats = torch.empty((images * rows, 4), dtype=torch.float32, device=x.device) if keep else None
         if rows:
-            with torch.cuda.device(x.device):
+            with on_device(x.device):
                 lib().mia_blocknorm_fwd(_DT[x.dtype], _p(x), _p(f), images, rows, C, _p(scale), _p(gate), post, _p(w1), _p(b1),
                                         pre, _p(w2), _p(b2), eps, _p(y), _p(z), _p(stats), _stream())
         ctx.meta = (images, rows, C, post, pre)
@@ -40,7 +40,7 @@ class GatedResidualNormFn(torch.autograd.Function):
         dy, dz = (t.contiguous() if t is not None else None for t in (dy, dz))
         nws = lib().mia_blocknorm_ws_floats(images, rows, C, 1 if gate is not None else 0)
         ws = torch.empty((nws,), dtype=torch.float32, device=x.device)
-        with torch.cuda.device(x.device):
+        with on_device(x.device):
             lib().mia_blocknorm_bwd(_DT[x.dtype], _p(dy), _p(dz), _p(x), _p(f), _p(stats), images, rows, C, _p(scale), _p(gate),
                                     post, _p(w1), _p(b1), pre, _p(w2), _p(ws), nws, _p(dx), _p(df), *[_p(g) for g in grads],
                                     _stream())

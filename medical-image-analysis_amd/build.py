@@ -14,7 +14,7 @@ LIB = os.path.join(HERE, "libmia_hip.so")
 # of their forms have given wrong results now and then, without an error. The host pass warns that it does not know the
 # feature, which is harmless.
 HIPFLAGS = ["--offload-arch=gfx950", "-O3", "-fPIC", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-SOURCES = ["runtime.hip", "gemm.hip", "dwconv.hip", "pointwise.hip", "head.hip", "preprocess.hip", "optim.hip", "seg.hip", "metrics.hip", "augment.hip", "blocknorm.hip"]
+SOURCES = ["runtime.hip", "gemm.hip", "dwconv.hip", "pointwise.hip", "head.hip", "preprocess.hip", "optim.hip", "seg.hip", "metrics.hip", "augment.hip", "blocknorm.hip", "relpos.hip"]
 
 
 def kernel_tree_hash() -> str:

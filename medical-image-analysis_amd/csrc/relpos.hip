@@ -1,0 +1,1098 @@
+// Attention with a learned relative position bias, forward and backward (gfx950).
+//
+//   s_ij = scale * q_i . k_j + table[bucket(pos_j - pos_i)][head],  P = softmax over the unmasked keys,  O = P V
+//   dV = P^T dO,  dP = dO V^T,  D_i = sum_j P_ij dP_ij,  dS = P o (dP - D),  dQ = scale dS K,  dK = scale dS^T Q,
+//   dtable[k][head] = sum of dS over the batch and over all pairs whose offset lies in bucket k
+//
+// Tokens are the positions of an H x W map in row order (a sequence is a map of one row). With c(p) = (p / W)(2W - 1) + p % W
+// the offset of a pair is the single number c(j) - c(i): it names (dy, dx) uniquely, so one fp32 vector per head over the
+// (2H - 1)(2W - 1) offsets holds the whole bias. relpos_expand_kernel forms it from the table (divided by scale, because
+// the matrix accumulators start from it: acc = q.k + bias / scale), and a tile of pairs needs only the short window of it
+// that its tokens' c span, which is staged in LDS next to the tile.
+//
+// Matrix cores: S^T = K Q^T with keys as rows leaves a lane of v_mfma_f32_16x16x* four consecutive keys of ONE query: the
+// softmax runs down registers plus two lane exchanges, and the four values are already the B operand of O^T = V^T P^T (V^T
+// read from the row-major tile by the transposing LDS read). fp32 runs the same code on 16x16x4. No L x L array exists in
+// memory; the backward recomputes P from the row statistics, once with queries as columns (dQ) and once with keys as
+// columns (dK, dV, dtable). P and dS are rounded to bf16 only as operands of bf16 products; statistics, D and the bias
+// gradient stay fp32.
+//
+// D is needed to fp32 accuracy because the rows of dS sum to zero and a bucket's gradient is what is left of many terms. The
+// output a bf16 caller holds is too coarse for it. The dQ kernel therefore starts from D~ = dO . out, adds up
+// sum_j P_ij (dP_ij - D~_i) = D_i - D~_i in fp32 on the way, and leaves the exact D for the dK / dV / dtable kernel.
+#include "common.h"
+
+typedef __attribute__((ext_vector_type(4))) float rp_f32x4;
+typedef __attribute__((ext_vector_type(4))) short rp_s16x4;
+typedef __attribute__((ext_vector_type(8))) short rp_s16x8;
+typedef __attribute__((ext_vector_type(8))) __bf16 rp_bf16x8;
+
+#define RP_LOG2E 1.4426950408889634f
+#define RP_TILE 64          // tokens of a staged tile
+#define RP_MAX_WIDTH 1024   // of a map of several rows: bounds the bias window of a tile
+
+struct RpStride {
+    long long b, t, h;   // elements
+};
+struct RpArgs {
+    const void *q, *k, *v, *dout, *out;
+    void *o, *dq, *dk, *dv;
+    RpStride sq, sk, sv, sdq, sdk, sdv;
+    const float* bias;            // [heads][n_off]
+    float2* stat;                 // [B][heads][Lq]: maximum of acc, log2 of the sum of exponentials
+    float* dsum;                  // [B][heads][Lq]
+    const uint8_t* mask;          // [B][Lk], nullable
+    float* slab;                  // dK/dV kernel: [B * heads * key blocks][slab_ld], nullable
+    float *po, *pml;              // split forward: [splits][B * heads * Lq][D], [..][2]
+    int B, heads, Lq, Lk, D, W, pitch, off, n_off, q_start;
+    int tiles, splits, win, acc_mask, slab_ld;
+    float scale, sl2, pdrop;
+    unsigned long long seed;
+    const unsigned long long* seed_off;
+};
+
+__device__ __forceinline__ unsigned long long rp_seed(const RpArgs& a) {
+    return a.seed_off ? a.seed + a.seed_off[0] * 0x9E3779B97F4A7C15ull : a.seed;
+}
+// the same counter-based mask as the other dropout kernels of the library
+__device__ __forceinline__ float rp_drop(unsigned long long seed, unsigned long long idx, float p) {
+    unsigned long long z = idx + seed * 0x9E3779B97F4A7C15ull + 0xD1B54A32D192ED03ull;
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    z = z ^ (z >> 31);
+    const float u = (float)(z >> 40) * (1.0f / 16777216.0f);
+    return u >= p ? 1.0f / (1.0f - p) : 0.f;
+}
+
+__device__ __forceinline__ int rp_c(const RpArgs& a, int p) {
+    const int y = p / a.W;
+    return y * a.pitch + (p - y * a.W);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Matrix operands. A Frag is 16 bytes of one row (8 bf16 or 4 fp32): lane (g = lane / 16, l = lane % 16) holds elements
+// PER * g .. of row l in the current chunk of 4 * PER elements. Both operands of a product use the same assignment of elements
+// to reduction indices, so any assignment is right; this one makes every operand load one 16-byte access.
+// ------------------------------------------------------------------------------------------------
+template <typename T>
+struct RpOp;
+
+template <>
+struct RpOp<bf16_t> {
+    typedef rp_bf16x8 Frag;
+    typedef rp_bf16x8 Pair;    // two 16-row blocks of a D-layout result as one B operand (reduction length 32)
+    typedef rp_bf16x8 TFrag;
+    static constexpr int PER = 8, CHUNK = 32;
+    static __device__ __forceinline__ rp_f32x4 dot(Frag a, Frag b, rp_f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ Pair pack(const rp_f32x4& x, const rp_f32x4& y) {
+        return __builtin_bit_cast(Pair, make_uint4(pack_bf16x2(v2f{x[0], x[1]}), pack_bf16x2(v2f{x[2], x[3]}),
+                                                   pack_bf16x2(v2f{y[0], y[1]}), pack_bf16x2(v2f{y[2], y[3]})));
+    }
+    // A operand of a product over rows: rows ra .. ra+3 and rb .. rb+3 (per 16-lane group) of columns col0 .. col0+15.
+    // ra_ptr / rb_ptr: element [ra][col0] of this lane's group.
+    static __device__ __forceinline__ TFrag load_t(const bf16_t* ra_ptr, const bf16_t* rb_ptr, int ld, int l) {
+        typedef __attribute__((address_space(3))) rp_s16x4 lds4;
+        const int at = (l >> 2) * ld + 4 * (l & 3);
+        const rp_s16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(ra_ptr + at));
+        const rp_s16x4 y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(rb_ptr + at));
+        const rp_s16x8 r = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        return __builtin_bit_cast(TFrag, r);
+    }
+    static __device__ __forceinline__ rp_f32x4 dot_t(const TFrag& a, const Pair& b, rp_f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float inner(Frag a, Frag b) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s = fmaf((float)a[i], (float)b[i], s);
+        return s;
+    }
+};
+
+template <>
+struct RpOp<float> {
+    typedef rp_f32x4 Frag;
+    struct Pair {
+        rp_f32x4 x, y;
+    };
+    typedef Pair TFrag;
+    static constexpr int PER = 4, CHUNK = 16;
+    static __device__ __forceinline__ rp_f32x4 dot(Frag a, Frag b, rp_f32x4 c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ Pair pack(const rp_f32x4& x, const rp_f32x4& y) { return {x, y}; }
+    static __device__ __forceinline__ TFrag load_t(const float* ra_ptr, const float* rb_ptr, int ld, int l) {
+        TFrag r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            r.x[i] = ra_ptr[i * ld + l];
+            r.y[i] = rb_ptr[i * ld + l];
+        }
+        return r;
+    }
+    static __device__ __forceinline__ rp_f32x4 dot_t(const TFrag& a, const Pair& b, rp_f32x4 c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.x[i], b.x[i], c, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.y[i], b.y[i], c, 0, 0, 0);
+        return c;
+    }
+    static __device__ __forceinline__ float inner(Frag a, Frag b) {
+        return fmaf(a[0], b[0], fmaf(a[1], b[1], fmaf(a[2], b[2], a[3] * b[3])));
+    }
+};
+
+template <typename T, int DP>
+struct RpDim {
+    static constexpr int ES = (int)sizeof(T), PER = RpOp<T>::PER;
+    static constexpr int NCH = (DP + RpOp<T>::CHUNK - 1) / RpOp<T>::CHUNK;   // operand chunks of a row
+    static constexpr int LD = NCH * RpOp<T>::CHUNK + PER;                    // LDS row stride: 16 bytes of padding
+    static constexpr int CPR = DP / PER;                                     // 16-byte pieces of a staged row
+    static constexpr int NST = (RP_TILE * CPR + 255) / 256;                  // pieces per thread
+    static constexpr int DB = DP / 16;                                       // 16-wide output blocks
+};
+
+// 16-byte pieces of one row for this lane: elements beyond D are zeros (D is a multiple of 8)
+template <typename T, int DP>
+__device__ __forceinline__ void rp_row_frags(const T* row, bool ok, int D, int g, typename RpOp<T>::Frag (&f)[RpDim<T, DP>::NCH]) {
+    typedef typename RpOp<T>::Frag Frag;
+#pragma unroll
+    for (int s = 0; s < RpDim<T, DP>::NCH; ++s) {
+        const int col = s * RpOp<T>::CHUNK + g * RpOp<T>::PER;
+        f[s] = ok && col < D ? *reinterpret_cast<const Frag*>(row + col) : Frag{};
+    }
+}
+
+// one tile of rows on its way to LDS, kept in registers while the tile before it is worked on
+template <typename T, int DP>
+struct RpTile {
+    uint4 r[RpDim<T, DP>::NST];
+    // rows first .. first + 63 of src (row stride st); bit i of valid clear = row i becomes zeros
+    __device__ __forceinline__ void fetch(const T* src, long long st, int first, unsigned long long valid, int D) {
+        constexpr int CPR = RpDim<T, DP>::CPR;
+#pragma unroll
+        for (int i = 0; i < RpDim<T, DP>::NST; ++i) {
+            const int id = i * 256 + threadIdx.x, row = id / CPR, col = (id - row * CPR) * RpOp<T>::PER;
+            r[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (row < RP_TILE && ((valid >> row) & 1) && col < D)
+                r[i] = *reinterpret_cast<const uint4*>(src + (long long)(first + row) * st + col);
+        }
+    }
+    // INS: extra elements after every 16 rows
+    template <int INS>
+    __device__ __forceinline__ void put(T* lds) const {
+        constexpr int CPR = RpDim<T, DP>::CPR;
+#pragma unroll
+        for (int i = 0; i < RpDim<T, DP>::NST; ++i) {
+            const int id = i * 256 + threadIdx.x, row = id / CPR, col = (id - row * CPR) * RpOp<T>::PER;
+            if (row < RP_TILE) *reinterpret_cast<uint4*>(lds + row * RpDim<T, DP>::LD + (row >> 4) * INS + col) = r[i];
+        }
+    }
+};
+
+// columns between DP and the padded reduction length are read as operands and never staged: zero once
+template <typename T, int DP, int INS>
+__device__ __forceinline__ void rp_zero_pad(T* lds) {
+    constexpr int LD = RpDim<T, DP>::LD, PADC = RpDim<T, DP>::NCH * RpOp<T>::CHUNK - DP;
+    if constexpr (PADC > 0)
+        for (int i = threadIdx.x; i < RP_TILE * PADC; i += 256) {
+            const int row = i / PADC;
+            lds[row * LD + (row >> 4) * INS + DP + (i - row * PADC)] = from_f32<T>(0.f);
+        }
+}
+
+__device__ __forceinline__ float rp_xor_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16));
+    return fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float rp_xor_sum(float v) {
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+
+// A row's statistics for the backward pass: P = exp2((acc - max) * scale * log2(e) - log2(sum)). The maximum is subtracted before
+// anything else, so that rows whose scores are all at the lowest value come out right (their maximum times a constant, rounded,
+// would be off by more than any exponent); a row without keys gets an infinite sum, and so weights of zero.
+__device__ __forceinline__ float2 rp_stat(float m, float total) {
+    return total == 0.f ? make_float2(0.f, INFINITY) : make_float2(m, __builtin_amdgcn_logf(total));
+}
+
+__device__ __forceinline__ unsigned long long rp_valid(const RpArgs& a, int b, int k0) {
+    const int key = k0 + (int)(threadIdx.x & 63);
+    bool ok = key < a.Lk;
+    if (ok && a.mask) ok = a.mask[(size_t)b * a.Lk + key] != 0;
+    return __ballot(ok);
+}
+
+// blocks of one (image, head) stay on one XCD, whose L2 then holds that head's keys and values: consecutive hardware
+// workgroup ids go to the eight XCDs in turn. The grid is a multiple of 8; ids past `total` have nothing to do.
+__device__ __forceinline__ int rp_block(int id, int grid) { return (id & 7) * (grid >> 3) + (id >> 3); }
+
+// ------------------------------------------------------------------------------------------------
+// bias[h][o] = table[bucket[o]][h] / scale. Finite values stay finite (the largest ones are clamped): a table entry at the
+// type's lowest value is a very low score, not a forbidden one.
+// ------------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void relpos_expand_kernel(const float* __restrict__ table, const int* __restrict__ bucket,
+                                                            int n_off, int heads, float inv_scale, float limit,
+                                                            float* __restrict__ bias) {
+    const int o = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y;
+    if (o >= n_off) return;
+    float t = table[(size_t)bucket[o] * heads + h];
+    if (fabsf(t) < INFINITY) t = fminf(fmaxf(t, -limit), limit) * inv_scale;
+    bias[(size_t)h * n_off + o] = t;
+}
+
+// the bias window of one tile on its way to LDS
+struct RpWindow {
+    float r[4];
+    __device__ __forceinline__ void fetch(const float* src, int n) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = i * 256 + (int)threadIdx.x < n ? src[i * 256 + threadIdx.x] : 0.f;
+    }
+    __device__ __forceinline__ void put(float* dst, const float* src, int n) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i * 256 + (int)threadIdx.x < n) dst[i * 256 + threadIdx.x] = r[i];
+        for (int i = 1024 + threadIdx.x; i < n; i += 256) dst[i] = src[i];
+    }
+};
+
+// ------------------------------------------------------------------------------------------------
+// forward: a workgroup owns 64 * QB queries of one (image, head), 16 * QB a wave, and walks the keys in tiles of 64 with the
+// running maximum and sum of a softmax. With several splits (few queries, many keys) it walks one range of the tiles and
+// leaves an unnormalised partial result.
+// ------------------------------------------------------------------------------------------------
+template <typename T, int DP, int QB>
+__global__ __launch_bounds__(256) void relpos_fwd_kernel(RpArgs a) {
+    typedef RpOp<T> Op;
+    typedef RpDim<T, DP> Dim;
+    constexpr int LD = Dim::LD, QT = 64 * QB;
+    extern __shared__ __attribute__((aligned(16))) char rp_sm[];
+    T* Ks = reinterpret_cast<T*>(rp_sm);
+    T* Vs = Ks + RP_TILE * LD;
+    int* ck = reinterpret_cast<int*>(Vs + RP_TILE * LD);
+    float* bw = reinterpret_cast<float*>(ck + RP_TILE);
+    const int qtiles = (a.Lq + QT - 1) / QT, id = rp_block(blockIdx.x, gridDim.x);
+    if (id >= a.B * a.heads * qtiles) return;
+    const int bh = id / qtiles, b = bh / a.heads, h = bh - b * a.heads, q0 = (id - bh * qtiles) * QT;
+    const int t0 = (int)((long long)a.tiles * blockIdx.y / a.splits), t1 = (int)((long long)a.tiles * (blockIdx.y + 1) / a.splits);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const T* kp = (const T*)a.k + b * a.sk.b + h * a.sk.h;
+    const T* vp = (const T*)a.v + b * a.sv.b + h * a.sv.h;
+    const float* bias = a.bias + (size_t)h * a.n_off;
+    const int q_hi = min(q0 + QT, a.Lq) - 1;
+    const int cq_lo = rp_c(a, a.q_start + q0), cq_hi = rp_c(a, a.q_start + q_hi);
+
+    typename Op::Frag qf[QB][Dim::NCH];
+    int qi[QB], cq[QB];
+    float m[QB], sum[QB];
+    rp_f32x4 o[QB][Dim::DB];
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+        qi[i] = q0 + (wave * QB + i) * 16 + l;
+        cq[i] = rp_c(a, a.q_start + min(qi[i], q_hi)) - cq_hi;
+        rp_row_frags<T, DP>((const T*)a.q + b * a.sq.b + (long long)min(qi[i], q_hi) * a.sq.t + h * a.sq.h, qi[i] < a.Lq, a.D, g, qf[i]);
+        m[i] = -INFINITY;
+        sum[i] = 0.f;
+#pragma unroll
+        for (int d = 0; d < Dim::DB; ++d) o[i][d] = rp_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const bool idle = q0 + wave * QB * 16 >= a.Lq;   // a wave without queries only helps to stage
+    const unsigned long long seed = a.pdrop > 0.f ? rp_seed(a) : 0ull;
+    rp_zero_pad<T, DP, 0>(Ks);
+
+    RpTile<T, DP> kt, vt;
+    RpWindow wt;
+    unsigned long long valid = 0ull, next = 0ull;
+    int ck_lo = 0, n_win = 0, base = 0;
+    auto fetch = [&](int t) {
+        const int k0 = t * RP_TILE;
+        next = rp_valid(a, b, k0);
+        kt.fetch(kp, a.sk.t, k0, next, a.D);
+        vt.fetch(vp, a.sv.t, k0, next, a.D);
+        ck_lo = rp_c(a, k0);
+        base = ck_lo - cq_hi + a.off;
+        n_win = rp_c(a, min(k0 + RP_TILE, a.Lk) - 1) - ck_lo + cq_hi - cq_lo + 1;
+        wt.fetch(bias + base, n_win);
+    };
+    if (t0 < t1) fetch(t0);
+    for (int t = t0; t < t1; ++t) {
+        __syncthreads();
+        kt.template put<0>(Ks);
+        vt.template put<0>(Vs);
+        wt.put(bw, bias + base, n_win);
+        if (threadIdx.x < RP_TILE) ck[threadIdx.x] = rp_c(a, min(t * RP_TILE + (int)threadIdx.x, a.Lk - 1)) - ck_lo;
+        valid = next;
+        __syncthreads();
+        if (t + 1 < t1) fetch(t + 1);
+        if (idle || valid == 0ull) continue;
+        rp_f32x4 s[4][QB];
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+            const int4 c4 = *reinterpret_cast<const int4*>(ck + kb * 16 + g * 4);
+#pragma unroll
+            for (int i = 0; i < QB; ++i) {
+                s[kb][i] = rp_f32x4{bw[c4.x - cq[i]], bw[c4.y - cq[i]], bw[c4.z - cq[i]], bw[c4.w - cq[i]]};
+            }
+#pragma unroll
+            for (int c = 0; c < Dim::NCH; ++c) {
+                const typename Op::Frag kf = *reinterpret_cast<const typename Op::Frag*>(Ks + (kb * 16 + l) * LD + c * Op::CHUNK + g * Op::PER);
+#pragma unroll
+                for (int i = 0; i < QB; ++i) s[kb][i] = Op::dot(kf, qf[i][c], s[kb][i]);
+            }
+            if (valid != ~0ull) {
+                const unsigned bits = (unsigned)(valid >> (kb * 16 + g * 4));
+#pragma unroll
+                for (int i = 0; i < QB; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (!((bits >> r) & 1)) s[kb][i][r] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < QB; ++i) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[kb][i][r]);
+            mx = fmaxf(m[i], rp_xor_max(mx));
+            const float use = mx == -INFINITY ? 0.f : mx;
+            if (__any(mx > m[i])) {
+                const float alpha = __builtin_amdgcn_exp2f((m[i] - use) * a.sl2);
+                sum[i] *= alpha;
+#pragma unroll
+                for (int d = 0; d < Dim::DB; ++d) o[i][d] *= alpha;
+            }
+            m[i] = mx;
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float p = __builtin_amdgcn_exp2f((s[kb][i][r] - use) * a.sl2);
+                    sum[i] += p;
+                    s[kb][i][r] = p;
+                }
+            if (a.pdrop > 0.f) {
+                const unsigned long long at = ((unsigned long long)bh * a.Lq + qi[i]) * a.Lk + t * RP_TILE + g * 4;
+#pragma unroll
+                for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[kb][i][r] *= rp_drop(seed, at + kb * 16 + r, a.pdrop);
+            }
+        }
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            typename Op::Pair p[QB];
+#pragma unroll
+            for (int i = 0; i < QB; ++i) p[i] = Op::pack(s[2 * kk][i], s[2 * kk + 1][i]);
+#pragma unroll
+            for (int d = 0; d < Dim::DB; ++d) {
+                const T* v0 = Vs + (kk * 32 + g * 4) * LD + d * 16;
+                const typename Op::TFrag vf = Op::load_t(v0, v0 + 16 * LD, LD, l);
+#pragma unroll
+                for (int i = 0; i < QB; ++i) o[i][d] = Op::dot_t(vf, p[i], o[i][d]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+        const float total = rp_xor_sum(sum[i]);
+        if (qi[i] >= a.Lq) continue;
+        const size_t row = (size_t)bh * a.Lq + qi[i];
+        if (a.splits > 1) {
+            const size_t prow = (size_t)blockIdx.y * a.B * a.heads * a.Lq + row;
+            if (g == 0) {
+                a.pml[2 * prow] = m[i];
+                a.pml[2 * prow + 1] = total;
+            }
+#pragma unroll
+            for (int d = 0; d < Dim::DB; ++d) {
+                const int col = d * 16 + g * 4;
+                if (col < a.D) *reinterpret_cast<rp_f32x4*>(a.po + prow * a.D + col) = o[i][d];
+            }
+            continue;
+        }
+        const float inv = total == 0.f ? 0.f : 1.0f / total;   // a row without keys is zero
+        if (a.stat && g == 0) a.stat[row] = rp_stat(m[i], total);
+        T* op = (T*)a.o + (((size_t)b * a.Lq + qi[i]) * a.heads + h) * a.D;
+#pragma unroll
+        for (int d = 0; d < Dim::DB; ++d) {
+            const int col = d * 16 + g * 4;
+            if (col < a.D) store4<T>(op + col, {o[i][d][0] * inv, o[i][d][1] * inv, o[i][d][2] * inv, o[i][d][3] * inv});
+        }
+    }
+}
+
+// joins the partial results of a split forward: one workgroup of D threads a row
+template <typename T>
+__global__ void relpos_join_kernel(RpArgs a) {
+    const size_t rows = (size_t)a.B * a.heads * a.Lq, row = blockIdx.x;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.pml[2 * (s * rows + row)]);
+    const float use = m == -INFINITY ? 0.f : m;
+    float total = 0.f, acc = 0.f;
+    const int d = threadIdx.x;
+    for (int s = 0; s < a.splits; ++s) {
+        const size_t p = s * rows + row;
+        const float w = __builtin_amdgcn_exp2f((a.pml[2 * p] - use) * a.sl2);
+        total = fmaf(a.pml[2 * p + 1], w, total);
+        if (d < a.D) acc = fmaf(a.po[p * a.D + d], w, acc);
+    }
+    const size_t bh = row / a.Lq, b = bh / a.heads, h = bh - b * a.heads, q = row - bh * a.Lq;
+    if (d < a.D) ((T*)a.o)[((b * a.Lq + q) * a.heads + h) * a.D + d] = from_f32<T>(total == 0.f ? 0.f : acc / total);
+    if (a.stat && d == 0) a.stat[row] = rp_stat(m, total);
+}
+
+// ------------------------------------------------------------------------------------------------
+// backward, queries as columns: dQ and the exact D. The same walk as the forward.
+// ------------------------------------------------------------------------------------------------
+template <typename T, int DP, int QB>
+__global__ __launch_bounds__(256) void relpos_bwd_q_kernel(RpArgs a) {
+    typedef RpOp<T> Op;
+    typedef RpDim<T, DP> Dim;
+    constexpr int LD = Dim::LD, QT = 64 * QB;
+    extern __shared__ __attribute__((aligned(16))) char rp_sm[];
+    T* Ks = reinterpret_cast<T*>(rp_sm);
+    T* Vs = Ks + RP_TILE * LD;
+    int* ck = reinterpret_cast<int*>(Vs + RP_TILE * LD);
+    float* bw = reinterpret_cast<float*>(ck + RP_TILE);
+    const int qtiles = (a.Lq + QT - 1) / QT, id = rp_block(blockIdx.x, gridDim.x);
+    if (id >= a.B * a.heads * qtiles) return;
+    const int bh = id / qtiles, b = bh / a.heads, h = bh - b * a.heads, q0 = (id - bh * qtiles) * QT;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const T* kp = (const T*)a.k + b * a.sk.b + h * a.sk.h;
+    const T* vp = (const T*)a.v + b * a.sv.b + h * a.sv.h;
+    const float* bias = a.bias + (size_t)h * a.n_off;
+    const int q_hi = min(q0 + QT, a.Lq) - 1;
+    const int cq_lo = rp_c(a, a.q_start + q0), cq_hi = rp_c(a, a.q_start + q_hi);
+
+    typename Op::Frag qf[QB][Dim::NCH], gf[QB][Dim::NCH];
+    int qi[QB], cq[QB];
+    float mx[QB], lg[QB], D0[QB], extra[QB];
+    rp_f32x4 dq[QB][Dim::DB];
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+        qi[i] = q0 + (wave * QB + i) * 16 + l;
+        const int row = min(qi[i], q_hi);
+        const bool ok = qi[i] < a.Lq;
+        cq[i] = rp_c(a, a.q_start + row) - cq_hi;
+        rp_row_frags<T, DP>((const T*)a.q + b * a.sq.b + (long long)row * a.sq.t + h * a.sq.h, ok, a.D, g, qf[i]);
+        const size_t orow = (((size_t)b * a.Lq + row) * a.heads + h) * a.D;
+        typename Op::Frag of[Dim::NCH];
+        rp_row_frags<T, DP>((const T*)a.dout + orow, ok, a.D, g, gf[i]);
+        rp_row_frags<T, DP>((const T*)a.out + orow, ok, a.D, g, of);
+        float d = 0.f;
+#pragma unroll
+        for (int c = 0; c < Dim::NCH; ++c) d += Op::inner(gf[i][c], of[c]);
+        D0[i] = rp_xor_sum(d);
+        const float2 st = a.stat[(size_t)bh * a.Lq + row];
+        mx[i] = st.x;
+        lg[i] = ok ? st.y : INFINITY;
+        extra[i] = 0.f;
+#pragma unroll
+        for (int c = 0; c < Dim::DB; ++c) dq[i][c] = rp_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    const bool idle = q0 + wave * QB * 16 >= a.Lq;
+    const unsigned long long seed = a.pdrop > 0.f ? rp_seed(a) : 0ull;
+    rp_zero_pad<T, DP, 0>(Ks);
+    rp_zero_pad<T, DP, 0>(Vs);
+
+    RpTile<T, DP> kt, vt;
+    RpWindow wt;
+    unsigned long long valid = 0ull, next = 0ull;
+    int ck_lo = 0, n_win = 0, base = 0;
+    auto fetch = [&](int t) {
+        const int k0 = t * RP_TILE;
+        next = rp_valid(a, b, k0);
+        kt.fetch(kp, a.sk.t, k0, next, a.D);
+        vt.fetch(vp, a.sv.t, k0, next, a.D);
+        ck_lo = rp_c(a, k0);
+        base = ck_lo - cq_hi + a.off;
+        n_win = rp_c(a, min(k0 + RP_TILE, a.Lk) - 1) - ck_lo + cq_hi - cq_lo + 1;
+        wt.fetch(bias + base, n_win);
+    };
+    fetch(0);
+    for (int t = 0; t < a.tiles; ++t) {
+        __syncthreads();
+        kt.template put<0>(Ks);
+        vt.template put<0>(Vs);
+        wt.put(bw, bias + base, n_win);
+        if (threadIdx.x < RP_TILE) ck[threadIdx.x] = rp_c(a, min(t * RP_TILE + (int)threadIdx.x, a.Lk - 1)) - ck_lo;
+        valid = next;
+        __syncthreads();
+        if (t + 1 < a.tiles) fetch(t + 1);
+        if (idle || valid == 0ull) continue;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            rp_f32x4 ds[2][QB];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int kb = 2 * kk + e;
+                const int4 c4 = *reinterpret_cast<const int4*>(ck + kb * 16 + g * 4);
+                rp_f32x4 s[QB], dp[QB];
+#pragma unroll
+                for (int i = 0; i < QB; ++i) {
+                    s[i] = rp_f32x4{bw[c4.x - cq[i]], bw[c4.y - cq[i]], bw[c4.z - cq[i]], bw[c4.w - cq[i]]};
+                    dp[i] = rp_f32x4{0.f, 0.f, 0.f, 0.f};
+                }
+#pragma unroll
+                for (int c = 0; c < Dim::NCH; ++c) {
+                    const int at = (kb * 16 + l) * LD + c * Op::CHUNK + g * Op::PER;
+                    const typename Op::Frag kf = *reinterpret_cast<const typename Op::Frag*>(Ks + at);
+                    const typename Op::Frag vf = *reinterpret_cast<const typename Op::Frag*>(Vs + at);
+#pragma unroll
+                    for (int i = 0; i < QB; ++i) {
+                        s[i] = Op::dot(kf, qf[i][c], s[i]);
+                        dp[i] = Op::dot(vf, gf[i][c], dp[i]);
+                    }
+                }
+                if (valid != ~0ull) {
+                    const unsigned bits = (unsigned)(valid >> (kb * 16 + g * 4));
+#pragma unroll
+                    for (int i = 0; i < QB; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (!((bits >> r) & 1)) s[i][r] = -INFINITY;
+                }
+#pragma unroll
+                for (int i = 0; i < QB; ++i) {
+                    if (a.pdrop > 0.f) {
+                        const unsigned long long at = ((unsigned long long)bh * a.Lq + qi[i]) * a.Lk + t * RP_TILE + kb * 16 + g * 4;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) dp[i][r] *= rp_drop(seed, at + r, a.pdrop);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float p = __builtin_amdgcn_exp2f(fmaf(s[i][r] - mx[i], a.sl2, -lg[i]));
+                        const float d = p * (dp[i][r] - D0[i]);
+                        extra[i] += d;
+                        ds[e][i][r] = d;
+                    }
+                }
+            }
+            typename Op::Pair p[QB];
+#pragma unroll
+            for (int i = 0; i < QB; ++i) p[i] = Op::pack(ds[0][i], ds[1][i]);
+#pragma unroll
+            for (int d = 0; d < Dim::DB; ++d) {
+                const T* k0 = Ks + (kk * 32 + g * 4) * LD + d * 16;
+                const typename Op::TFrag kf = Op::load_t(k0, k0 + 16 * LD, LD, l);
+#pragma unroll
+                for (int i = 0; i < QB; ++i) dq[i][d] = Op::dot_t(kf, p[i], dq[i][d]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+        const float Di = D0[i] + rp_xor_sum(extra[i]);
+        if (qi[i] >= a.Lq) continue;
+        if (g == 0) a.dsum[(size_t)bh * a.Lq + qi[i]] = Di;
+        T* out = (T*)a.dq + b * a.sdq.b + (long long)qi[i] * a.sdq.t + h * a.sdq.h;
+#pragma unroll
+        for (int d = 0; d < Dim::DB; ++d) {
+            const int col = d * 16 + g * 4;
+            if (col < a.D)
+                store4<T>(out + col, {dq[i][d][0] * a.scale, dq[i][d][1] * a.scale, dq[i][d][2] * a.scale, dq[i][d][3] * a.scale});
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// backward, keys as columns: dK, dV and the bias gradient per offset. A workgroup owns 64 * KB keys of one (image, head), 16 *
+// KB a wave, whose K and V operands stay in registers, and walks the queries in tiles of 64.
+//
+// Row a = 4 g + r of the m-th 16-row block of a tile is query 16 g + 4 m + r. In register r of a block the 64 lanes then hold
+// four queries 16 apart against 16 consecutive keys: 64 different token distances, hence 64 different offsets. So one LDS
+// add instruction never meets an address twice, and each wave adds its dS into an accumulator array of its OWN: the additions
+// to one address come from one wave in program order, and the result does not depend on timing. The array is a ring over the
+// offsets; offsets that later tiles cannot reach any more (queries only go up, so offsets only go down) are added over
+// the waves in wave order and leave for the slab after every tile.
+// ------------------------------------------------------------------------------------------------
+template <typename T, int DP, int KB>
+__global__ __launch_bounds__(256) void relpos_bwd_kv_kernel(RpArgs a) {
+    typedef RpOp<T> Op;
+    typedef RpDim<T, DP> Dim;
+    constexpr int LD = Dim::LD, KT = 64 * KB;
+    constexpr int INS = 64 / (int)sizeof(T);   // 16 rows apart = 64 bytes further in the banks: the transposing reads' four row groups
+    constexpr int TILE = RP_TILE * LD + 4 * INS;
+    extern __shared__ __attribute__((aligned(16))) char rp_sm[];
+    T* Qs = reinterpret_cast<T*>(rp_sm);
+    T* Gs = Qs + TILE;
+    float* ms = reinterpret_cast<float*>(Gs + TILE);
+    float* ls = ms + RP_TILE;
+    float* dsm = ls + RP_TILE;
+    int* cqs = reinterpret_cast<int*>(dsm + RP_TILE);
+    float* bw = reinterpret_cast<float*>(cqs + RP_TILE);   // ring, acc_mask + 1 floats
+    const int ring = a.acc_mask + 1;
+    float* acc = bw + ring;                                // [4 waves][ring]
+    const int ktiles = (a.Lk + KT - 1) / KT, id = rp_block(blockIdx.x, gridDim.x);
+    if (id >= a.B * a.heads * ktiles) return;
+    const int bh = id / ktiles, b = bh / a.heads, h = bh - b * a.heads, k0 = (id - bh * ktiles) * KT;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const T* qp = (const T*)a.q + b * a.sq.b + h * a.sq.h;
+    const T* gp = (const T*)a.dout + ((size_t)b * a.Lq * a.heads + h) * a.D;
+    const long long gst = (long long)a.heads * a.D;
+    const float* bias = a.bias + (size_t)h * a.n_off;
+    const float2* stat = a.stat + (size_t)bh * a.Lq;
+    const float* dsum = a.dsum + (size_t)bh * a.Lq;
+    const int k_hi = min(k0 + KT, a.Lk) - 1;
+    const int ck_lo = rp_c(a, k0) + a.off, ck_hi = rp_c(a, k_hi) + a.off;   // offset of a pair = this - c(query)
+    const bool grad_bias = a.slab != nullptr;
+    float* slab = grad_bias ? a.slab + (size_t)id * a.slab_ld : nullptr;
+    const int slab_lo = ck_lo - rp_c(a, a.q_start + a.Lq - 1);
+    float* mine = acc + wave * ring;
+
+    typename Op::Frag kf[KB][Dim::NCH], vf[KB][Dim::NCH];
+    int key[KB], ck[KB];
+    bool ok[KB], any_bad = false, any_ok = false;
+    rp_f32x4 dk[KB][Dim::DB], dv[KB][Dim::DB];
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+        key[j] = k0 + (wave * KB + j) * 16 + l;
+        const int row = min(key[j], k_hi);
+        ok[j] = key[j] < a.Lk && (!a.mask || a.mask[(size_t)b * a.Lk + row] != 0);
+        any_bad |= !ok[j];
+        any_ok |= ok[j];
+        ck[j] = rp_c(a, row) + a.off;
+        rp_row_frags<T, DP>((const T*)a.k + b * a.sk.b + (long long)row * a.sk.t + h * a.sk.h, ok[j], a.D, g, kf[j]);
+        rp_row_frags<T, DP>((const T*)a.v + b * a.sv.b + (long long)row * a.sv.t + h * a.sv.h, ok[j], a.D, g, vf[j]);
+#pragma unroll
+        for (int d = 0; d < Dim::DB; ++d) dk[j][d] = dv[j][d] = rp_f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    any_bad = __any(any_bad);
+    any_ok = __any(any_ok);
+    const unsigned long long seed = a.pdrop > 0.f ? rp_seed(a) : 0ull;
+    rp_zero_pad<T, DP, INS>(Qs);
+    rp_zero_pad<T, DP, INS>(Gs);
+    if (grad_bias)
+        for (int i = threadIdx.x; i < 4 * ring; i += 256) acc[i] = 0.f;
+
+    // offsets (from, to] leave the ring for the slab
+    auto flush = [&](int from, int to) {
+        for (int i = from + 1 + (int)threadIdx.x; i <= to; i += 256) {
+            float* p = acc + (i & a.acc_mask);
+            const float v = (p[0] + p[ring]) + (p[2 * ring] + p[3 * ring]);
+            p[0] = p[ring] = p[2 * ring] = p[3 * ring] = 0.f;
+            slab[i - slab_lo] = v;
+        }
+    };
+
+    RpTile<T, DP> qt, gt;
+    float2 sr = make_float2(0.f, 0.f);
+    float dr = 0.f;
+    const int qtiles = (a.Lq + RP_TILE - 1) / RP_TILE;
+    auto fetch = [&](int t) {
+        const int first = t * RP_TILE, left = a.Lq - first;
+        const unsigned long long rows = left >= 64 ? ~0ull : (1ull << left) - 1;
+        qt.fetch(qp, a.sq.t, first, rows, a.D);
+        gt.fetch(gp, gst, first, rows, a.D);
+        if (threadIdx.x < RP_TILE) {
+            const bool in = (int)threadIdx.x < left;
+            sr = in ? stat[first + threadIdx.x] : make_float2(0.f, INFINITY);
+            dr = in ? dsum[first + threadIdx.x] : 0.f;
+        }
+    };
+    fetch(0);
+    int top = ck_hi - rp_c(a, a.q_start);   // highest offset still in the ring
+    for (int t = 0; t < qtiles; ++t) {
+        const int first = t * RP_TILE, q_hi = min(first + RP_TILE, a.Lq) - 1;
+        const int cq_lo = rp_c(a, a.q_start + first), cq_hi = rp_c(a, a.q_start + q_hi);
+        __syncthreads();
+        if (grad_bias) {
+            const int reach = ck_hi - cq_lo;
+            flush(reach, top);
+            top = reach;
+        }
+        qt.template put<INS>(Qs);
+        gt.template put<INS>(Gs);
+        for (int i = ck_lo - cq_hi + (int)threadIdx.x; i <= ck_hi - cq_lo; i += 256) bw[i & a.acc_mask] = bias[i];
+        if (threadIdx.x < RP_TILE) {
+            ms[threadIdx.x] = sr.x;
+            ls[threadIdx.x] = sr.y;
+            dsm[threadIdx.x] = dr;
+            cqs[threadIdx.x] = rp_c(a, a.q_start + min(first + (int)threadIdx.x, q_hi));
+        }
+        __syncthreads();
+        if (t + 1 < qtiles) fetch(t + 1);
+        if (!any_ok) continue;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            rp_f32x4 p[2][KB], ds[2][KB];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int mb = 2 * kk + e;
+                const int4 c4 = *reinterpret_cast<const int4*>(cqs + g * 16 + mb * 4);
+                const rp_f32x4 m4 = *reinterpret_cast<const rp_f32x4*>(ms + g * 16 + mb * 4);
+                const rp_f32x4 l4 = *reinterpret_cast<const rp_f32x4*>(ls + g * 16 + mb * 4);
+                const rp_f32x4 d4 = *reinterpret_cast<const rp_f32x4*>(dsm + g * 16 + mb * 4);
+                const int cr[4] = {c4.x, c4.y, c4.z, c4.w};
+                int at[KB][4];
+#pragma unroll
+                for (int j = 0; j < KB; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        at[j][r] = (ck[j] - cr[r]) & a.acc_mask;
+                        p[e][j][r] = bw[at[j][r]];
+                        ds[e][j][r] = 0.f;
+                    }
+                const int arow = (l >> 2) * (16 * LD + INS) + (mb * 4 + (l & 3)) * LD;
+#pragma unroll
+                for (int c = 0; c < Dim::NCH; ++c) {
+                    const typename Op::Frag qf = *reinterpret_cast<const typename Op::Frag*>(Qs + arow + c * Op::CHUNK + g * Op::PER);
+                    const typename Op::Frag gf = *reinterpret_cast<const typename Op::Frag*>(Gs + arow + c * Op::CHUNK + g * Op::PER);
+#pragma unroll
+                    for (int j = 0; j < KB; ++j) {
+                        p[e][j] = Op::dot(qf, kf[j][c], p[e][j]);
+                        ds[e][j] = Op::dot(gf, vf[j][c], ds[e][j]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < KB; ++j) {
+                    if (any_bad && !ok[j]) p[e][j] = rp_f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    float keep[4] = {1.f, 1.f, 1.f, 1.f};
+                    if (a.pdrop > 0.f) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            keep[r] = rp_drop(seed, ((unsigned long long)bh * a.Lq + first + g * 16 + mb * 4 + r) * a.Lk + key[j], a.pdrop);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float w = __builtin_amdgcn_exp2f(fmaf(p[e][j][r] - m4[r], a.sl2, -l4[r]));
+                        ds[e][j][r] = w * (ds[e][j][r] * keep[r] - d4[r]);
+                        p[e][j][r] = w * keep[r];
+                    }
+                    if (grad_bias) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            __hip_atomic_fetch_add(mine + at[j][r], ds[e][j][r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    }
+                }
+            }
+            typename Op::Pair pp[KB], pd[KB];
+#pragma unroll
+            for (int j = 0; j < KB; ++j) {
+                pp[j] = Op::pack(p[0][j], p[1][j]);
+                pd[j] = Op::pack(ds[0][j], ds[1][j]);
+            }
+            const int trow = g * (16 * LD + INS) + kk * 8 * LD;
+#pragma unroll
+            for (int d = 0; d < Dim::DB; ++d) {
+                const typename Op::TFrag qa = Op::load_t(Qs + trow + d * 16, Qs + trow + 4 * LD + d * 16, LD, l);
+                const typename Op::TFrag ga = Op::load_t(Gs + trow + d * 16, Gs + trow + 4 * LD + d * 16, LD, l);
+#pragma unroll
+                for (int j = 0; j < KB; ++j) {
+                    dk[j][d] = Op::dot_t(qa, pd[j], dk[j][d]);
+                    dv[j][d] = Op::dot_t(ga, pp[j], dv[j][d]);
+                }
+            }
+        }
+    }
+    if (grad_bias) {
+        __syncthreads();
+        flush(slab_lo - 1, top);
+    }
+#pragma unroll
+    for (int j = 0; j < KB; ++j) {
+        if (key[j] >= a.Lk) continue;
+        T* kd = (T*)a.dk + b * a.sdk.b + (long long)key[j] * a.sdk.t + h * a.sdk.h;
+        T* vd = (T*)a.dv + b * a.sdv.b + (long long)key[j] * a.sdv.t + h * a.sdv.h;
+#pragma unroll
+        for (int d = 0; d < Dim::DB; ++d) {
+            const int col = d * 16 + g * 4;
+            if (col >= a.D) continue;
+            if (ok[j]) {
+                store4<T>(kd + col, {dk[j][d][0] * a.scale, dk[j][d][1] * a.scale, dk[j][d][2] * a.scale, dk[j][d][3] * a.scale});
+                store4<T>(vd + col, {dv[j][d][0], dv[j][d][1], dv[j][d][2], dv[j][d][3]});
+            } else {   // a masked key has no gradient, whatever its own values are
+                store4<T>(kd + col, {0.f, 0.f, 0.f, 0.f});
+                store4<T>(vd + col, {0.f, 0.f, 0.f, 0.f});
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// bias gradient: offsets over images and key blocks, then buckets over their offsets (the offsets of bucket k are
+// order[start[k]] .. order[start[k + 1] - 1]). Fixed order everywhere.
+// ------------------------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void relpos_offsets_kernel(const float* __restrict__ slab, RpArgs a, int ktiles, int kt,
+                                                             float* __restrict__ per_off) {
+    __shared__ float sm[4][64];
+    const int col = threadIdx.x & 63, part = threadIdx.x >> 6, o = blockIdx.x * 64 + col, h = blockIdx.y;
+    const int c_last = rp_c(a, a.q_start + a.Lq - 1), c_first = rp_c(a, a.q_start);
+    float v = 0.f;
+    if (o < a.n_off)
+        for (int i = part; i < a.B * ktiles; i += 4) {
+            const int b = i / ktiles, kb = i - b * ktiles, k0 = kb * kt;
+            const int lo = rp_c(a, k0) + a.off - c_last, hi = rp_c(a, min(k0 + kt, a.Lk) - 1) + a.off - c_first;
+            if (o >= lo && o <= hi) v += slab[((size_t)(b * a.heads + h) * ktiles + kb) * a.slab_ld + (o - lo)];
+        }
+    sm[part][col] = v;
+    __syncthreads();
+    if (part == 0 && o < a.n_off) per_off[(size_t)h * a.n_off + o] = (sm[0][col] + sm[1][col]) + (sm[2][col] + sm[3][col]);
+}
+
+__global__ __launch_bounds__(256) void relpos_buckets_kernel(const float* __restrict__ per_off, int n_off, int heads,
+                                                             const int* __restrict__ order, const int* __restrict__ start,
+                                                             float* __restrict__ dtable) {
+    __shared__ float sm[4];
+    const int k = blockIdx.x, h = blockIdx.y;
+    float v = 0.f;
+    for (int i = start[k] + threadIdx.x; i < start[k + 1]; i += 256) v += per_off[(size_t)h * n_off + order[i]];
+    v = wave_sum(v);
+    if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) dtable[(size_t)k * heads + h] = (sm[0] + sm[1]) + (sm[2] + sm[3]);
+}
+
+// ------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------
+// largest difference of c between two of n consecutive tokens
+static int rp_span(const RpArgs& a, int n, int tokens) {
+    if (n > tokens) n = tokens;
+    if (n <= 1) return 0;
+    const int wraps = a.pitch == 0 || tokens <= a.W ? 0 : (n - 1 + a.W - 1) / a.W;
+    return (n - 1) + wraps * (a.W - 1);
+}
+
+static int rp_dp(int D) { return D <= 16 ? 16 : D <= 32 ? 32 : D <= 48 ? 48 : D <= 64 ? 64 : D <= 96 ? 96 : 128; }
+
+static int rp_ld(int dtype, int DP) {   // RpDim::LD
+    const int chunk = dtype == MIA_BF16 ? 32 : 16;
+    return (DP + chunk - 1) / chunk * chunk + chunk / 4;
+}
+static size_t rp_es(int dtype) { return dtype == MIA_BF16 ? 2 : 4; }
+
+// Queries / keys of a workgroup: 128 (two 16-wide columns a wave: each operand read from LDS serves both) when that still gives
+// two workgroups a CU, else 64. fp32 keeps 64: its operands are twice as large.
+static int rp_cols(int dtype, int DP, long long bh, int L, int max_dp) {
+    if (dtype == MIA_F32 || DP > max_dp) return 1;
+    return bh * ((L + 127) / 128) >= 512 ? 2 : 1;
+}
+static int rp_kv_cols(int dtype, int D, long long bh, int Lk) { return rp_cols(dtype, rp_dp(D), bh, Lk, 64); }
+
+// key ranges of a forward with few workgroups: enough of them for two workgroups a CU, at least four tiles each
+static int rp_splits(long long wgs, int tiles) {
+    if (wgs >= 256 || tiles < 8) return 1;
+    long long s = (512 + wgs - 1) / wgs;
+    if (s > tiles / 4) s = tiles / 4;
+    return s < 1 ? 1 : (int)(s > 64 ? 64 : s);
+}
+static int rp_fwd_splits(int dtype, int B, int heads, int Lq, int Lk, int D, int& cols) {
+    const long long bh = (long long)B * heads;
+    cols = rp_cols(dtype, rp_dp(D), bh, Lq, 128);
+    return rp_splits(bh * ((Lq + 64 * cols - 1) / (64 * cols)), (Lk + RP_TILE - 1) / RP_TILE);
+}
+
+template <typename K>
+static int rp_launch(const char* name, K kernel, dim3 grid, size_t lds, const RpArgs& a, hipStream_t s) {
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        MIA_CHECK_ARG(e == hipSuccess, "%s: %zu bytes of LDS refused: %s", name, lds, hipGetErrorString(e));
+    }
+    MIA_LAUNCH(kernel, grid, dim3(256), lds, s, a);
+    MIA_CHECK_LAUNCH(name);
+    return 0;
+}
+
+enum { RP_FWD, RP_BWD_Q, RP_BWD_KV };
+
+template <typename T, int DP, int COLS>
+static int rp_run(int what, const char* name, dim3 grid, size_t lds, const RpArgs& a, hipStream_t s) {
+    if (what == RP_FWD) return rp_launch(name, relpos_fwd_kernel<T, DP, COLS>, grid, lds, a, s);
+    if constexpr (COLS == 1 || DP <= 64) {
+        if (what == RP_BWD_Q) return rp_launch(name, relpos_bwd_q_kernel<T, DP, COLS>, grid, lds, a, s);
+        return rp_launch(name, relpos_bwd_kv_kernel<T, DP, COLS>, grid, lds, a, s);
+    }
+    mia_set_error("%s: dispatch failed", name);
+    return -1;
+}
+
+static int rp_dispatch(int what, const char* name, int dtype, int cols, dim3 grid, size_t lds, const RpArgs& a, hipStream_t s) {
+#define RP_CASE(DP_)                                                                                      \
+    case DP_:                                                                                             \
+        if (dtype == MIA_F32) return rp_run<float, DP_, 1>(what, name, grid, lds, a, s);                  \
+        return cols == 2 ? rp_run<bf16_t, DP_, 2>(what, name, grid, lds, a, s)                            \
+                         : rp_run<bf16_t, DP_, 1>(what, name, grid, lds, a, s);
+    switch (rp_dp(a.D)) {
+        RP_CASE(16)
+        RP_CASE(32)
+        RP_CASE(48)
+        RP_CASE(64)
+        RP_CASE(96)
+        RP_CASE(128)
+    }
+#undef RP_CASE
+    return -1;
+}
+
+static dim3 rp_grid(long long blocks, int splits) { return dim3((unsigned)((blocks + 7) / 8 * 8), (unsigned)splits); }
+
+static int rp_checks(const char* name, int dtype, int B, int heads, int Lq, int Lk, int D, int height, int width, int q_start,
+                     float scale, float pdrop) {
+    MIA_CHECK_ARG(dtype == MIA_F32 || dtype == MIA_BF16, "%s: bad dtype %d", name, dtype);
+    MIA_CHECK_ARG(B > 0 && heads > 0 && Lq > 0 && Lk > 0 && D > 0, "%s: bad shape B=%d heads=%d queries=%d keys=%d D=%d", name, B, heads, Lq, Lk, D);
+    MIA_CHECK_ARG(D % 8 == 0 && D <= 128, "%s: head width %d is not a multiple of 8 up to 128", name, D);
+    MIA_CHECK_ARG(height > 0 && width > 0 && (height == 1 || width <= RP_MAX_WIDTH), "%s: bad map %d x %d (at most %d wide if of several rows)", name,
+                  height, width, RP_MAX_WIDTH);
+    MIA_CHECK_ARG((2ll * height - 1) * (2ll * width - 1) <= (1ll << 28), "%s: a map of %d x %d has too many offsets", name, height, width);
+    const long long tokens = (long long)height * width;
+    MIA_CHECK_ARG(Lk <= tokens && q_start >= 0 && (long long)q_start + Lq <= tokens,
+                  "%s: %d keys and %d queries from %d on do not fit a map of %lld tokens", name, Lk, Lq, q_start, tokens);
+    MIA_CHECK_ARG(scale > 0.f && scale < 1e30f, "%s: scale must be positive (got %g)", name, (double)scale);
+    MIA_CHECK_ARG(pdrop >= 0.f && pdrop < 1.f, "%s: dropout %g is not in [0, 1)", name, (double)pdrop);
+    MIA_CHECK_ARG((long long)B * heads * ((Lq + 63ll) / 64) <= 0x3fffffffll && (long long)B * heads * ((Lk + 63ll) / 64) <= 0x3fffffffll,
+                  "%s: too many workgroups", name);
+    return 0;
+}
+
+static int rp_aligned(const char* name, int dtype, const void* p, const RpStride& s) {
+    const long long per = dtype == MIA_BF16 ? 8 : 4;
+    MIA_CHECK_ARG(((uintptr_t)p & 15) == 0 && s.b % per == 0 && s.t % per == 0 && s.h % per == 0,
+                  "%s: rows must start at multiples of 16 bytes", name);
+    return 0;
+}
+
+static void rp_fill(RpArgs& a, int B, int heads, int Lq, int Lk, int D, int height, int width, int q_start, float scale,
+                    float pdrop, unsigned long long seed, const unsigned long long* seed_offset) {
+    a.B = B; a.heads = heads; a.Lq = Lq; a.Lk = Lk; a.D = D; a.W = width; a.pitch = 2 * width - 1;
+    a.off = (height - 1) * a.pitch + width - 1;
+    a.n_off = (2 * height - 1) * a.pitch;
+    a.q_start = q_start; a.scale = scale; a.sl2 = scale * RP_LOG2E;
+    a.pdrop = pdrop; a.seed = seed; a.seed_off = seed_offset;
+    a.tiles = (Lk + RP_TILE - 1) / RP_TILE;
+    a.splits = 1;
+}
+
+static RpStride rp_stride(const long long* s) { return {s[0], s[1], s[2]}; }
+
+extern "C" int mia_relpos_bias(const float* table, const int* bucket, int height, int width, int heads, float scale, float* bias,
+                               void* stream) {
+    MIA_CHECK_ARG(table && bucket && bias, "mia_relpos_bias: null");
+    MIA_CHECK_ARG(height > 0 && width > 0 && heads > 0 && heads <= 65535 && (2ll * height - 1) * (2ll * width - 1) <= (1ll << 28) && scale > 0.f,
+                  "mia_relpos_bias: bad arguments");
+    const int n_off = (2 * height - 1) * (2 * width - 1);
+    // after the division by scale and the later product with scale * log2(e) everything has to stay finite
+    const float limit = 1e38f * fminf(1.f, scale);
+    MIA_LAUNCH(relpos_expand_kernel, dim3(cdiv(n_off, 256), heads), dim3(256), 0, reinterpret_cast<hipStream_t>(stream), table, bucket,
+               n_off, heads, 1.0f / scale, limit, bias);
+    MIA_CHECK_LAUNCH("mia_relpos_bias");
+    return 0;
+}
+
+extern "C" long long mia_relpos_fwd_ws_floats(int dtype, int B, int heads, int Lq, int Lk, int D) {
+    int cols = 1;
+    const int splits = rp_fwd_splits(dtype, B, heads, Lq, Lk, D, cols);
+    return splits > 1 ? (long long)splits * B * heads * Lq * (D + 2) : 0;
+}
+
+extern "C" int mia_relpos_fwd(int dtype, const void* q, const void* k, const void* v, const long long* strides, int B, int heads,
+                              int Lq, int Lk, int D, const float* bias, int height, int width, int q_start,
+                              const uint8_t* key_mask, float scale, float pdrop, unsigned long long seed,
+                              const unsigned long long* seed_offset, float* ws, long long ws_floats, void* out, float* stat,
+                              void* stream) {
+    if (rp_checks("mia_relpos_fwd", dtype, B, heads, Lq, Lk, D, height, width, q_start, scale, pdrop)) return -1;
+    MIA_CHECK_ARG(q && k && v && strides && bias && out, "mia_relpos_fwd: null");
+    MIA_CHECK_ARG(((uintptr_t)stat & 7) == 0, "mia_relpos_fwd: stat must start at a multiple of 8 bytes");
+    RpArgs a = {};
+    a.q = q; a.k = k; a.v = v; a.o = out; a.bias = bias; a.mask = key_mask; a.stat = reinterpret_cast<float2*>(stat);
+    a.sq = rp_stride(strides); a.sk = rp_stride(strides + 3); a.sv = rp_stride(strides + 6);
+    if (rp_aligned("mia_relpos_fwd", dtype, q, a.sq) || rp_aligned("mia_relpos_fwd", dtype, k, a.sk) ||
+        rp_aligned("mia_relpos_fwd", dtype, v, a.sv) || rp_aligned("mia_relpos_fwd", dtype, out, RpStride{0, 0, 0}))
+        return -1;
+    rp_fill(a, B, heads, Lq, Lk, D, height, width, q_start, scale, pdrop, seed, seed_offset);
+    int cols = 1;
+    a.splits = rp_fwd_splits(dtype, B, heads, Lq, Lk, D, cols);
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const long long rows = (long long)B * heads * Lq;
+    if (a.splits > 1) {
+        MIA_CHECK_ARG(ws && ws_floats >= mia_relpos_fwd_ws_floats(dtype, B, heads, Lq, Lk, D),
+                      "mia_relpos_fwd: workspace of %lld floats is too small (%lld needed)", ws_floats,
+                      mia_relpos_fwd_ws_floats(dtype, B, heads, Lq, Lk, D));
+        MIA_CHECK_ARG(((uintptr_t)ws & 15) == 0, "mia_relpos_fwd: the workspace must start at a multiple of 16 bytes");
+        a.po = ws;
+        a.pml = ws + (long long)a.splits * rows * D;
+    }
+    const int tokens = height * width, DP = rp_dp(D);
+    a.win = rp_span(a, RP_TILE, tokens) + rp_span(a, 64 * cols, tokens) + 1;
+    const size_t lds = 2 * (size_t)RP_TILE * rp_ld(dtype, DP) * rp_es(dtype) + RP_TILE * 4 + (size_t)a.win * 4;
+    const int rc = rp_dispatch(RP_FWD, "mia_relpos_fwd", dtype, cols, rp_grid((long long)B * heads * ((Lq + 64 * cols - 1) / (64 * cols)), a.splits), lds, a, s);
+    if (rc || a.splits == 1) return rc;
+    const dim3 threads((D + 63) / 64 * 64);
+    if (dtype == MIA_BF16) MIA_LAUNCH(relpos_join_kernel<bf16_t>, dim3((unsigned)rows), threads, 0, s, a);
+    else MIA_LAUNCH(relpos_join_kernel<float>, dim3((unsigned)rows), threads, 0, s, a);
+    MIA_CHECK_LAUNCH("mia_relpos_fwd");
+    return 0;
+}
+
+// floats of one slab row, and key blocks of one (image, head)
+static int rp_slab_ld(const RpArgs& a, int tokens, int cols) {
+    return rp_span(a, a.Lq, tokens) + rp_span(a, 64 * cols, tokens) + 1;
+}
+
+extern "C" long long mia_relpos_bwd_ws_floats(int dtype, int B, int heads, int Lq, int Lk, int D, int height, int width, int want_bias) {
+    const long long rows = ((long long)B * heads * Lq + 3) / 4 * 4;
+    if (!want_bias) return rows;
+    RpArgs a = {};
+    rp_fill(a, B, heads, Lq, Lk, D, height, width, 0, 1.f, 0.f, 0, nullptr);
+    const int cols = rp_kv_cols(dtype, D, (long long)B * heads, Lk);
+    return rows + (long long)heads * a.n_off +
+           (long long)B * heads * ((Lk + 64 * cols - 1) / (64 * cols)) * rp_slab_ld(a, height * width, cols);
+}
+
+extern "C" int mia_relpos_bwd(int dtype, const void* q, const void* k, const void* v, const long long* strides, const void* dout,
+                              const void* out, const float* stat, int B, int heads, int Lq, int Lk, int D, const float* bias,
+                              int height, int width, int q_start, const uint8_t* key_mask, float scale, float pdrop,
+                              unsigned long long seed, const unsigned long long* seed_offset, const int* order, const int* start,
+                              int buckets, float* ws, long long ws_floats, void* dq, void* dk, void* dv,
+                              const long long* grad_strides, float* dtable, void* stream) {
+    if (rp_checks("mia_relpos_bwd", dtype, B, heads, Lq, Lk, D, height, width, q_start, scale, pdrop)) return -1;
+    MIA_CHECK_ARG(q && k && v && strides && dout && out && stat && bias && ws && dq && dk && dv && grad_strides, "mia_relpos_bwd: null");
+    MIA_CHECK_ARG(((uintptr_t)stat & 7) == 0, "mia_relpos_bwd: stat must start at a multiple of 8 bytes");
+    MIA_CHECK_ARG(!dtable || (order && start && buckets > 0), "mia_relpos_bwd: the bias gradient needs the bucket lists");
+    MIA_CHECK_ARG(heads <= 65535, "mia_relpos_bwd: %d heads are too many", heads);
+    const long long need = mia_relpos_bwd_ws_floats(dtype, B, heads, Lq, Lk, D, height, width, dtable != nullptr);
+    MIA_CHECK_ARG(ws_floats >= need, "mia_relpos_bwd: workspace of %lld floats is too small (%lld needed)", ws_floats, need);
+    RpArgs a = {};
+    a.q = q; a.k = k; a.v = v; a.dout = dout; a.out = out; a.bias = bias; a.mask = key_mask;
+    a.stat = reinterpret_cast<float2*>(const_cast<float*>(stat));
+    a.dq = dq; a.dk = dk; a.dv = dv; a.dsum = ws;
+    a.sq = rp_stride(strides); a.sk = rp_stride(strides + 3); a.sv = rp_stride(strides + 6);
+    a.sdq = rp_stride(grad_strides); a.sdk = rp_stride(grad_strides + 3); a.sdv = rp_stride(grad_strides + 6);
+    const void* ptrs[] = {q, k, v, dq, dk, dv, dout, out};
+    const RpStride sts[] = {a.sq, a.sk, a.sv, a.sdq, a.sdk, a.sdv, {0, 0, 0}, {0, 0, 0}};
+    for (int i = 0; i < 8; ++i)
+        if (rp_aligned("mia_relpos_bwd", dtype, ptrs[i], sts[i])) return -1;
+    rp_fill(a, B, heads, Lq, Lk, D, height, width, q_start, scale, pdrop, seed, seed_offset);
+    hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+    const long long bh = (long long)B * heads;
+    const int tokens = height * width, DP = rp_dp(D);
+    const size_t tile = (size_t)RP_TILE * rp_ld(dtype, DP) * rp_es(dtype);
+    const int qc = rp_cols(dtype, DP, bh, Lq, 64);
+    a.win = rp_span(a, RP_TILE, tokens) + rp_span(a, 64 * qc, tokens) + 1;
+    if (rp_dispatch(RP_BWD_Q, "mia_relpos_bwd", dtype, qc, rp_grid(bh * ((Lq + 64 * qc - 1) / (64 * qc)), 1), 2 * tile + RP_TILE * 4 + (size_t)a.win * 4, a, s))
+        return -2;
+    const int kc = rp_kv_cols(dtype, D, bh, Lk), ktiles = (Lk + 64 * kc - 1) / (64 * kc);
+    int ring = 64;
+    while (ring < rp_span(a, RP_TILE, tokens) + rp_span(a, 64 * kc, tokens) + 1) ring *= 2;
+    a.acc_mask = ring - 1;
+    float* per_off = ws + (bh * Lq + 3) / 4 * 4;
+    if (dtable) {
+        a.slab_ld = rp_slab_ld(a, tokens, kc);
+        a.slab = per_off + (long long)heads * a.n_off;
+    }
+    const size_t kv_lds = 2 * (tile + 256) + 4 * RP_TILE * 4 + (size_t)ring * 4 * (dtable ? 5 : 1);
+    if (rp_dispatch(RP_BWD_KV, "mia_relpos_bwd", dtype, kc, rp_grid(bh * ktiles, 1), kv_lds, a, s)) return -2;
+    if (!dtable) return 0;
+    MIA_LAUNCH(relpos_offsets_kernel, dim3(cdiv(a.n_off, 64), heads), dim3(256), 0, s, a.slab, a, ktiles, 64 * kc, per_off);
+    MIA_CHECK_LAUNCH("mia_relpos_bwd");
+    MIA_LAUNCH(relpos_buckets_kernel, dim3(buckets, heads), dim3(256), 0, s, per_off, a.n_off, heads, order, start, dtable);
+    MIA_CHECK_LAUNCH("mia_relpos_bwd");
+    return 0;
+}

@@ -10,7 +10,7 @@ from array import array
 import torch
 
 from ._lib import lib
-from .ops import _DT, Side, WeightEpoch, _p, _stream
+from .ops import _DT, Side, WeightEpoch, _p, _stream, on_device
 
 
 def _grad_table(grads):
@@ -65,7 +65,7 @@ def grad_norm(grads):
     if not grads:
         return torch.zeros(())
     n, ptrs, dtypes, sizes, device = _grad_table(grads)
-    with torch.cuda.device(device):
+    with on_device(device):
         ws, nws = _norm_ws(n, sizes, device)
         out = torch.empty((2,), dtype=torch.float32, device=device)
         lib().mia_grad_norm(n, _addr(ptrs), _addr(dtypes), _addr(sizes), 1.0, 0.0, _p(ws), nws, _p(out), _stream())
@@ -88,7 +88,7 @@ def clip_grads_(grads, max_norm):
     n, ptrs, dtypes, sizes, device = _grad_table(grads)
     if len(set(ptrs)) != n and len({a for a, k in zip(ptrs, sizes) if k}) != sum(1 for k in sizes if k):
         raise ValueError("a tensor is listed twice: it would be scaled twice")
-    with torch.cuda.device(device):
+    with on_device(device):
         ws, nws = _norm_ws(n, sizes, device)
         out = torch.empty((2,), dtype=torch.float32, device=device)
         lib().mia_grad_clip(n, _addr(ptrs), _addr(dtypes), _addr(sizes), max_norm, _p(ws), nws, _p(out), _stream())

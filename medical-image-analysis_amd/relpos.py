@@ -1,0 +1,212 @@
+"""Multi-head attention with a learned relative position bias, on the gfx950 kernels of csrc/relpos.hip: no limit on the
+number of tokens, masked keys, few queries against many keys, gradients of everything including the bias table."""
+import math
+from array import array
+
+import torch
+
+from . import ops
+from ._lib import lib
+from .ops import _DT, _p, _stream, on_device
+
+
+class RelativePositionBuckets:
+    """Which bucket (= row of a bias table) every offset between two positions of an H x W map falls into; a sequence is a map
+    of height 1. Positions are numbered row by row, and the offset (dy, dx) = position of the key - position of the query has
+    the number (dy + H - 1) * (2 W - 1) + dx + W - 1 in `index`.
+
+    The constructor buckets each axis on its own: half of num_buckets for each direction, half of those one distance each, the
+    rest logarithmic up to max_distance and one for everything beyond; a map of several rows has num_buckets ** 2 rows of
+    bias, a sequence num_buckets. from_index takes any assignment (one bucket per offset, shared buckets, ...).
+    Built once and kept, like the weights: it holds the index and the offsets sorted by bucket on the device."""
+
+    def __init__(self, height, width, num_buckets=32, max_distance=128, device="cuda"):
+        if num_buckets < 4 or num_buckets % 4:
+            raise ValueError(f"num_buckets must be a multiple of 4 (got {num_buckets})")
+        if max_distance <= num_buckets // 4:
+            raise ValueError(f"max_distance must exceed the {num_buckets // 4} exact distances (got {max_distance})")
+        self._check_map(height, width)
+        rows = 1 if height == 1 else num_buckets
+        by, bx = self._axis(height, num_buckets, max_distance), self._axis(width, num_buckets, max_distance)
+        index = by[:, None] * num_buckets + bx[None, :]
+        self._set(height, width, index.reshape(-1), rows * num_buckets, device)
+
+    @staticmethod
+    def _axis(n, buckets, max_distance):
+        if n == 1:
+            return torch.zeros(1, dtype=torch.int64)
+        d = torch.arange(1 - n, n, dtype=torch.float64)
+        half, exact = buckets // 2, buckets // 4
+        far = exact + ((d.abs().clamp(min=exact) / exact).log() / math.log(max_distance / exact) * (half - exact)).floor()
+        return torch.where(d.abs() < exact, d.abs(), far.clamp(max=half - 1)).long() + half * (d > 0).long()
+
+    @classmethod
+    def from_index(cls, height, width, index, num_buckets=None, device="cuda"):
+        """index: (2H - 1)(2W - 1) integers (any shape) on any device; num_buckets defaults to the largest + 1."""
+        cls._check_map(height, width)
+        index = torch.as_tensor(index)
+        if index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
+            raise TypeError(f"index holds integers (got {index.dtype})")
+        self = cls.__new__(cls)
+        self._set(height, width, index.detach().cpu().long().reshape(-1), num_buckets, device)
+        return self
+
+    @staticmethod
+    def _check_map(height, width):
+        if height < 1 or width < 1 or (height > 1 and width > 1024) or (2 * height - 1) * (2 * width - 1) > 1 << 28:
+            raise ValueError(f"a map of {height} x {width} is not supported (several rows: at most 1024 wide; at most 2 ** 28 offsets)")
+
+    def _set(self, height, width, index, num_buckets, device):
+        n = (2 * height - 1) * (2 * width - 1)
+        if index.numel() != n:
+            raise ValueError(f"a map of {height} x {width} has {n} offsets (got an index of {index.numel()})")
+        low, high = int(index.min()), int(index.max())
+        num_buckets = high + 1 if num_buckets is None else int(num_buckets)
+        if low < 0 or high >= num_buckets:
+            raise ValueError(f"buckets {low}..{high} are not all in 0..{num_buckets - 1}")
+        self.height, self.width, self.num_buckets = int(height), int(width), num_buckets
+        start = torch.zeros(num_buckets + 1, dtype=torch.int64)
+        start[1:] = torch.bincount(index, minlength=num_buckets).cumsum(0)
+        self.index = index.to(torch.int32).to(device)
+        self.order = index.argsort(stable=True).to(torch.int32).to(device)
+        self.start = start.to(torch.int32).to(device)
+
+    @property
+    def device(self):
+        return self.index.device
+
+
+def _rows(t):
+    """The tensor itself when the kernels can read it where it lies (head elements contiguous, rows at multiples of 16
+    bytes), else a contiguous copy; and its (batch, token, head) strides in elements."""
+    per = 16 // t.element_size()
+    st = [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride())]
+    if (t.stride(3) != 1 and t.shape[3] != 1) or any(s % per or s < 0 for s in st) or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:       # a contiguous view that starts in between
+            t = t.clone()
+        st = [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride())]
+    return t, st
+
+
+class RelPosAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, table, plan, mask, scale, q_start, pdrop, seed):
+        ctx.packed = k is None
+        if ctx.packed:
+            q, k, v = q.unbind(2)
+        B, Lq, heads, D = q.shape
+        Lk = k.shape[1]
+        dev, f32 = q.device, dict(dtype=torch.float32, device=q.device)
+        ctx.meta = (B, heads, Lq, Lk, D, plan, scale, q_start, pdrop, seed, ops.seed_offset())
+        ctx.empty = 0 in (B, Lq, Lk, heads)
+        if ctx.empty:
+            out = torch.zeros((B, Lq, heads, D), dtype=q.dtype, device=dev)
+            ctx.save_for_backward(q, k, v, table)
+            return out
+        out = torch.empty((B, Lq, heads, D), dtype=q.dtype, device=dev)
+        (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
+        table, mask = table.contiguous(), mask.contiguous() if mask is not None else None
+        strides = array("q", sq + sk + sv)
+        bias = torch.empty((heads, plan.index.numel()), **f32)
+        stat = torch.empty((B, heads, Lq, 2), **f32) if any(ctx.needs_input_grad) else None
+        dt = _DT[q.dtype]
+        nws = lib().mia_relpos_fwd_ws_floats(dt, B, heads, Lq, Lk, D)
+        ws = torch.empty((nws,), **f32) if nws else None
+        with on_device(dev):
+            lib().mia_relpos_bias(_p(table), _p(plan.index), plan.height, plan.width, heads, scale, _p(bias), _stream())
+            lib().mia_relpos_fwd(dt, _p(q), _p(k), _p(v), strides.buffer_info()[0], B, heads, Lq, Lk, D, _p(bias), plan.height,
+                                 plan.width, q_start, _p(mask), scale, pdrop, seed, ops.seed_offset(), _p(ws), nws, _p(out),
+                                 _p(stat), _stream())
+        ctx.strides = strides
+        ctx.save_for_backward(q, k, v, bias, mask, out, stat)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        B, heads, Lq, Lk, D, plan, scale, q_start, pdrop, seed, soff = ctx.meta
+        if ctx.empty:
+            q, k, v, table = ctx.saved_tensors
+            dt = torch.zeros_like(table)
+            if ctx.packed:
+                return (torch.zeros((B, Lq, 3, heads, D), dtype=q.dtype, device=q.device), None, None, dt) + (None,) * 6
+            return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), dt) + (None,) * 6
+        q, k, v, bias, mask, out, stat = ctx.saved_tensors
+        if ctx.packed:
+            dqkv = torch.empty((B, Lq, 3, heads, D), dtype=q.dtype, device=q.device)
+            dq, dk, dv = dqkv.unbind(2)
+        else:
+            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dout = _rows(dout.contiguous())[0]
+        f32 = dict(dtype=torch.float32, device=q.device)
+        want = ctx.needs_input_grad[3]
+        dtable = torch.empty((plan.num_buckets, heads), **f32) if want else None
+        nws = lib().mia_relpos_bwd_ws_floats(_DT[q.dtype], B, heads, Lq, Lk, D, plan.height, plan.width, 1 if want else 0)
+        ws = torch.empty((nws,), **f32)
+        gst = array("q", [s for t in (dq, dk, dv) for s in (0 if n == 1 else st for n, st in zip(t.shape[:3], t.stride()))])
+        with on_device(q.device):
+            lib().mia_relpos_bwd(_DT[q.dtype], _p(q), _p(k), _p(v), ctx.strides.buffer_info()[0], _p(dout), _p(out), _p(stat), B,
+                                 heads, Lq, Lk, D, _p(bias), plan.height, plan.width, q_start, _p(mask), scale, pdrop, seed, soff,
+                                 _p(plan.order), _p(plan.start), plan.num_buckets, _p(ws), nws, _p(dq), _p(dk), _p(dv),
+                                 gst.buffer_info()[0], _p(dtable), _stream())
+        if ctx.packed:
+            return (dqkv, None, None, dtable) + (None,) * 6
+        return (dq, dk, dv, dtable) + (None,) * 6
+
+
+def _attend(name, q, k, v, table, buckets, key_mask, scale, q_start, dropout_p, seed, packed):
+    B, Lq, heads, D = q.shape
+    Lk = k.shape[1]
+    if q.dtype not in _DT or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"{name}: queries, keys and values are all fp32 or all bf16 (got {q.dtype}, {k.dtype}, {v.dtype})")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError(f"{name}: the head width must be a multiple of 8 up to 128 (got {D})")
+    tokens = buckets.height * buckets.width
+    q_start = int(q_start)
+    if Lk > tokens or q_start < 0 or q_start + Lq > tokens:
+        raise ValueError(f"{name}: {Lk} keys and {Lq} queries from {q_start} on do not fit a map of {buckets.height} x {buckets.width}")
+    if tuple(table.shape) != (buckets.num_buckets, heads) or table.dtype != torch.float32:
+        raise ValueError(f"{name}: the table must be fp32 {(buckets.num_buckets, heads)} (got {table.dtype} {tuple(table.shape)})")
+    if key_mask is not None and (tuple(key_mask.shape) != (B, Lk) or key_mask.dtype not in (torch.bool, torch.uint8)):
+        raise ValueError(f"{name}: key_mask must be bool {(B, Lk)}, true where a key counts (got {key_mask.dtype} {tuple(key_mask.shape)})")
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 1e-30 < scale < 1e30:
+        raise ValueError(f"{name}: scale must be positive (got {scale})")
+    dropout_p = float(dropout_p)
+    if not 0.0 <= dropout_p < 1.0:
+        raise ValueError(f"{name}: dropout must be in [0, 1) (got {dropout_p})")
+    for what, t in (("queries", q), ("keys", k), ("values", v), ("table", table), ("buckets", buckets.index), ("key_mask", key_mask)):
+        if t is not None and (not t.is_cuda or t.device != q.device):
+            raise RuntimeError(f"{name} needs its tensors on one MI355X device; there is no CPU path ({what}: {t.device})")
+    if dropout_p > 0.0 and seed is None:
+        from .head_ops import _seed
+        seed = _seed()
+    first = (packed, None, None) if packed is not None else (q, k, v)
+    return RelPosAttentionFn.apply(*first, table, buckets, key_mask, scale, q_start, dropout_p, int(seed or 0))
+
+
+def relpos_attention(q, k, v, table, buckets, key_mask=None, scale=None, q_start=0, dropout_p=0.0, seed=None):
+    """out[b, i, h] = sum_j softmax_j(scale * q[b, i, h] . k[b, j, h] + table[bucket(position of j - position of i), h]) v[b, j, h]
+
+    q [B, Lq, heads, D], k and v [B, Lk, heads, D], fp32 or bf16, any strides (read in place when heads are contiguous rows at
+    multiples of 16 bytes); D a multiple of 8 up to 128. buckets: a RelativePositionBuckets over a map of at least Lk tokens;
+    key j is at token j, query i at token q_start + i (a new token against a series: q_start = Lk - 1). table: fp32
+    [buckets.num_buckets, heads]. key_mask: bool [B, Lk], false = the key does not exist (what its rows hold is never read into a
+    result); a query without any key gives zeros. scale defaults to 1/sqrt(D). dropout_p drops attention weights with the
+    counter-based mask of the library's other dropouts. Returns [B, Lq, heads, D]; differentiable in q, k, v and table, the
+    same bits every time."""
+    for what, t in (("q", q), ("k", k), ("v", v)):
+        if t.dim() != 4:
+            raise ValueError(f"relpos_attention: {what} must be [batch, tokens, heads, D] (got {tuple(t.shape)})")
+    if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+        raise ValueError(f"relpos_attention: shapes do not belong together: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    return _attend("relpos_attention", q, k, v, table, buckets, key_mask, scale, q_start, dropout_p, seed, None)
+
+
+def relpos_self_attention(qkv, table, buckets, key_mask=None, scale=None, dropout_p=0.0, seed=None):
+    """relpos_attention of a packed projection qkv [B, L, 3, heads, D] over the first L tokens of the map; its gradient comes
+    back packed as well."""
+    if qkv.dim() != 5 or qkv.shape[2] != 3:
+        raise ValueError(f"relpos_self_attention: qkv must be [batch, tokens, 3, heads, D] (got {tuple(qkv.shape)})")
+    q, k, v = qkv.detach().unbind(2)
+    return _attend("relpos_self_attention", q, k, v, table, buckets, key_mask, scale, 0, dropout_p, seed, qkv)
