@@ -29,6 +29,9 @@ typedef __attribute__((ext_vector_type(8))) __bf16 rp_bf16x8;
 
 #define RP_LOG2E 1.4426950408889634f
 #define RP_TILE 64          // tokens of a staged tile
+// Largest maximum, in units of the exponent, up to which P = exp2(acc * sl2 - shift) is formed by one FMA with shift rounded to
+// fp32 (64 * 2^-24 = 4e-6 relative in P at worst); rows beyond it subtract first.
+#define RP_FAR 64.f
 #define RP_MAX_WIDTH 896    // of a map of several rows: keeps the dK/dV kernel's rings (RP_RING_MAX offsets) in LDS
 #define RP_RING_MAX 2048
 
@@ -47,7 +50,7 @@ struct RpArgs {
     float *po, *pml;              // split forward: [splits][B * heads * Lq][D], [..][2]
     int B, heads, Lq, Lk, D, W, off, n_off, q_start;
     unsigned inv_w;               // ceil(2^32 / W)
-    int tiles, splits, win, acc_mask, slab_ld;
+    int tiles, splits, acc_mask, slab_ld;
     float scale, sl2, pdrop;
     unsigned long long seed;
     const unsigned long long* seed_off;
@@ -155,6 +158,7 @@ struct RpDim {
     static constexpr int CPR = DP / PER;                                     // 16-byte pieces of a staged row
     static constexpr int NST = (RP_TILE * CPR + 255) / 256;                  // pieces per thread
     static constexpr int DB = DP / 16;                                       // 16-wide output blocks
+    static constexpr bool EARLY = ES == 2 && DP <= 64;                       // registers for operands requested ahead
 };
 
 // 16-byte pieces of one row for this lane: elements beyond D are zeros (D is a multiple of 8)
@@ -168,41 +172,95 @@ __device__ __forceinline__ void rp_row_frags(const T* row, bool ok, int D, int g
     }
 }
 
-// One tile of rows on its way to LDS, kept in registers while the tile before it is worked on. The loads are unconditional
-// (rows past the end read the last row, columns past D the first): what counts is decided when the tile is put down.
+// One tile of rows on its way to LDS, kept in registers while the tile before it is worked on; a group of 256 threads, tid its
+// thread. The loads are unconditional (rows past the end read the last row, columns past D the first): what counts is
+// decided when the tile is put down. Their addresses are one scalar per tile plus 32-bit offsets that never change.
 template <typename T, int DP>
 struct RpTile {
     static constexpr int CPR = RpDim<T, DP>::CPR, NST = RpDim<T, DP>::NST;
     uint4 r[NST];
-    // rows first .. first + 63 of src (row stride st), of `limit` rows in all
-    __device__ __forceinline__ void fetch(const T* src, long long st, int first, int limit, int D) {
+    unsigned off[NST];   // bytes
+    __device__ __forceinline__ void init(long long st, int D, int tid) {
 #pragma unroll
         for (int i = 0; i < NST; ++i) {
-            const int id = i * 256 + threadIdx.x, row = id / CPR, col = (id - row * CPR) * RpOp<T>::PER;
-            r[i] = *reinterpret_cast<const uint4*>(src + (long long)min(first + row, limit - 1) * st + (col < D ? col : 0));
+            const int id = i * 256 + tid, row = min(id / CPR, RP_TILE - 1), col = (id % CPR) * RpOp<T>::PER;
+            off[i] = ((unsigned)row * (unsigned)st + (unsigned)(col < D ? col : 0)) * (unsigned)sizeof(T);
         }
     }
-    // bit i of valid clear: row i becomes zeros. INS: extra elements after every 16 rows
-    template <int INS>
-    __device__ __forceinline__ void put(T* lds, unsigned long long valid, int D) const {
+    // rows first .. first + 63 of src (row stride st), of `limit` rows in all
+    __device__ __forceinline__ void fetch(const T* src, long long st, int first, int limit, int D, int tid) {
+        const char* base = reinterpret_cast<const char*>(src + (long long)first * st);
+        if (first + RP_TILE <= limit) {
 #pragma unroll
-        for (int i = 0; i < NST; ++i) {
-            const int id = i * 256 + threadIdx.x, row = id / CPR, col = (id - row * CPR) * RpOp<T>::PER;
-            const bool keep = ((valid >> (row & 63)) & 1) && col < D;
-            if ((RP_TILE * CPR) % 256 == 0 || row < RP_TILE)
-                *reinterpret_cast<uint4*>(lds + row * RpDim<T, DP>::LD + (row >> 4) * INS + col) = keep ? r[i] : make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < NST; ++i) r[i] = *reinterpret_cast<const uint4*>(base + off[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NST; ++i) {
+                const int id = i * 256 + tid, row = min(id / CPR, limit - 1 - first), col = (id % CPR) * RpOp<T>::PER;
+                r[i] = *reinterpret_cast<const uint4*>(base + ((unsigned)row * (unsigned)st + (unsigned)(col < D ? col : 0)) * (unsigned)sizeof(T));
+            }
         }
+    }
+    // bit i of valid clear: row i becomes zeros. Columns past D are not written (rp_zero_pad). INS: extra elements after every
+    // 16 rows
+    template <int INS>
+    __device__ __forceinline__ void put(T* lds, unsigned long long valid, int D, int tid) const {
+        if (valid == ~0ull) {
+#pragma unroll
+            for (int i = 0; i < NST; ++i)
+                if (used(i, D, tid)) *place<INS>(lds, i, tid) = r[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < NST; ++i)
+                if (used(i, D, tid)) *place<INS>(lds, i, tid) = (valid >> ((i * 256 + tid) / CPR)) & 1 ? r[i] : make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+    static __device__ __forceinline__ bool used(int i, int D, int tid) {
+        const int id = i * 256 + tid;
+        return ((RP_TILE * CPR) % 256 == 0 || id < RP_TILE * CPR) && (id % CPR) * RpOp<T>::PER < D;
+    }
+    template <int INS>
+    static __device__ __forceinline__ uint4* place(T* lds, int i, int tid) {
+        const int id = i * 256 + tid, row = id / CPR;
+        return reinterpret_cast<uint4*>(lds + row * RpDim<T, DP>::LD + (row >> 4) * INS + (id - row * CPR) * RpOp<T>::PER);
     }
 };
 
-// columns between DP and the padded reduction length are read as operands and never staged: zero once
+// a value loaded before a loop is waited for here: without it the wait falls on its first use inside the loop, where it also
+// waits for whatever the loop has in flight
+template <typename V>
+__device__ __forceinline__ void rp_settle(V& v) {
+    asm volatile("" : "+v"(v));
+}
+
+// Barrier between the waves' LDS work on one tile and the next. The wait is explicit because LDS additions return nothing that a
+// later instruction would wait for, and the compiler has been seen to leave none of its own in front of the barrier at a loop's
+// top: the ring below was then read before the last additions had arrived.
+__device__ __forceinline__ void rp_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
+enum { RP_FWD, RP_BWD_Q, RP_BWD_KV };
+// Waves a SIMD has room for: the most that leave a kernel without scratch. Asking for two already keeps the compiler from
+// spreading over the accumulation registers, whose moves cost issue slots (38x38 maps, batch 4, 8 heads of 64: forward 50 -> 45
+// us, dK/dV 140 -> 107).
+constexpr int rp_waves(int what, bool half, int DP, int cols) {
+    if (what == RP_FWD)
+        return half ? (cols == 1 ? (DP <= 32 ? 4 : DP <= 64 ? 3 : 2) : (DP <= 16 ? 3 : 2)) : (DP <= 32 ? 4 : DP <= 64 ? 3 : 2);
+    if (what == RP_BWD_Q) return half ? (cols == 1 ? (DP <= 32 ? 4 : DP <= 64 ? 3 : 2) : (DP <= 32 ? 3 : 2)) : (DP <= 32 ? 4 : DP <= 96 ? 2 : 1);
+    return half ? (cols == 1 ? (DP <= 32 ? 4 : DP <= 64 ? 3 : 2) : (DP <= 16 ? 3 : 2)) : (DP <= 16 ? 4 : DP <= 32 ? 3 : DP <= 64 ? 2 : 1);
+}
+
+// columns between D and the padded reduction length are read as operands and never staged: zero once
 template <typename T, int DP, int INS>
-__device__ __forceinline__ void rp_zero_pad(T* lds) {
-    constexpr int LD = RpDim<T, DP>::LD, PADC = RpDim<T, DP>::NCH * RpOp<T>::CHUNK - DP;
-    if constexpr (PADC > 0)
-        for (int i = threadIdx.x; i < RP_TILE * PADC; i += 256) {
-            const int row = i / PADC;
-            lds[row * LD + (row >> 4) * INS + DP + (i - row * PADC)] = from_f32<T>(0.f);
+__device__ __forceinline__ void rp_zero_pad(T* lds, int D, int tid) {
+    const int pad = RpDim<T, DP>::NCH * RpOp<T>::CHUNK - D;
+    if (pad > 0)
+#pragma unroll 1
+        for (int i = tid; i < RP_TILE * pad; i += 256) {
+            const int row = i / pad;
+            lds[row * RpDim<T, DP>::LD + (row >> 4) * INS + D + (i - row * pad)] = from_f32<T>(0.f);
         }
 }
 
@@ -238,9 +296,18 @@ __device__ __forceinline__ unsigned long long rp_valid(const RpArgs& a, int k0, 
     return __ballot(byte != 0 && k0 + (int)(threadIdx.x & 63) < a.Lk);
 }
 
-// blocks of one (image, head) stay on one XCD, whose L2 then holds that head's keys and values: consecutive hardware
-// workgroup ids go to the eight XCDs in turn. The grid is a multiple of 8; ids past `total` have nothing to do.
-__device__ __forceinline__ int rp_block(int id, int grid) { return (id & 7) * (grid >> 3) + (id >> 3); }
+// Which block (of `per` blocks of each (image, head)) a workgroup works on. Consecutive hardware workgroup ids go to the eight XCDs
+// in turn; the blocks of one (image, head) stay on one XCD, whose L2 then holds that head's keys and values. Images are dealt to
+// the XCDs in turn when their number is a multiple of eight (the heads of a packed token share cache lines: 10x10 maps, batch 128,
+// 8 heads of 48: forward 20 us, 23 with heads dealt out), else (image, head)s are (an image that is masked out then costs
+// every XCD the same: 38x38 maps, batch 4, one of them empty: forward 46 us, 48 with a run for each XCD), else each XCD gets an
+// equal run of blocks. The grid is a multiple of 8; ids past the last block have nothing to do.
+__device__ __forceinline__ int rp_block(const RpArgs& a, int per) {
+    const int id = blockIdx.x, bhs = a.B * a.heads;
+    if (bhs & 7) return (id & 7) * ((int)gridDim.x >> 3) + (id >> 3);
+    const int unit = a.B & 7 ? per : per * a.heads, j = id >> 3, q = j / unit;
+    return (q * 8 + (id & 7)) * unit + (j - q * unit);
+}
 
 // ------------------------------------------------------------------------------------------------
 // bias[h][o] = table[bucket[o]][h] / scale. Finite values stay finite (the largest ones are clamped): a table entry at the
@@ -259,15 +326,16 @@ __global__ __launch_bounds__(256) void relpos_expand_kernel(const float* __restr
 // the bias window of one tile on its way to LDS
 struct RpWindow {
     float r[2];
-    __device__ __forceinline__ void fetch(const float* src, int n) {
+    __device__ __forceinline__ void fetch(const float* src, int n, int tid) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) r[i] = src[min(i * 256 + (int)threadIdx.x, n - 1)];
+        for (int i = 0; i < 2; ++i) r[i] = src[min(i * 256 + tid, n - 1)];
     }
-    __device__ __forceinline__ void put(float* dst, const float* src, int n) const {
+    __device__ __forceinline__ void put(float* dst, const float* src, int n, int tid) const {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            if (i * 256 + (int)threadIdx.x < n) dst[i * 256 + threadIdx.x] = r[i];
-        for (int i = 512 + threadIdx.x; i < n; i += 256) dst[i] = src[i];
+            if (i * 256 + tid < n) dst[i * 256 + tid] = r[i];
+#pragma unroll 1
+        for (int i = 512 + tid; i < n; i += 256) dst[i] = src[i];
     }
 };
 // four entries of the window: c4 holds byte offsets of four rows, cq that of the column
@@ -283,20 +351,21 @@ __device__ __forceinline__ rp_f32x4 rp_bias4(const float* bw, const int4& c4, in
 // leaves an unnormalised partial result.
 // ------------------------------------------------------------------------------------------------
 template <typename T, int DP, int QB>
-__global__ __launch_bounds__(256) void relpos_fwd_kernel(RpArgs a) {
+__global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void relpos_fwd_kernel(RpArgs a) {
     typedef RpOp<T> Op;
     typedef RpDim<T, DP> Dim;
     constexpr int LD = Dim::LD, QT = 64 * QB;
     extern __shared__ __attribute__((aligned(16))) char rp_sm[];
+    const int tid = threadIdx.x;
     T* Ks = reinterpret_cast<T*>(rp_sm);
     T* Vs = Ks + RP_TILE * LD;
     int* ck = reinterpret_cast<int*>(Vs + RP_TILE * LD);
-    float* bw = reinterpret_cast<float*>(ck + RP_TILE);
-    const int qtiles = (a.Lq + QT - 1) / QT, id = rp_block(blockIdx.x, gridDim.x);
+    float* cap = reinterpret_cast<float*>(ck + RP_TILE);   // scores end at this: -inf for a key that does not exist
+    float* bw = cap + RP_TILE;
+    const int qtiles = (a.Lq + QT - 1) / QT, id = rp_block(a, qtiles);
     if (id >= a.B * a.heads * qtiles) return;
     const int bh = id / qtiles, b = bh / a.heads, h = bh - b * a.heads, q0 = (id - bh * qtiles) * QT;
-    const int t0 = (int)((long long)a.tiles * blockIdx.y / a.splits), t1 = (int)((long long)a.tiles * (blockIdx.y + 1) / a.splits);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const int lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
     const T* kp = (const T*)a.k + b * a.sk.b + h * a.sk.h;
     const T* vp = (const T*)a.v + b * a.sv.b + h * a.sv.h;
     const float* bias = a.bias + (size_t)h * a.n_off;
@@ -317,33 +386,45 @@ __global__ __launch_bounds__(256) void relpos_fwd_kernel(RpArgs a) {
 #pragma unroll
         for (int d = 0; d < Dim::DB; ++d) o[i][d] = rp_f32x4{0.f, 0.f, 0.f, 0.f};
     }
+#pragma unroll
+    for (int i = 0; i < QB; ++i)
+#pragma unroll
+        for (int c = 0; c < Dim::NCH; ++c) rp_settle(qf[i][c]);
     const bool idle = q0 + wave * QB * 16 >= a.Lq;   // a wave without queries only helps to stage
     const unsigned long long seed = a.pdrop > 0.f ? rp_seed(a) : 0ull;
-    rp_zero_pad<T, DP, 0>(Ks);
+    rp_zero_pad<T, DP, 0>(Ks, a.D, tid);
+    rp_zero_pad<T, DP, 0>(Vs, a.D, tid);
 
     RpTile<T, DP> kt, vt;
+    kt.init(a.sk.t, a.D, tid);
+    vt.init(a.sv.t, a.D, tid);
     RpWindow wt;
     unsigned long long valid = 0ull;
     int byte = 0, ck_lo = 0, n_win = 0, base = 0;
     auto fetch = [&](int t) {
         const int k0 = t * RP_TILE;
         byte = rp_mask_byte(a, b, k0);
-        kt.fetch(kp, a.sk.t, k0, a.Lk, a.D);
-        vt.fetch(vp, a.sv.t, k0, a.Lk, a.D);
+        kt.fetch(kp, a.sk.t, k0, a.Lk, a.D, tid);
+        vt.fetch(vp, a.sv.t, k0, a.Lk, a.D, tid);
         ck_lo = rp_c(a, k0);
         base = ck_lo - cq_hi + a.off;
         n_win = rp_c(a, min(k0 + RP_TILE, a.Lk) - 1) - ck_lo + cq_hi - cq_lo + 1;
-        wt.fetch(bias + base, n_win);
+        wt.fetch(bias + base, n_win, tid);
     };
-    if (t0 < t1) fetch(t0);
-    for (int t = t0; t < t1; ++t) {
-        __syncthreads();
+    const int t1 = (int)((long long)a.tiles * (blockIdx.y + 1) / a.splits);
+    int t = (int)((long long)a.tiles * blockIdx.y / a.splits);
+    if (t < t1) fetch(t);
+    for (; t < t1; ++t) {
+        rp_barrier();
         valid = rp_valid(a, t * RP_TILE, byte);
-        kt.template put<0>(Ks, valid, a.D);
-        vt.template put<0>(Vs, valid, a.D);
-        wt.put(bw, bias + base, n_win);
-        if (threadIdx.x < RP_TILE) ck[threadIdx.x] = 4 * (rp_c(a, min(t * RP_TILE + (int)threadIdx.x, a.Lk - 1)) - ck_lo);
-        __syncthreads();
+        kt.template put<0>(Ks, valid, a.D, tid);
+        vt.template put<0>(Vs, valid, a.D, tid);
+        wt.put(bw, bias + base, n_win, tid);
+        if (tid < RP_TILE) {
+            ck[tid] = 4 * (rp_c(a, min(t * RP_TILE + tid, a.Lk - 1)) - ck_lo);
+            cap[tid] = (valid >> tid) & 1 ? INFINITY : -INFINITY;
+        }
+        rp_barrier();
         if (t + 1 < t1) fetch(t + 1);
         if (idle || valid == 0ull) continue;
         rp_f32x4 s[4][QB];
@@ -361,15 +442,27 @@ __global__ __launch_bounds__(256) void relpos_fwd_kernel(RpArgs a) {
 #pragma unroll
                 for (int i = 0; i < QB; ++i) s[kb][i] = Op::dot(kf, qf[i][c], s[kb][i]);
             }
+        // the value operands are requested here, so that they arrive while the softmax runs
+        typename Op::TFrag vf[2][Dim::DB];
+        auto values = [&](int kk) {
+#pragma unroll
+            for (int d = 0; d < Dim::DB; ++d) {
+                const T* v0 = Vs + (kk * 32 + g * 4) * LD + d * 16;
+                vf[kk][d] = Op::load_t(v0, v0 + 16 * LD, LD, l);
+            }
+        };
+        if constexpr (Dim::EARLY) {
+            values(0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         if (valid != ~0ull) {
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
-                const unsigned bits = (unsigned)(valid >> (kb * 16 + g * 4));
+                const rp_f32x4 c4 = *reinterpret_cast<const rp_f32x4*>(cap + kb * 16 + g * 4);
 #pragma unroll
                 for (int i = 0; i < QB; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (!((bits >> r) & 1)) s[kb][i][r] = -INFINITY;
+                    for (int r = 0; r < 4; ++r) s[kb][i][r] = fminf(s[kb][i][r], c4[r]);
             }
         }
 #pragma unroll
@@ -388,14 +481,23 @@ __global__ __launch_bounds__(256) void relpos_fwd_kernel(RpArgs a) {
                 for (int d = 0; d < Dim::DB; ++d) o[i][d] *= alpha;
             }
             m[i] = mx;
+            // one FMA where the rounding of use * sl2 cannot matter, the difference first where it would
+            if (!__any(fabsf(use) * a.sl2 > RP_FAR)) {
+                const float shift = use * a.sl2;
 #pragma unroll
-            for (int kb = 0; kb < 4; ++kb)
+                for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float p = __builtin_amdgcn_exp2f((s[kb][i][r] - use) * a.sl2);
-                    sum[i] += p;
-                    s[kb][i][r] = p;
-                }
+                    for (int r = 0; r < 4; ++r) s[kb][i][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][i][r], a.sl2, -shift));
+            } else {
+#pragma unroll
+                for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) s[kb][i][r] = __builtin_amdgcn_exp2f((s[kb][i][r] - use) * a.sl2);
+            }
+            float part[4];
+#pragma unroll
+            for (int kb = 0; kb < 4; ++kb) part[kb] = (s[kb][i][0] + s[kb][i][1]) + (s[kb][i][2] + s[kb][i][3]);
+            sum[i] += (part[0] + part[1]) + (part[2] + part[3]);
             if (a.pdrop > 0.f) {
                 const unsigned long long at = ((unsigned long long)bh * a.Lq + qi[i]) * a.Lk + t * RP_TILE + g * 4;
 #pragma unroll
@@ -409,13 +511,12 @@ __global__ __launch_bounds__(256) void relpos_fwd_kernel(RpArgs a) {
             typename Op::Pair p[QB];
 #pragma unroll
             for (int i = 0; i < QB; ++i) p[i] = Op::pack(s[2 * kk][i], s[2 * kk + 1][i]);
+            if (!Dim::EARLY) values(kk);
+            else if (kk == 0) values(1);
 #pragma unroll
-            for (int d = 0; d < Dim::DB; ++d) {
-                const T* v0 = Vs + (kk * 32 + g * 4) * LD + d * 16;
-                const typename Op::TFrag vf = Op::load_t(v0, v0 + 16 * LD, LD, l);
+            for (int d = 0; d < Dim::DB; ++d)
 #pragma unroll
-                for (int i = 0; i < QB; ++i) o[i][d] = Op::dot_t(vf, p[i], o[i][d]);
-            }
+                for (int i = 0; i < QB; ++i) o[i][d] = Op::dot_t(vf[kk][d], p[i], o[i][d]);
         }
     }
 #pragma unroll
@@ -471,19 +572,21 @@ __global__ void relpos_join_kernel(RpArgs a) {
 // backward, queries as columns: dQ and the exact D. The same walk as the forward.
 // ------------------------------------------------------------------------------------------------
 template <typename T, int DP, int QB>
-__global__ __launch_bounds__(256) void relpos_bwd_q_kernel(RpArgs a) {
+__global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) void relpos_bwd_q_kernel(RpArgs a) {
     typedef RpOp<T> Op;
     typedef RpDim<T, DP> Dim;
     constexpr int LD = Dim::LD, QT = 64 * QB;
     extern __shared__ __attribute__((aligned(16))) char rp_sm[];
+    const int tid = threadIdx.x;
     T* Ks = reinterpret_cast<T*>(rp_sm);
     T* Vs = Ks + RP_TILE * LD;
     int* ck = reinterpret_cast<int*>(Vs + RP_TILE * LD);
-    float* bw = reinterpret_cast<float*>(ck + RP_TILE);
-    const int qtiles = (a.Lq + QT - 1) / QT, id = rp_block(blockIdx.x, gridDim.x);
+    float* cap = reinterpret_cast<float*>(ck + RP_TILE);   // scores end at this: -inf for a key that does not exist
+    float* bw = cap + RP_TILE;
+    const int qtiles = (a.Lq + QT - 1) / QT, id = rp_block(a, qtiles);
     if (id >= a.B * a.heads * qtiles) return;
     const int bh = id / qtiles, b = bh / a.heads, h = bh - b * a.heads, q0 = (id - bh * qtiles) * QT;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
+    const int lane = tid & 63, wave = tid >> 6, l = lane & 15, g = lane >> 4;
     const T* kp = (const T*)a.k + b * a.sk.b + h * a.sk.h;
     const T* vp = (const T*)a.v + b * a.sv.b + h * a.sv.h;
     const float* bias = a.bias + (size_t)h * a.n_off;
@@ -492,7 +595,8 @@ __global__ __launch_bounds__(256) void relpos_bwd_q_kernel(RpArgs a) {
 
     typename Op::Frag qf[QB][Dim::NCH], gf[QB][Dim::NCH];
     int qi[QB], cq[QB];
-    float mx[QB], lg[QB], D0[QB], extra[QB];
+    float mx[QB], lg[QB], shift[QB], D0[QB], extra[QB];
+    bool far = false;
     rp_f32x4 dq[QB][Dim::DB];
 #pragma unroll
     for (int i = 0; i < QB; ++i) {
@@ -516,35 +620,54 @@ __global__ __launch_bounds__(256) void relpos_bwd_q_kernel(RpArgs a) {
 #pragma unroll
         for (int c = 0; c < Dim::DB; ++c) dq[i][c] = rp_f32x4{0.f, 0.f, 0.f, 0.f};
     }
+#pragma unroll
+    for (int i = 0; i < QB; ++i) {
+#pragma unroll
+        for (int c = 0; c < Dim::NCH; ++c) {
+            rp_settle(qf[i][c]);
+            rp_settle(gf[i][c]);
+        }
+        rp_settle(mx[i]);
+        rp_settle(lg[i]);
+        shift[i] = fmaf(mx[i], a.sl2, lg[i]);
+        far |= fabsf(mx[i]) * a.sl2 > RP_FAR;
+    }
+    far = __any(far);
     const bool idle = q0 + wave * QB * 16 >= a.Lq;
     const unsigned long long seed = a.pdrop > 0.f ? rp_seed(a) : 0ull;
-    rp_zero_pad<T, DP, 0>(Ks);
-    rp_zero_pad<T, DP, 0>(Vs);
+    rp_zero_pad<T, DP, 0>(Ks, a.D, tid);
+    rp_zero_pad<T, DP, 0>(Vs, a.D, tid);
 
     RpTile<T, DP> kt, vt;
+    kt.init(a.sk.t, a.D, tid);
+    vt.init(a.sv.t, a.D, tid);
     RpWindow wt;
     unsigned long long valid = 0ull;
     int byte = 0, ck_lo = 0, n_win = 0, base = 0;
     auto fetch = [&](int t) {
         const int k0 = t * RP_TILE;
         byte = rp_mask_byte(a, b, k0);
-        kt.fetch(kp, a.sk.t, k0, a.Lk, a.D);
-        vt.fetch(vp, a.sv.t, k0, a.Lk, a.D);
+        kt.fetch(kp, a.sk.t, k0, a.Lk, a.D, tid);
+        vt.fetch(vp, a.sv.t, k0, a.Lk, a.D, tid);
         ck_lo = rp_c(a, k0);
         base = ck_lo - cq_hi + a.off;
         n_win = rp_c(a, min(k0 + RP_TILE, a.Lk) - 1) - ck_lo + cq_hi - cq_lo + 1;
-        wt.fetch(bias + base, n_win);
+        wt.fetch(bias + base, n_win, tid);
     };
+    const int t1 = a.tiles;
     fetch(0);
-    for (int t = 0; t < a.tiles; ++t) {
-        __syncthreads();
+    for (int t = 0; t < t1; ++t) {
+        rp_barrier();
         valid = rp_valid(a, t * RP_TILE, byte);
-        kt.template put<0>(Ks, valid, a.D);
-        vt.template put<0>(Vs, valid, a.D);
-        wt.put(bw, bias + base, n_win);
-        if (threadIdx.x < RP_TILE) ck[threadIdx.x] = 4 * (rp_c(a, min(t * RP_TILE + (int)threadIdx.x, a.Lk - 1)) - ck_lo);
-        __syncthreads();
-        if (t + 1 < a.tiles) fetch(t + 1);
+        kt.template put<0>(Ks, valid, a.D, tid);
+        vt.template put<0>(Vs, valid, a.D, tid);
+        wt.put(bw, bias + base, n_win, tid);
+        if (tid < RP_TILE) {
+            ck[tid] = 4 * (rp_c(a, min(t * RP_TILE + tid, a.Lk - 1)) - ck_lo);
+            cap[tid] = (valid >> tid) & 1 ? INFINITY : -INFINITY;
+        }
+        rp_barrier();
+        if (t + 1 < t1) fetch(t + 1);
         if (idle || valid == 0ull) continue;
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
@@ -571,15 +694,23 @@ __global__ __launch_bounds__(256) void relpos_bwd_q_kernel(RpArgs a) {
                         ds[e][i] = Op::dot(vf, gf[i][c], ds[e][i]);
                     }
                 }
+            typename Op::TFrag kt_[Dim::DB];   // requested ahead of the exponentials
+            if constexpr (Dim::EARLY) {
+#pragma unroll
+                for (int d = 0; d < Dim::DB; ++d) {
+                    const T* k0 = Ks + (kk * 32 + g * 4) * LD + d * 16;
+                    kt_[d] = Op::load_t(k0, k0 + 16 * LD, LD, l);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
             if (valid != ~0ull) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const unsigned bits = (unsigned)(valid >> ((2 * kk + e) * 16 + g * 4));
+                    const rp_f32x4 c4 = *reinterpret_cast<const rp_f32x4*>(cap + (2 * kk + e) * 16 + g * 4);
 #pragma unroll
                     for (int i = 0; i < QB; ++i)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (!((bits >> r) & 1)) s[e][i][r] = -INFINITY;
+                        for (int r = 0; r < 4; ++r) s[e][i][r] = fminf(s[e][i][r], c4[r]);
                 }
             }
             if (a.pdrop > 0.f) {
@@ -592,26 +723,43 @@ __global__ __launch_bounds__(256) void relpos_bwd_q_kernel(RpArgs a) {
                         for (int r = 0; r < 4; ++r) ds[e][i][r] *= rp_drop(seed, at + e * 16 + r, a.pdrop);
                 }
             }
+            if (far) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+                for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int i = 0; i < QB; ++i)
+                    for (int i = 0; i < QB; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float p = __builtin_amdgcn_exp2f(fmaf(s[e][i][r] - mx[i], a.sl2, -lg[i]));
-                        const float d = p * (ds[e][i][r] - D0[i]);
-                        extra[i] += d;
-                        ds[e][i][r] = d;
-                    }
+                        for (int r = 0; r < 4; ++r) s[e][i][r] = __builtin_amdgcn_exp2f(fmaf(s[e][i][r] - mx[i], a.sl2, -lg[i]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int i = 0; i < QB; ++i)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[e][i][r] = __builtin_amdgcn_exp2f(fmaf(s[e][i][r], a.sl2, -shift[i]));
+            }
+#pragma unroll
+            for (int i = 0; i < QB; ++i) {
+                float part[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) ds[e][i][r] = s[e][i][r] * (ds[e][i][r] - D0[i]);
+                    part[e] = (ds[e][i][0] + ds[e][i][1]) + (ds[e][i][2] + ds[e][i][3]);
+                }
+                extra[i] += part[0] + part[1];
+            }
             typename Op::Pair p[QB];
 #pragma unroll
             for (int i = 0; i < QB; ++i) p[i] = Op::pack(ds[0][i], ds[1][i]);
 #pragma unroll
             for (int d = 0; d < Dim::DB; ++d) {
-                const T* k0 = Ks + (kk * 32 + g * 4) * LD + d * 16;
-                const typename Op::TFrag kf = Op::load_t(k0, k0 + 16 * LD, LD, l);
+                if constexpr (!Dim::EARLY) {
+                    const T* k0 = Ks + (kk * 32 + g * 4) * LD + d * 16;
+                    kt_[d] = Op::load_t(k0, k0 + 16 * LD, LD, l);
+                }
 #pragma unroll
-                for (int i = 0; i < QB; ++i) dq[i][d] = Op::dot_t(kf, p[i], dq[i][d]);
+                for (int i = 0; i < QB; ++i) dq[i][d] = Op::dot_t(kt_[d], p[i], dq[i][d]);
             }
         }
     }
@@ -643,7 +791,7 @@ __global__ __launch_bounds__(256) void relpos_bwd_q_kernel(RpArgs a) {
 // 11.5 cycles a wave instruction and floats at 194 (measured): 481 -> 152 us for this kernel on 38x38 maps, batch 4, 8 heads of 64.
 // ------------------------------------------------------------------------------------------------
 template <typename T, int DP, int KB>
-__global__ __launch_bounds__(256) void relpos_bwd_kv_kernel(RpArgs a) {
+__global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) void relpos_bwd_kv_kernel(RpArgs a) {
     typedef RpOp<T> Op;
     typedef RpDim<T, DP> Dim;
     constexpr int LD = Dim::LD, KT = 64 * KB;
@@ -654,12 +802,13 @@ __global__ __launch_bounds__(256) void relpos_bwd_kv_kernel(RpArgs a) {
     T* Gs = Qs + TILE;
     float* ms = reinterpret_cast<float*>(Gs + TILE);
     float* ls = ms + RP_TILE;
-    float* dsm = ls + RP_TILE;
+    float* sh = ls + RP_TILE;
+    float* dsm = sh + RP_TILE;
     int* cqs = reinterpret_cast<int*>(dsm + RP_TILE);
     float* bw = reinterpret_cast<float*>(cqs + RP_TILE);   // ring, acc_mask + 1 floats
     const int ring = a.acc_mask + 1;
     double* acc = reinterpret_cast<double*>(bw + ring);    // [4 waves][ring]
-    const int ktiles = (a.Lk + KT - 1) / KT, id = rp_block(blockIdx.x, gridDim.x);
+    const int ktiles = (a.Lk + KT - 1) / KT, id = rp_block(a, ktiles);
     if (id >= a.B * a.heads * ktiles) return;
     const int bh = id / ktiles, b = bh / a.heads, h = bh - b * a.heads, k0 = (id - bh * ktiles) * KT;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane & 15, g = lane >> 4;
@@ -693,11 +842,18 @@ __global__ __launch_bounds__(256) void relpos_bwd_kv_kernel(RpArgs a) {
 #pragma unroll
         for (int d = 0; d < Dim::DB; ++d) dk[j][d] = dv[j][d] = rp_f32x4{0.f, 0.f, 0.f, 0.f};
     }
+#pragma unroll
+    for (int j = 0; j < KB; ++j)
+#pragma unroll
+        for (int c = 0; c < Dim::NCH; ++c) {
+            rp_settle(kf[j][c]);
+            rp_settle(vf[j][c]);
+        }
     any_bad = __any(any_bad);
     any_ok = __any(any_ok);
     const unsigned long long seed = a.pdrop > 0.f ? rp_seed(a) : 0ull;
-    rp_zero_pad<T, DP, INS>(Qs);
-    rp_zero_pad<T, DP, INS>(Gs);
+    rp_zero_pad<T, DP, INS>(Qs, a.D, threadIdx.x);
+    rp_zero_pad<T, DP, INS>(Gs, a.D, threadIdx.x);
     if (grad_bias)
         for (int i = threadIdx.x; i < 4 * ring; i += 256) acc[i] = 0.0;
 
@@ -712,14 +868,16 @@ __global__ __launch_bounds__(256) void relpos_bwd_kv_kernel(RpArgs a) {
     };
 
     RpTile<T, DP> qt, gt;
+    qt.init(a.sq.t, a.D, threadIdx.x);
+    gt.init(gst, a.D, threadIdx.x);
     float2 sr = make_float2(0.f, 0.f);
     float dr = 0.f, br[2];
     int b_lo = 0, b_hi = 0;
     const int qtiles = (a.Lq + RP_TILE - 1) / RP_TILE;
     auto fetch = [&](int t) {
         const int first = t * RP_TILE, left = a.Lq - first;
-        qt.fetch(qp, a.sq.t, first, a.Lq, a.D);
-        gt.fetch(gp, gst, first, a.Lq, a.D);
+        qt.fetch(qp, a.sq.t, first, a.Lq, a.D, threadIdx.x);
+        gt.fetch(gp, gst, first, a.Lq, a.D, threadIdx.x);
         if (threadIdx.x < RP_TILE) {
             const bool in = (int)threadIdx.x < left;
             sr = in ? stat[first + threadIdx.x] : make_float2(0.f, INFINITY);
@@ -736,7 +894,7 @@ __global__ __launch_bounds__(256) void relpos_bwd_kv_kernel(RpArgs a) {
     for (int t = 0; t < qtiles; ++t) {
         const int first = t * RP_TILE, q_hi = min(first + RP_TILE, a.Lq) - 1;
         const int cq_lo = rp_c(a, a.q_start + first);
-        __syncthreads();
+        rp_barrier();
         if (grad_bias) {
             const int reach = ck_hi - cq_lo;
             flush(reach, top);
@@ -744,8 +902,8 @@ __global__ __launch_bounds__(256) void relpos_bwd_kv_kernel(RpArgs a) {
         }
         const int left = a.Lq - first;
         const unsigned long long rows = left >= 64 ? ~0ull : (1ull << left) - 1;
-        qt.template put<INS>(Qs, rows, a.D);
-        gt.template put<INS>(Gs, rows, a.D);
+        qt.template put<INS>(Qs, rows, a.D, threadIdx.x);
+        gt.template put<INS>(Gs, rows, a.D, threadIdx.x);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             if (b_lo + i * 256 + (int)threadIdx.x <= b_hi) bw[(b_lo + i * 256 + threadIdx.x) & a.acc_mask] = br[i];
@@ -753,10 +911,12 @@ __global__ __launch_bounds__(256) void relpos_bwd_kv_kernel(RpArgs a) {
         if (threadIdx.x < RP_TILE) {
             ms[threadIdx.x] = sr.x;
             ls[threadIdx.x] = sr.y;
+            sh[threadIdx.x] = fmaf(sr.x, a.sl2, sr.y);
             dsm[threadIdx.x] = dr;
             cqs[threadIdx.x] = rp_c(a, a.q_start + min(first + (int)threadIdx.x, q_hi));
         }
-        __syncthreads();
+        rp_barrier();
+        const bool far = __any(fabsf(ms[lane]) * a.sl2 > RP_FAR);
         if (t + 1 < qtiles) fetch(t + 1);
         if (!any_ok) continue;
 #pragma unroll
@@ -812,16 +972,25 @@ __global__ __launch_bounds__(256) void relpos_bwd_kv_kernel(RpArgs a) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int row = g * 16 + (2 * kk + e) * 4;
-                const rp_f32x4 m4 = *reinterpret_cast<const rp_f32x4*>(ms + row);
-                const rp_f32x4 l4 = *reinterpret_cast<const rp_f32x4*>(ls + row);
                 const rp_f32x4 d4 = *reinterpret_cast<const rp_f32x4*>(dsm + row);
+                if (far) {
+                    const rp_f32x4 m4 = *reinterpret_cast<const rp_f32x4*>(ms + row);
+                    const rp_f32x4 l4 = *reinterpret_cast<const rp_f32x4*>(ls + row);
+#pragma unroll
+                    for (int j = 0; j < KB; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) p[e][j][r] = __builtin_amdgcn_exp2f(fmaf(p[e][j][r] - m4[r], a.sl2, -l4[r]));
+                } else {
+                    const rp_f32x4 s4 = *reinterpret_cast<const rp_f32x4*>(sh + row);
+#pragma unroll
+                    for (int j = 0; j < KB; ++j)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) p[e][j][r] = __builtin_amdgcn_exp2f(fmaf(p[e][j][r], a.sl2, -s4[r]));
+                }
 #pragma unroll
                 for (int j = 0; j < KB; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        p[e][j][r] = __builtin_amdgcn_exp2f(fmaf(p[e][j][r] - m4[r], a.sl2, -l4[r]));
-                        ds[e][j][r] = p[e][j][r] * (ds[e][j][r] - d4[r]);
-                    }
+                    for (int r = 0; r < 4; ++r) ds[e][j][r] = p[e][j][r] * (ds[e][j][r] - d4[r]);
             }
             if (grad_bias) {
 #pragma unroll
@@ -861,7 +1030,7 @@ __global__ __launch_bounds__(256) void relpos_bwd_kv_kernel(RpArgs a) {
         }
     }
     if (grad_bias) {
-        __syncthreads();
+        rp_barrier();
         flush(slab_lo - 1, top);
     }
 #pragma unroll
@@ -954,7 +1123,7 @@ static int rp_splits(long long wgs, int tiles) {
 }
 static int rp_fwd_splits(int dtype, int B, int heads, int Lq, int Lk, int D, int& cols) {
     const long long bh = (long long)B * heads;
-    cols = rp_cols(dtype, rp_dp(D), bh, Lq, 128);
+    cols = rp_cols(dtype, rp_dp(D), bh, Lq, 96);
     return rp_splits(bh * ((Lq + 64 * cols - 1) / (64 * cols)), (Lk + RP_TILE - 1) / RP_TILE);
 }
 
@@ -969,11 +1138,12 @@ static int rp_launch(const char* name, K kernel, dim3 grid, size_t lds, const Rp
     return 0;
 }
 
-enum { RP_FWD, RP_BWD_Q, RP_BWD_KV };
-
+// cols: 16-wide columns of a wave
 template <typename T, int DP, int COLS>
 static int rp_run(int what, const char* name, dim3 grid, size_t lds, const RpArgs& a, hipStream_t s) {
-    if (what == RP_FWD) return rp_launch(name, relpos_fwd_kernel<T, DP, COLS>, grid, lds, a, s);
+    if constexpr (COLS == 1 || DP <= 96) {
+        if (what == RP_FWD) return rp_launch(name, relpos_fwd_kernel<T, DP, COLS>, grid, lds, a, s);
+    }
     if constexpr (COLS == 1 || DP <= 64) {
         if (what == RP_BWD_Q) return rp_launch(name, relpos_bwd_q_kernel<T, DP, COLS>, grid, lds, a, s);
         return rp_launch(name, relpos_bwd_kv_kernel<T, DP, COLS>, grid, lds, a, s);
@@ -985,8 +1155,8 @@ static int rp_run(int what, const char* name, dim3 grid, size_t lds, const RpArg
 static int rp_dispatch(int what, const char* name, int dtype, int cols, dim3 grid, size_t lds, const RpArgs& a, hipStream_t s) {
 #define RP_CASE(DP_)                                                                                      \
     case DP_:                                                                                             \
-        if (dtype == MIA_F32) return rp_run<float, DP_, 1>(what, name, grid, lds, a, s);                  \
-        return cols == 2 ? rp_run<bf16_t, DP_, 2>(what, name, grid, lds, a, s)                            \
+        if (dtype == MIA_F32) return rp_run<float, DP_, 1>(what, name, grid, lds, a, s);          \
+        return cols == 2 ? rp_run<bf16_t, DP_, 2>(what, name, grid, lds, a, s)                    \
                          : rp_run<bf16_t, DP_, 1>(what, name, grid, lds, a, s);
     switch (rp_dp(a.D)) {
         RP_CASE(16)
@@ -998,6 +1168,12 @@ static int rp_dispatch(int what, const char* name, int dtype, int cols, dim3 gri
     }
 #undef RP_CASE
     return -1;
+}
+
+// LDS of a query kernel: two tiles, the keys' c and caps, the bias window
+static size_t rp_query_lds(const RpArgs& a, int dtype, int DP, int cols, int tokens) {
+    const int win = rp_span(a, RP_TILE, tokens) + rp_span(a, 64 * cols, tokens) + 1;
+    return 2 * (size_t)RP_TILE * rp_ld(dtype, DP) * rp_es(dtype) + RP_TILE * 8 + (size_t)win * 4;
 }
 
 static dim3 rp_grid(long long blocks, int splits) { return dim3((unsigned)((blocks + 7) / 8 * 8), (unsigned)splits); }
@@ -1025,6 +1201,7 @@ static int rp_aligned(const char* name, int dtype, const void* p, const RpStride
     const long long per = dtype == MIA_BF16 ? 8 : 4;
     MIA_CHECK_ARG(((uintptr_t)p & 15) == 0 && s.b % per == 0 && s.t % per == 0 && s.h % per == 0,
                   "%s: rows must start at multiples of 16 bytes", name);
+    MIA_CHECK_ARG(s.t >= 0 && s.t < (1ll << 24), "%s: token stride %lld is not in 0 .. 2^24 - 1", name, s.t);
     return 0;
 }
 
@@ -1090,8 +1267,7 @@ extern "C" int mia_relpos_fwd(int dtype, const void* q, const void* k, const voi
         a.pml = ws + (long long)a.splits * rows * D;
     }
     const int tokens = height * width, DP = rp_dp(D);
-    a.win = rp_span(a, RP_TILE, tokens) + rp_span(a, 64 * cols, tokens) + 1;
-    const size_t lds = 2 * (size_t)RP_TILE * rp_ld(dtype, DP) * rp_es(dtype) + RP_TILE * 4 + (size_t)a.win * 4;
+    const size_t lds = rp_query_lds(a, dtype, DP, cols, tokens);
     const int rc = rp_dispatch(RP_FWD, "mia_relpos_fwd", dtype, cols, rp_grid((long long)B * heads * ((Lq + 64 * cols - 1) / (64 * cols)), a.splits), lds, a, s);
     if (rc || a.splits == 1) return rc;
     const dim3 threads((D + 63) / 64 * 64);
@@ -1145,9 +1321,8 @@ extern "C" int mia_relpos_bwd(int dtype, const void* q, const void* k, const voi
     const int tokens = height * width, DP = rp_dp(D);
     const size_t tile = (size_t)RP_TILE * rp_ld(dtype, DP) * rp_es(dtype);
     const int qc = rp_cols(dtype, DP, bh, Lq, 64);
-    a.win = rp_span(a, RP_TILE, tokens) + rp_span(a, 64 * qc, tokens) + 1;
-    if (rp_dispatch(RP_BWD_Q, "mia_relpos_bwd", dtype, qc, rp_grid(bh * ((Lq + 64 * qc - 1) / (64 * qc)), 1), 2 * tile + RP_TILE * 4 + (size_t)a.win * 4, a, s))
-        return -2;
+    const size_t q_lds = rp_query_lds(a, dtype, DP, qc, tokens);
+    if (int rc = rp_dispatch(RP_BWD_Q, "mia_relpos_bwd", dtype, qc, rp_grid(bh * ((Lq + 64 * qc - 1) / (64 * qc)), 1), q_lds, a, s)) return rc;
     const int kc = rp_kv_cols(dtype, D, bh, Lk), ktiles = (Lk + 64 * kc - 1) / (64 * kc);
     int ring = 64;
     while (ring < rp_span(a, RP_TILE, tokens) + rp_span(a, 64 * kc, tokens) + 1) ring *= 2;
@@ -1158,8 +1333,8 @@ extern "C" int mia_relpos_bwd(int dtype, const void* q, const void* k, const voi
         a.slab_ld = rp_slab_ld(a, tokens, kc);
         a.slab = per_off + (long long)heads * a.n_off;
     }
-    const size_t kv_lds = 2 * (tile + 256) + 4 * RP_TILE * 4 + (size_t)ring * (dtable ? 4 + 4 * 8 : 4);
-    if (rp_dispatch(RP_BWD_KV, "mia_relpos_bwd", dtype, kc, rp_grid(bh * ktiles, 1), kv_lds, a, s)) return -2;
+    const size_t kv_lds = 2 * (tile + 256) + 5 * RP_TILE * 4 + (size_t)ring * (dtable ? 4 + 4 * 8 : 4);
+    if (int rc = rp_dispatch(RP_BWD_KV, "mia_relpos_bwd", dtype, kc, rp_grid(bh * ktiles, 1), kv_lds, a, s)) return rc;
     if (!dtable) return 0;
     MIA_LAUNCH(relpos_offsets_kernel, dim3(cdiv(a.n_off, 64), heads), dim3(256), 0, s, a.slab, a, ktiles, 64 * kc, per_off);
     MIA_CHECK_LAUNCH("mia_relpos_bwd");

@@ -81,7 +81,7 @@ def _rows(t):
     bytes), else a contiguous copy; and its (batch, token, head) strides in elements."""
     per = 16 // t.element_size()
     st = [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride())]
-    if (t.stride(3) != 1 and t.shape[3] != 1) or any(s % per or s < 0 for s in st) or t.data_ptr() % 16:
+    if (t.stride(3) != 1 and t.shape[3] != 1) or any(s % per or s < 0 for s in st) or st[1] >= 1 << 24 or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:       # a contiguous view that starts in between
             t = t.clone()
