@@ -28,7 +28,7 @@ typedef __attribute__((ext_vector_type(8))) short rp_s16x8;
 typedef __attribute__((ext_vector_type(8))) __bf16 rp_bf16x8;
 
 #define RP_LOG2E 1.4426950408889634f
-#define RP_TILE 64          // tokens of a staged tile
+#define RP_TILE 64          // tokens that one round of products works on
 // Largest maximum, in units of the exponent, up to which P = exp2(acc * sl2 - shift) is formed by one FMA with shift rounded to
 // fp32 (64 * 2^-24 = 4e-6 relative in P at worst); rows beyond it subtract first.
 #define RP_FAR 64.f
@@ -156,7 +156,9 @@ struct RpDim {
     static constexpr int NCH = (DP + RpOp<T>::CHUNK - 1) / RpOp<T>::CHUNK;   // operand chunks of a row
     static constexpr int LD = NCH * RpOp<T>::CHUNK + PER;                    // LDS row stride: 16 bytes of padding
     static constexpr int CPR = DP / PER;                                     // 16-byte pieces of a staged row
-    static constexpr int NST = (RP_TILE * CPR + 255) / 256;                  // pieces per thread
+    // keys that the query kernels stage between two barriers: the fixed cost of a round of staging is a third of a 64-key tile's
+    // instructions, so two tiles share it where registers and LDS allow
+    static constexpr int HALVES = ES == 2 && DP <= 64 ? 2 : 1, STAGE = HALVES * RP_TILE;
     static constexpr int DB = DP / 16;                                       // 16-wide output blocks
     static constexpr bool EARLY = ES == 2 && DP <= 64;                       // registers for operands requested ahead
 };
@@ -175,22 +177,22 @@ __device__ __forceinline__ void rp_row_frags(const T* row, bool ok, int D, int g
 // One tile of rows on its way to LDS, kept in registers while the tile before it is worked on; a group of 256 threads, tid its
 // thread. The loads are unconditional (rows past the end read the last row, columns past D the first): what counts is
 // decided when the tile is put down. Their addresses are one scalar per tile plus 32-bit offsets that never change.
-template <typename T, int DP>
+template <typename T, int DP, int ROWS>
 struct RpTile {
-    static constexpr int CPR = RpDim<T, DP>::CPR, NST = RpDim<T, DP>::NST;
+    static constexpr int CPR = RpDim<T, DP>::CPR, NST = (ROWS * CPR + 255) / 256, WORDS = ROWS / 64;   // 16-byte pieces per thread
     uint4 r[NST];
     unsigned off[NST];   // bytes
     __device__ __forceinline__ void init(long long st, int D, int tid) {
 #pragma unroll
         for (int i = 0; i < NST; ++i) {
-            const int id = i * 256 + tid, row = min(id / CPR, RP_TILE - 1), col = (id % CPR) * RpOp<T>::PER;
+            const int id = i * 256 + tid, row = min(id / CPR, ROWS - 1), col = (id % CPR) * RpOp<T>::PER;
             off[i] = ((unsigned)row * (unsigned)st + (unsigned)(col < D ? col : 0)) * (unsigned)sizeof(T);
         }
     }
-    // rows first .. first + 63 of src (row stride st), of `limit` rows in all
+    // rows first .. first + ROWS - 1 of src (row stride st), of `limit` rows in all
     __device__ __forceinline__ void fetch(const T* src, long long st, int first, int limit, int D, int tid) {
         const char* base = reinterpret_cast<const char*>(src + (long long)first * st);
-        if (first + RP_TILE <= limit) {
+        if (first + ROWS <= limit) {
 #pragma unroll
             for (int i = 0; i < NST; ++i) r[i] = *reinterpret_cast<const uint4*>(base + off[i]);
         } else {
@@ -201,23 +203,27 @@ struct RpTile {
             }
         }
     }
-    // bit i of valid clear: row i becomes zeros. Columns past D are not written (rp_zero_pad). INS: extra elements after every
+    // bit i of valid (64 to a word) clear: row i becomes zeros. Columns past D are not written (rp_zero_pad). INS: extra elements after every
     // 16 rows
     template <int INS>
-    __device__ __forceinline__ void put(T* lds, unsigned long long valid, int D, int tid) const {
-        if (valid == ~0ull) {
+    __device__ __forceinline__ void put(T* lds, const unsigned long long (&valid)[WORDS], int D, int tid) const {
+        if (valid[0] == ~0ull && valid[WORDS - 1] == ~0ull) {
 #pragma unroll
             for (int i = 0; i < NST; ++i)
                 if (used(i, D, tid)) *place<INS>(lds, i, tid) = r[i];
         } else {
 #pragma unroll
             for (int i = 0; i < NST; ++i)
-                if (used(i, D, tid)) *place<INS>(lds, i, tid) = (valid >> ((i * 256 + tid) / CPR)) & 1 ? r[i] : make_uint4(0u, 0u, 0u, 0u);
+                if (used(i, D, tid)) {
+                    const int row = (i * 256 + tid) / CPR;
+                    const unsigned long long word = WORDS == 1 || row < 64 ? valid[0] : valid[WORDS - 1];
+                    *place<INS>(lds, i, tid) = (word >> (row & 63)) & 1 ? r[i] : make_uint4(0u, 0u, 0u, 0u);
+                }
         }
     }
     static __device__ __forceinline__ bool used(int i, int D, int tid) {
         const int id = i * 256 + tid;
-        return ((RP_TILE * CPR) % 256 == 0 || id < RP_TILE * CPR) && (id % CPR) * RpOp<T>::PER < D;
+        return ((ROWS * CPR) % 256 == 0 || id < ROWS * CPR) && (id % CPR) * RpOp<T>::PER < D;
     }
     template <int INS>
     static __device__ __forceinline__ uint4* place(T* lds, int i, int tid) {
@@ -253,12 +259,12 @@ constexpr int rp_waves(int what, bool half, int DP, int cols) {
 }
 
 // columns between D and the padded reduction length are read as operands and never staged: zero once
-template <typename T, int DP, int INS>
+template <typename T, int DP, int INS, int ROWS>
 __device__ __forceinline__ void rp_zero_pad(T* lds, int D, int tid) {
     const int pad = RpDim<T, DP>::NCH * RpOp<T>::CHUNK - D;
     if (pad > 0)
 #pragma unroll 1
-        for (int i = tid; i < RP_TILE * pad; i += 256) {
+        for (int i = tid; i < ROWS * pad; i += 256) {
             const int row = i / pad;
             lds[row * RpDim<T, DP>::LD + (row >> 4) * INS + D + (i - row * pad)] = from_f32<T>(0.f);
         }
@@ -354,14 +360,14 @@ template <typename T, int DP, int QB>
 __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void relpos_fwd_kernel(RpArgs a) {
     typedef RpOp<T> Op;
     typedef RpDim<T, DP> Dim;
-    constexpr int LD = Dim::LD, QT = 64 * QB;
+    constexpr int LD = Dim::LD, QT = 64 * QB, ST = Dim::STAGE, HV = Dim::HALVES;
     extern __shared__ __attribute__((aligned(16))) char rp_sm[];
     const int tid = threadIdx.x;
     T* Ks = reinterpret_cast<T*>(rp_sm);
-    T* Vs = Ks + RP_TILE * LD;
-    int* ck = reinterpret_cast<int*>(Vs + RP_TILE * LD);
-    float* cap = reinterpret_cast<float*>(ck + RP_TILE);   // scores end at this: -inf for a key that does not exist
-    float* bw = cap + RP_TILE;
+    T* Vs = Ks + ST * LD;
+    int* ck = reinterpret_cast<int*>(Vs + ST * LD);
+    float* cap = reinterpret_cast<float*>(ck + ST);   // scores end at this: -inf for a key that does not exist
+    float* bw = cap + ST;
     const int qtiles = (a.Lq + QT - 1) / QT, id = rp_block(a, qtiles);
     if (id >= a.B * a.heads * qtiles) return;
     const int bh = id / qtiles, b = bh / a.heads, h = bh - b * a.heads, q0 = (id - bh * qtiles) * QT;
@@ -392,23 +398,24 @@ __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void
         for (int c = 0; c < Dim::NCH; ++c) rp_settle(qf[i][c]);
     const bool idle = q0 + wave * QB * 16 >= a.Lq;   // a wave without queries only helps to stage
     const unsigned long long seed = a.pdrop > 0.f ? rp_seed(a) : 0ull;
-    rp_zero_pad<T, DP, 0>(Ks, a.D, tid);
-    rp_zero_pad<T, DP, 0>(Vs, a.D, tid);
+    rp_zero_pad<T, DP, 0, Dim::STAGE>(Ks, a.D, tid);
+    rp_zero_pad<T, DP, 0, Dim::STAGE>(Vs, a.D, tid);
 
-    RpTile<T, DP> kt, vt;
+    RpTile<T, DP, ST> kt, vt;
     kt.init(a.sk.t, a.D, tid);
     vt.init(a.sv.t, a.D, tid);
     RpWindow wt;
-    unsigned long long valid = 0ull;
-    int byte = 0, ck_lo = 0, n_win = 0, base = 0;
+    unsigned long long valid[HV];
+    int byte[HV], ck_lo = 0, n_win = 0, base = 0;
     auto fetch = [&](int t) {
-        const int k0 = t * RP_TILE;
-        byte = rp_mask_byte(a, b, k0);
+        const int k0 = t * ST;
+#pragma unroll
+        for (int i = 0; i < HV; ++i) byte[i] = rp_mask_byte(a, b, k0 + 64 * i);
         kt.fetch(kp, a.sk.t, k0, a.Lk, a.D, tid);
         vt.fetch(vp, a.sv.t, k0, a.Lk, a.D, tid);
         ck_lo = rp_c(a, k0);
         base = ck_lo - cq_hi + a.off;
-        n_win = rp_c(a, min(k0 + RP_TILE, a.Lk) - 1) - ck_lo + cq_hi - cq_lo + 1;
+        n_win = rp_c(a, min(k0 + ST, a.Lk) - 1) - ck_lo + cq_hi - cq_lo + 1;
         wt.fetch(bias + base, n_win, tid);
     };
     const int t1 = (int)((long long)a.tiles * (blockIdx.y + 1) / a.splits);
@@ -416,21 +423,28 @@ __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void
     if (t < t1) fetch(t);
     for (; t < t1; ++t) {
         rp_barrier();
-        valid = rp_valid(a, t * RP_TILE, byte);
+#pragma unroll
+        for (int i = 0; i < HV; ++i) valid[i] = rp_valid(a, t * ST + 64 * i, byte[i]);
         kt.template put<0>(Ks, valid, a.D, tid);
         vt.template put<0>(Vs, valid, a.D, tid);
         wt.put(bw, bias + base, n_win, tid);
-        if (tid < RP_TILE) {
-            ck[tid] = 4 * (rp_c(a, min(t * RP_TILE + tid, a.Lk - 1)) - ck_lo);
-            cap[tid] = (valid >> tid) & 1 ? INFINITY : -INFINITY;
+        if (tid < ST) {
+            ck[tid] = 4 * (rp_c(a, min(t * ST + tid, a.Lk - 1)) - ck_lo);
+            cap[tid] = ((tid < 64 ? valid[0] : valid[HV - 1]) >> (tid & 63)) & 1 ? INFINITY : -INFINITY;
         }
         rp_barrier();
         if (t + 1 < t1) fetch(t + 1);
-        if (idle || valid == 0ull) continue;
+        if (idle) continue;
+#pragma unroll 1
+        for (int hv = 0; hv < HV; ++hv) {
+        const unsigned long long here = HV == 1 || hv == 0 ? valid[0] : valid[HV - 1];
+        if (here == 0ull) continue;
+        const T *Kh = Ks + hv * RP_TILE * LD, *Vh = Vs + hv * RP_TILE * LD;
+        const int* ckh = ck + hv * RP_TILE;
         rp_f32x4 s[4][QB];
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
-            const int4 c4 = *reinterpret_cast<const int4*>(ck + kb * 16 + g * 4);
+            const int4 c4 = *reinterpret_cast<const int4*>(ckh + kb * 16 + g * 4);
 #pragma unroll
             for (int i = 0; i < QB; ++i) s[kb][i] = rp_bias4(bw, c4, cq[i]);
         }
@@ -438,7 +452,7 @@ __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void
         for (int c = 0; c < Dim::NCH; ++c)
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
-                const typename Op::Frag kf = *reinterpret_cast<const typename Op::Frag*>(Ks + (kb * 16 + l) * LD + c * Op::CHUNK + g * Op::PER);
+                const typename Op::Frag kf = *reinterpret_cast<const typename Op::Frag*>(Kh + (kb * 16 + l) * LD + c * Op::CHUNK + g * Op::PER);
 #pragma unroll
                 for (int i = 0; i < QB; ++i) s[kb][i] = Op::dot(kf, qf[i][c], s[kb][i]);
             }
@@ -447,7 +461,7 @@ __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void
         auto values = [&](int kk) {
 #pragma unroll
             for (int d = 0; d < Dim::DB; ++d) {
-                const T* v0 = Vs + (kk * 32 + g * 4) * LD + d * 16;
+                const T* v0 = Vh + (kk * 32 + g * 4) * LD + d * 16;
                 vf[kk][d] = Op::load_t(v0, v0 + 16 * LD, LD, l);
             }
         };
@@ -455,10 +469,10 @@ __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void
             values(0);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if (valid != ~0ull) {
+        if (here != ~0ull) {
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
-                const rp_f32x4 c4 = *reinterpret_cast<const rp_f32x4*>(cap + kb * 16 + g * 4);
+                const rp_f32x4 c4 = *reinterpret_cast<const rp_f32x4*>(cap + hv * RP_TILE + kb * 16 + g * 4);
 #pragma unroll
                 for (int i = 0; i < QB; ++i)
 #pragma unroll
@@ -499,7 +513,7 @@ __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void
             for (int kb = 0; kb < 4; ++kb) part[kb] = (s[kb][i][0] + s[kb][i][1]) + (s[kb][i][2] + s[kb][i][3]);
             sum[i] += (part[0] + part[1]) + (part[2] + part[3]);
             if (a.pdrop > 0.f) {
-                const unsigned long long at = ((unsigned long long)bh * a.Lq + qi[i]) * a.Lk + t * RP_TILE + g * 4;
+                const unsigned long long at = ((unsigned long long)bh * a.Lq + qi[i]) * a.Lk + t * ST + hv * RP_TILE + g * 4;
 #pragma unroll
                 for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
@@ -517,6 +531,7 @@ __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void
             for (int d = 0; d < Dim::DB; ++d)
 #pragma unroll
                 for (int i = 0; i < QB; ++i) o[i][d] = Op::dot_t(vf[kk][d], p[i], o[i][d]);
+        }
         }
     }
 #pragma unroll
@@ -548,24 +563,51 @@ __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void
     }
 }
 
-// joins the partial results of a split forward: one workgroup of D threads a row
-template <typename T>
-__global__ void relpos_join_kernel(RpArgs a) {
-    const size_t rows = (size_t)a.B * a.heads * a.Lq, row = blockIdx.x;
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.pml[2 * (s * rows + row)]);
-    const float use = m == -INFINITY ? 0.f : m;
-    float total = 0.f, acc = 0.f;
-    const int d = threadIdx.x;
-    for (int s = 0; s < a.splits; ++s) {
-        const size_t p = s * rows + row;
-        const float w = __builtin_amdgcn_exp2f((a.pml[2 * p] - use) * a.sl2);
-        total = fmaf(a.pml[2 * p + 1], w, total);
-        if (d < a.D) acc = fmaf(a.po[p * a.D + d], w, acc);
+// Joins the partial results of kernels that were split over the tokens they walk: a thread per four channels of a row, the
+// partials of one row added in order of the splits.
+//   RP_FWD    the running maxima and sums of the splits, their unnormalised outputs
+//   RP_BWD_Q  dQ and the sums that make D exact
+//   RP_BWD_KV dK and dV
+template <typename T, int WHAT>
+__global__ __launch_bounds__(256) void relpos_join_kernel(RpArgs a) {
+    const int vecs = a.D >> 2, tokens = WHAT == RP_BWD_KV ? a.Lk : a.Lq;
+    const size_t rows = (size_t)a.B * a.heads * tokens, i = (size_t)blockIdx.x * 256 + threadIdx.x, row = i / vecs;
+    if (row >= rows) return;
+    const int d = (int)(i - row * vecs) * 4;
+    const size_t bh = row / tokens, b = bh / a.heads, h = bh - b * a.heads, t = row - bh * tokens;
+    if constexpr (WHAT == RP_BWD_KV) {
+        const size_t part = rows * a.D;
+        rp_f32x4 k = {0.f, 0.f, 0.f, 0.f}, v = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < a.splits; ++s) {
+            const float* p = a.po + 2 * s * part + row * a.D + d;
+            k += *reinterpret_cast<const rp_f32x4*>(p);
+            v += *reinterpret_cast<const rp_f32x4*>(p + part);
+        }
+        store4<T>((T*)a.dk + b * a.sdk.b + t * a.sdk.t + h * a.sdk.h + d, {k[0] * a.scale, k[1] * a.scale, k[2] * a.scale, k[3] * a.scale});
+        store4<T>((T*)a.dv + b * a.sdv.b + t * a.sdv.t + h * a.sdv.h + d, {v[0], v[1], v[2], v[3]});
+    } else {
+        const float2* pml = reinterpret_cast<const float2*>(a.pml);
+        float m = -INFINITY, total = 0.f;
+        if (WHAT == RP_FWD)
+            for (int s = 0; s < a.splits; ++s) m = fmaxf(m, pml[s * rows + row].x);
+        const float use = m == -INFINITY ? 0.f : m;
+        rp_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < a.splits; ++s) {
+            const float2 ml = pml[s * rows + row];
+            const float w = WHAT == RP_FWD ? __builtin_amdgcn_exp2f((ml.x - use) * a.sl2) : 1.f;
+            total = fmaf(ml.y, w, total);
+            acc += *reinterpret_cast<const rp_f32x4*>(a.po + (s * rows + row) * a.D + d) * w;
+        }
+        if (WHAT == RP_FWD) {
+            const float inv = total == 0.f ? 0.f : 1.0f / total;
+            store4<T>((T*)a.o + ((b * a.Lq + t) * a.heads + h) * a.D + d, {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv});
+            if (a.stat && d == 0) a.stat[row] = rp_stat(m, total);
+        } else {
+            store4<T>((T*)a.dq + b * a.sdq.b + t * a.sdq.t + h * a.sdq.h + d,
+                      {acc[0] * a.scale, acc[1] * a.scale, acc[2] * a.scale, acc[3] * a.scale});
+            if (d == 0) a.dsum[row] = pml[row].x + total;
+        }
     }
-    const size_t bh = row / a.Lq, b = bh / a.heads, h = bh - b * a.heads, q = row - bh * a.Lq;
-    if (d < a.D) ((T*)a.o)[((b * a.Lq + q) * a.heads + h) * a.D + d] = from_f32<T>(total == 0.f ? 0.f : acc / total);
-    if (a.stat && d == 0) a.stat[row] = rp_stat(m, total);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -575,14 +617,14 @@ template <typename T, int DP, int QB>
 __global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) void relpos_bwd_q_kernel(RpArgs a) {
     typedef RpOp<T> Op;
     typedef RpDim<T, DP> Dim;
-    constexpr int LD = Dim::LD, QT = 64 * QB;
+    constexpr int LD = Dim::LD, QT = 64 * QB, ST = Dim::STAGE, HV = Dim::HALVES;
     extern __shared__ __attribute__((aligned(16))) char rp_sm[];
     const int tid = threadIdx.x;
     T* Ks = reinterpret_cast<T*>(rp_sm);
-    T* Vs = Ks + RP_TILE * LD;
-    int* ck = reinterpret_cast<int*>(Vs + RP_TILE * LD);
-    float* cap = reinterpret_cast<float*>(ck + RP_TILE);   // scores end at this: -inf for a key that does not exist
-    float* bw = cap + RP_TILE;
+    T* Vs = Ks + ST * LD;
+    int* ck = reinterpret_cast<int*>(Vs + ST * LD);
+    float* cap = reinterpret_cast<float*>(ck + ST);   // scores end at this: -inf for a key that does not exist
+    float* bw = cap + ST;
     const int qtiles = (a.Lq + QT - 1) / QT, id = rp_block(a, qtiles);
     if (id >= a.B * a.heads * qtiles) return;
     const int bh = id / qtiles, b = bh / a.heads, h = bh - b * a.heads, q0 = (id - bh * qtiles) * QT;
@@ -635,46 +677,55 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) vo
     far = __any(far);
     const bool idle = q0 + wave * QB * 16 >= a.Lq;
     const unsigned long long seed = a.pdrop > 0.f ? rp_seed(a) : 0ull;
-    rp_zero_pad<T, DP, 0>(Ks, a.D, tid);
-    rp_zero_pad<T, DP, 0>(Vs, a.D, tid);
+    rp_zero_pad<T, DP, 0, Dim::STAGE>(Ks, a.D, tid);
+    rp_zero_pad<T, DP, 0, Dim::STAGE>(Vs, a.D, tid);
 
-    RpTile<T, DP> kt, vt;
+    RpTile<T, DP, ST> kt, vt;
     kt.init(a.sk.t, a.D, tid);
     vt.init(a.sv.t, a.D, tid);
     RpWindow wt;
-    unsigned long long valid = 0ull;
-    int byte = 0, ck_lo = 0, n_win = 0, base = 0;
+    unsigned long long valid[HV];
+    int byte[HV], ck_lo = 0, n_win = 0, base = 0;
     auto fetch = [&](int t) {
-        const int k0 = t * RP_TILE;
-        byte = rp_mask_byte(a, b, k0);
+        const int k0 = t * ST;
+#pragma unroll
+        for (int i = 0; i < HV; ++i) byte[i] = rp_mask_byte(a, b, k0 + 64 * i);
         kt.fetch(kp, a.sk.t, k0, a.Lk, a.D, tid);
         vt.fetch(vp, a.sv.t, k0, a.Lk, a.D, tid);
         ck_lo = rp_c(a, k0);
         base = ck_lo - cq_hi + a.off;
-        n_win = rp_c(a, min(k0 + RP_TILE, a.Lk) - 1) - ck_lo + cq_hi - cq_lo + 1;
+        n_win = rp_c(a, min(k0 + ST, a.Lk) - 1) - ck_lo + cq_hi - cq_lo + 1;
         wt.fetch(bias + base, n_win, tid);
     };
-    const int t1 = a.tiles;
-    fetch(0);
-    for (int t = 0; t < t1; ++t) {
+    const int t1 = (int)((long long)a.tiles * (blockIdx.y + 1) / a.splits);
+    int t = (int)((long long)a.tiles * blockIdx.y / a.splits);
+    if (t < t1) fetch(t);
+    for (; t < t1; ++t) {
         rp_barrier();
-        valid = rp_valid(a, t * RP_TILE, byte);
+#pragma unroll
+        for (int i = 0; i < HV; ++i) valid[i] = rp_valid(a, t * ST + 64 * i, byte[i]);
         kt.template put<0>(Ks, valid, a.D, tid);
         vt.template put<0>(Vs, valid, a.D, tid);
         wt.put(bw, bias + base, n_win, tid);
-        if (tid < RP_TILE) {
-            ck[tid] = 4 * (rp_c(a, min(t * RP_TILE + tid, a.Lk - 1)) - ck_lo);
-            cap[tid] = (valid >> tid) & 1 ? INFINITY : -INFINITY;
+        if (tid < ST) {
+            ck[tid] = 4 * (rp_c(a, min(t * ST + tid, a.Lk - 1)) - ck_lo);
+            cap[tid] = ((tid < 64 ? valid[0] : valid[HV - 1]) >> (tid & 63)) & 1 ? INFINITY : -INFINITY;
         }
         rp_barrier();
         if (t + 1 < t1) fetch(t + 1);
-        if (idle || valid == 0ull) continue;
+        if (idle) continue;
+#pragma unroll 1
+        for (int hv = 0; hv < HV; ++hv) {
+        const unsigned long long here = HV == 1 || hv == 0 ? valid[0] : valid[HV - 1];
+        if (here == 0ull) continue;
+        const T *Kh = Ks + hv * RP_TILE * LD, *Vh = Vs + hv * RP_TILE * LD;
+        const int* ckh = ck + hv * RP_TILE;
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
             rp_f32x4 s[2][QB], ds[2][QB];   // ds: dP, then dS
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int4 c4 = *reinterpret_cast<const int4*>(ck + (2 * kk + e) * 16 + g * 4);
+                const int4 c4 = *reinterpret_cast<const int4*>(ckh + (2 * kk + e) * 16 + g * 4);
 #pragma unroll
                 for (int i = 0; i < QB; ++i) {
                     s[e][i] = rp_bias4(bw, c4, cq[i]);
@@ -686,8 +737,8 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) vo
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const int at = ((2 * kk + e) * 16 + l) * LD + c * Op::CHUNK + g * Op::PER;
-                    const typename Op::Frag kf = *reinterpret_cast<const typename Op::Frag*>(Ks + at);
-                    const typename Op::Frag vf = *reinterpret_cast<const typename Op::Frag*>(Vs + at);
+                    const typename Op::Frag kf = *reinterpret_cast<const typename Op::Frag*>(Kh + at);
+                    const typename Op::Frag vf = *reinterpret_cast<const typename Op::Frag*>(Vh + at);
 #pragma unroll
                     for (int i = 0; i < QB; ++i) {
                         s[e][i] = Op::dot(kf, qf[i][c], s[e][i]);
@@ -698,15 +749,15 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) vo
             if constexpr (Dim::EARLY) {
 #pragma unroll
                 for (int d = 0; d < Dim::DB; ++d) {
-                    const T* k0 = Ks + (kk * 32 + g * 4) * LD + d * 16;
+                    const T* k0 = Kh + (kk * 32 + g * 4) * LD + d * 16;
                     kt_[d] = Op::load_t(k0, k0 + 16 * LD, LD, l);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
-            if (valid != ~0ull) {
+            if (here != ~0ull) {
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const rp_f32x4 c4 = *reinterpret_cast<const rp_f32x4*>(cap + (2 * kk + e) * 16 + g * 4);
+                    const rp_f32x4 c4 = *reinterpret_cast<const rp_f32x4*>(cap + hv * RP_TILE + (2 * kk + e) * 16 + g * 4);
 #pragma unroll
                     for (int i = 0; i < QB; ++i)
 #pragma unroll
@@ -716,7 +767,7 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) vo
             if (a.pdrop > 0.f) {
 #pragma unroll
                 for (int i = 0; i < QB; ++i) {
-                    const unsigned long long at = ((unsigned long long)bh * a.Lq + qi[i]) * a.Lk + t * RP_TILE + kk * 32 + g * 4;
+                    const unsigned long long at = ((unsigned long long)bh * a.Lq + qi[i]) * a.Lk + t * ST + hv * RP_TILE + kk * 32 + g * 4;
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -755,19 +806,31 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) vo
 #pragma unroll
             for (int d = 0; d < Dim::DB; ++d) {
                 if constexpr (!Dim::EARLY) {
-                    const T* k0 = Ks + (kk * 32 + g * 4) * LD + d * 16;
+                    const T* k0 = Kh + (kk * 32 + g * 4) * LD + d * 16;
                     kt_[d] = Op::load_t(k0, k0 + 16 * LD, LD, l);
                 }
 #pragma unroll
                 for (int i = 0; i < QB; ++i) dq[i][d] = Op::dot_t(kt_[d], p[i], dq[i][d]);
             }
         }
+        }
     }
 #pragma unroll
     for (int i = 0; i < QB; ++i) {
-        const float Di = D0[i] + rp_xor_sum(extra[i]);
+        const float more = rp_xor_sum(extra[i]);
         if (qi[i] >= a.Lq) continue;
-        if (g == 0) a.dsum[(size_t)bh * a.Lq + qi[i]] = Di;
+        const size_t row = (size_t)bh * a.Lq + qi[i];
+        if (a.splits > 1) {
+            const size_t prow = (size_t)blockIdx.y * a.B * a.heads * a.Lq + row;
+            if (g == 0) *reinterpret_cast<float2*>(a.pml + 2 * prow) = make_float2(D0[i], more);
+#pragma unroll
+            for (int d = 0; d < Dim::DB; ++d) {
+                const int col = d * 16 + g * 4;
+                if (col < a.D) *reinterpret_cast<rp_f32x4*>(a.po + prow * a.D + col) = dq[i][d];
+            }
+            continue;
+        }
+        if (g == 0) a.dsum[row] = D0[i] + more;
         T* out = (T*)a.dq + b * a.sdq.b + (long long)qi[i] * a.sdq.t + h * a.sdq.h;
 #pragma unroll
         for (int d = 0; d < Dim::DB; ++d) {
@@ -821,8 +884,10 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
     const int k_hi = min(k0 + KT, a.Lk) - 1;
     const int ck_lo = rp_c(a, k0) + a.off, ck_hi = rp_c(a, k_hi) + a.off;   // offset of a pair = this - c(query)
     const bool grad_bias = a.slab != nullptr;
-    float* slab = grad_bias ? a.slab + (size_t)id * a.slab_ld : nullptr;
-    const int slab_lo = ck_lo - rp_c(a, a.q_start + a.Lq - 1);
+    const int qtiles = (a.Lq + RP_TILE - 1) / RP_TILE;
+    const int t0 = (int)((long long)qtiles * blockIdx.y / a.splits), t1 = (int)((long long)qtiles * (blockIdx.y + 1) / a.splits);
+    float* slab = grad_bias ? a.slab + ((size_t)id * a.splits + blockIdx.y) * a.slab_ld : nullptr;
+    const int slab_lo = ck_lo - rp_c(a, a.q_start + min(t1 * RP_TILE, a.Lq) - 1);
     double* mine = acc + wave * ring;
 
     typename Op::Frag kf[KB][Dim::NCH], vf[KB][Dim::NCH];
@@ -852,8 +917,8 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
     any_bad = __any(any_bad);
     any_ok = __any(any_ok);
     const unsigned long long seed = a.pdrop > 0.f ? rp_seed(a) : 0ull;
-    rp_zero_pad<T, DP, INS>(Qs, a.D, threadIdx.x);
-    rp_zero_pad<T, DP, INS>(Gs, a.D, threadIdx.x);
+    rp_zero_pad<T, DP, INS, RP_TILE>(Qs, a.D, threadIdx.x);
+    rp_zero_pad<T, DP, INS, RP_TILE>(Gs, a.D, threadIdx.x);
     if (grad_bias)
         for (int i = threadIdx.x; i < 4 * ring; i += 256) acc[i] = 0.0;
 
@@ -867,13 +932,12 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
         }
     };
 
-    RpTile<T, DP> qt, gt;
+    RpTile<T, DP, RP_TILE> qt, gt;
     qt.init(a.sq.t, a.D, threadIdx.x);
     gt.init(gst, a.D, threadIdx.x);
     float2 sr = make_float2(0.f, 0.f);
     float dr = 0.f, br[2];
     int b_lo = 0, b_hi = 0;
-    const int qtiles = (a.Lq + RP_TILE - 1) / RP_TILE;
     auto fetch = [&](int t) {
         const int first = t * RP_TILE, left = a.Lq - first;
         qt.fetch(qp, a.sq.t, first, a.Lq, a.D, threadIdx.x);
@@ -885,13 +949,13 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
         }
         // the offsets that this tile is the first to reach: below those of the tile before it
         b_lo = ck_lo - rp_c(a, a.q_start + min(first + RP_TILE, a.Lq) - 1);
-        b_hi = t == 0 ? ck_hi - rp_c(a, a.q_start) : ck_lo - rp_c(a, a.q_start + first - 1) - 1;
+        b_hi = t == t0 ? ck_hi - rp_c(a, a.q_start + first) : ck_lo - rp_c(a, a.q_start + first - 1) - 1;
 #pragma unroll
         for (int i = 0; i < 2; ++i) br[i] = bias[min(b_lo + i * 256 + (int)threadIdx.x, b_hi)];
     };
-    fetch(0);
-    int top = ck_hi - rp_c(a, a.q_start);   // highest offset still in the ring
-    for (int t = 0; t < qtiles; ++t) {
+    fetch(t0);
+    int top = ck_hi - rp_c(a, a.q_start + t0 * RP_TILE);   // highest offset still in the ring
+    for (int t = t0; t < t1; ++t) {
         const int first = t * RP_TILE, q_hi = min(first + RP_TILE, a.Lq) - 1;
         const int cq_lo = rp_c(a, a.q_start + first);
         rp_barrier();
@@ -901,7 +965,7 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
             top = reach;
         }
         const int left = a.Lq - first;
-        const unsigned long long rows = left >= 64 ? ~0ull : (1ull << left) - 1;
+        const unsigned long long rows[1] = {left >= 64 ? ~0ull : (1ull << left) - 1};
         qt.template put<INS>(Qs, rows, a.D, threadIdx.x);
         gt.template put<INS>(Gs, rows, a.D, threadIdx.x);
 #pragma unroll
@@ -917,7 +981,7 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
         }
         rp_barrier();
         const bool far = __any(fabsf(ms[lane]) * a.sl2 > RP_FAR);
-        if (t + 1 < qtiles) fetch(t + 1);
+        if (t + 1 < t1) fetch(t + 1);
         if (!any_ok) continue;
 #pragma unroll
         for (int kk = 0; kk < 2; ++kk) {
@@ -1036,6 +1100,18 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
 #pragma unroll
     for (int j = 0; j < KB; ++j) {
         if (key[j] >= a.Lk) continue;
+        if (a.splits > 1) {
+            const size_t part = (size_t)a.B * a.heads * a.Lk * a.D;
+            float* p = a.po + 2 * blockIdx.y * part + ((size_t)bh * a.Lk + key[j]) * a.D;
+#pragma unroll
+            for (int d = 0; d < Dim::DB; ++d) {
+                const int col = d * 16 + g * 4;
+                if (col >= a.D) continue;
+                *reinterpret_cast<rp_f32x4*>(p + col) = ok[j] ? dk[j][d] : rp_f32x4{0.f, 0.f, 0.f, 0.f};
+                *reinterpret_cast<rp_f32x4*>(p + part + col) = ok[j] ? dv[j][d] : rp_f32x4{0.f, 0.f, 0.f, 0.f};
+            }
+            continue;
+        }
         T* kd = (T*)a.dk + b * a.sdk.b + (long long)key[j] * a.sdk.t + h * a.sdk.h;
         T* vd = (T*)a.dv + b * a.sdv.b + (long long)key[j] * a.sdv.t + h * a.sdv.h;
 #pragma unroll
@@ -1057,21 +1133,48 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
 // bias gradient: offsets over images and key blocks, then buckets over their offsets (the offsets of bucket k are
 // order[start[k]] .. order[start[k + 1] - 1]). Fixed order everywhere.
 // ------------------------------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void relpos_offsets_kernel(const float* __restrict__ slab, RpArgs a, int ktiles, int kt,
-                                                             float* __restrict__ per_off) {
-    __shared__ float sm[4][64];
-    const int col = threadIdx.x & 63, part = threadIdx.x >> 6, o = blockIdx.x * 64 + col, h = blockIdx.y;
-    const int c_last = rp_c(a, a.q_start + a.Lq - 1), c_first = rp_c(a, a.q_start);
+// Slab rows are [image][head][key block][query range]; the offsets that a row covers depend on the last two alone. A workgroup: 64
+// offsets, 16 waves that share the rows; a row that covers none of the 64 costs two comparisons.
+__global__ __launch_bounds__(1024) void relpos_offsets_kernel(RpArgs a, int ktiles, int kt, float* __restrict__ per_off) {
+    __shared__ float sm[16][64];
+    __shared__ int2 cover[1024];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, o0 = blockIdx.x * 64, o = o0 + lane, h = blockIdx.y;
+    const int rows = ktiles * a.splits, qtiles = (a.Lq + RP_TILE - 1) / RP_TILE;
+    const int wb = rows >= 16 ? 1 : 16, b0 = wb == 1 ? 0 : wave, r0 = wb == 1 ? wave : 0, rs = wb == 1 ? 16 : 1;   // waves over rows or images
+    const size_t image = (size_t)a.heads * rows * a.slab_ld;
     float v = 0.f;
-    if (o < a.n_off)
-        for (int i = part; i < a.B * ktiles; i += 4) {
-            const int b = i / ktiles, kb = i - b * ktiles, k0 = kb * kt;
-            const int lo = rp_c(a, k0) + a.off - c_last, hi = rp_c(a, min(k0 + kt, a.Lk) - 1) + a.off - c_first;
-            if (o >= lo && o <= hi) v += slab[((size_t)(b * a.heads + h) * ktiles + kb) * a.slab_ld + (o - lo)];
+    for (int first = 0; first < rows; first += 1024) {
+        const int n = min(1024, rows - first);
+        __syncthreads();
+        if ((int)threadIdx.x < n) {
+            const int r = first + threadIdx.x, kb = r / a.splits, sp = r - kb * a.splits, k0 = kb * kt;
+            const int q0 = (int)((long long)qtiles * sp / a.splits) * RP_TILE, q1 = min((int)((long long)qtiles * (sp + 1) / a.splits) * RP_TILE, a.Lq) - 1;
+            cover[threadIdx.x] = make_int2(rp_c(a, k0) + a.off - rp_c(a, a.q_start + q1), rp_c(a, min(k0 + kt, a.Lk) - 1) + a.off - rp_c(a, a.q_start + q0));
         }
-    sm[part][col] = v;
+        __syncthreads();
+        for (int i = r0; i < n; i += rs) {
+            const int lo = __builtin_amdgcn_readfirstlane(cover[i].x), hi = __builtin_amdgcn_readfirstlane(cover[i].y);
+            if (hi < o0 || lo > o0 + 63) continue;
+            const bool in = o >= lo && o <= hi;
+            const float* p = a.slab + ((size_t)h * rows + first + i) * a.slab_ld + (in ? o - lo : 0);
+            int b = b0;
+            for (; b + 3 * wb < a.B; b += 4 * wb) {
+                float x[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[u] = p[(b + u * wb) * image];
+                if (in) v += (x[0] + x[1]) + (x[2] + x[3]);
+            }
+            for (; b < a.B; b += wb) {
+                const float x = p[b * image];
+                if (in) v += x;
+            }
+        }
+    }
+    sm[wave][lane] = v;
     __syncthreads();
-    if (part == 0 && o < a.n_off) per_off[(size_t)h * a.n_off + o] = (sm[0][col] + sm[1][col]) + (sm[2][col] + sm[3][col]);
+    if (wave != 0 || o >= a.n_off) return;
+    for (int w = 1; w < 16; ++w) v += sm[w][lane];
+    per_off[(size_t)h * a.n_off + o] = v;
 }
 
 __global__ __launch_bounds__(256) void relpos_buckets_kernel(const float* __restrict__ per_off, int n_off, int heads,
@@ -1104,27 +1207,41 @@ static int rp_ld(int dtype, int DP) {   // RpDim::LD
     const int chunk = dtype == MIA_BF16 ? 32 : 16;
     return (DP + chunk - 1) / chunk * chunk + chunk / 4;
 }
+static int rp_stage(int dtype, int DP) { return dtype == MIA_BF16 && DP <= 64 ? 2 * RP_TILE : RP_TILE; }   // RpDim::STAGE
 static size_t rp_es(int dtype) { return dtype == MIA_BF16 ? 2 : 4; }
 
-// Queries / keys of a workgroup: 128 (two 16-wide columns a wave: each operand read from LDS serves both) when that still gives
-// two workgroups a CU, else 64. fp32 keeps 64: its operands are twice as large.
-static int rp_cols(int dtype, int DP, long long bh, int L, int max_dp) {
-    if (dtype == MIA_F32 || DP > max_dp) return 1;
-    return bh * ((L + 127) / 128) >= 512 ? 2 : 1;
-}
-static int rp_kv_cols(int dtype, int D, long long bh, int Lk) { return rp_cols(dtype, rp_dp(D), bh, Lk, 64); }
-
-// key ranges of a forward with few workgroups: enough of them for two workgroups a CU, at least four tiles each
-static int rp_splits(long long wgs, int tiles) {
-    if (wgs >= 256 || tiles < 8) return 1;
-    long long s = (512 + wgs - 1) / wgs;
-    if (s > tiles / 4) s = tiles / 4;
-    return s < 1 ? 1 : (int)(s > 64 ? 64 : s);
-}
-static int rp_fwd_splits(int dtype, int B, int heads, int Lq, int Lk, int D, int& cols) {
+// How the kernels are laid out over a problem.
+// cols: 16-wide columns of a wave, so 64 * cols queries (keys) of a workgroup. Two serve more products with every operand read from
+// LDS; they are taken unless only the narrower workgroups fill the chip. fp32 keeps one: its operands are twice as large.
+// splits: ranges of the tokens a workgroup walks, joined afterwards. The grid runs in turns of as many workgroups as are resident
+// (two a CU with two columns, three with one), so s splits take ceil(workgroups * s / resident) / s of an unsplit walk, plus
+// what starting and joining them costs; ranges of at least four rounds.
+struct RpPlan {
+    int cols, splits;
+};
+static RpPlan rp_plan(int what, int dtype, int B, int heads, int Lq, int Lk, int D) {
+    const int DP = rp_dp(D), owned = what == RP_BWD_KV ? Lk : Lq, walked = what == RP_BWD_KV ? Lq : Lk;
+    const int round = what == RP_BWD_KV ? RP_TILE : rp_stage(dtype, DP);
     const long long bh = (long long)B * heads;
-    cols = rp_cols(dtype, rp_dp(D), bh, Lq, 96);
-    return rp_splits(bh * ((Lq + 64 * cols - 1) / (64 * cols)), (Lk + RP_TILE - 1) / RP_TILE);
+    RpPlan p;
+    const long long one = bh * ((owned + 63) / 64), two = bh * ((owned + 127) / 128), rounds = (walked + round - 1) / round;
+    p.cols = dtype == MIA_F32 || DP > (what == RP_FWD ? 96 : 64) || owned <= 64 || (two < 512 && one >= 512) ? 1 : 2;
+#ifdef RP_TUNE
+    if (const char* e = getenv(what == RP_FWD ? "RP_CF" : what == RP_BWD_Q ? "RP_CQ" : "RP_CK")) p.cols = atoi(e);
+#endif
+    const long long wgs = p.cols == 1 ? one : two;
+    const long long resident = 256 * (p.cols == 1 ? 3 : 2), most = rounds / 4 < 64 ? rounds / 4 : 64;
+    long long s = 1;
+    double best = 1e30;
+    for (long long i = 1; i <= most && (i == 1 || wgs < 2 * resident); ++i) {
+        const double t = (double)((wgs * i + resident - 1) / resident) / i + 0.02 * i;
+        if (t < best - 0.1 * (s == 1)) best = t, s = i;
+    }
+#ifdef RP_TUNE
+    if (const char* e = getenv(what == RP_FWD ? "RP_SF" : what == RP_BWD_Q ? "RP_SQ" : "RP_SK")) s = atoi(e);
+#endif
+    p.splits = (int)(s > most ? (most < 1 ? 1 : most) : s);
+    return p;
 }
 
 template <typename K>
@@ -1172,8 +1289,8 @@ static int rp_dispatch(int what, const char* name, int dtype, int cols, dim3 gri
 
 // LDS of a query kernel: two tiles, the keys' c and caps, the bias window
 static size_t rp_query_lds(const RpArgs& a, int dtype, int DP, int cols, int tokens) {
-    const int win = rp_span(a, RP_TILE, tokens) + rp_span(a, 64 * cols, tokens) + 1;
-    return 2 * (size_t)RP_TILE * rp_ld(dtype, DP) * rp_es(dtype) + RP_TILE * 8 + (size_t)win * 4;
+    const int stage = rp_stage(dtype, DP), win = rp_span(a, stage, tokens) + rp_span(a, 64 * cols, tokens) + 1;
+    return 2 * (size_t)stage * rp_ld(dtype, DP) * rp_es(dtype) + stage * 8 + (size_t)win * 4;
 }
 
 static dim3 rp_grid(long long blocks, int splits) { return dim3((unsigned)((blocks + 7) / 8 * 8), (unsigned)splits); }
@@ -1213,7 +1330,6 @@ static void rp_fill(RpArgs& a, int B, int heads, int Lq, int Lk, int D, int heig
     a.n_off = (2 * height - 1) * (2 * width - 1);
     a.q_start = q_start; a.scale = scale; a.sl2 = scale * RP_LOG2E;
     a.pdrop = pdrop; a.seed = seed; a.seed_off = seed_offset;
-    a.tiles = (Lk + RP_TILE - 1) / RP_TILE;
     a.splits = 1;
 }
 
@@ -1233,10 +1349,24 @@ extern "C" int mia_relpos_bias(const float* table, const int* bucket, int height
     return 0;
 }
 
+// floats of the partial results of a split launch (rows of D and two more per query; dK and dV rows of D)
+static long long rp_part_floats(int what, const RpPlan& p, int B, int heads, int Lq, int Lk, int D) {
+    if (p.splits == 1) return 0;
+    return (long long)p.splits * B * heads * (what == RP_BWD_KV ? 2ll * Lk * D : (long long)Lq * (D + 2));
+}
+
+template <int WHAT>
+static int rp_join(const char* name, int dtype, const RpArgs& a, hipStream_t s) {
+    const long long threads = (long long)a.B * a.heads * (WHAT == RP_BWD_KV ? a.Lk : a.Lq) * (a.D / 4);
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    if (dtype == MIA_BF16) MIA_LAUNCH((relpos_join_kernel<bf16_t, WHAT>), grid, dim3(256), 0, s, a);
+    else MIA_LAUNCH((relpos_join_kernel<float, WHAT>), grid, dim3(256), 0, s, a);
+    MIA_CHECK_LAUNCH(name);
+    return 0;
+}
+
 extern "C" long long mia_relpos_fwd_ws_floats(int dtype, int B, int heads, int Lq, int Lk, int D) {
-    int cols = 1;
-    const int splits = rp_fwd_splits(dtype, B, heads, Lq, Lk, D, cols);
-    return splits > 1 ? (long long)splits * B * heads * Lq * (D + 2) : 0;
+    return rp_part_floats(RP_FWD, rp_plan(RP_FWD, dtype, B, heads, Lq, Lk, D), B, heads, Lq, Lk, D);
 }
 
 extern "C" int mia_relpos_fwd(int dtype, const void* q, const void* k, const void* v, const long long* strides, int B, int heads,
@@ -1254,8 +1384,11 @@ extern "C" int mia_relpos_fwd(int dtype, const void* q, const void* k, const voi
         rp_aligned("mia_relpos_fwd", dtype, v, a.sv) || rp_aligned("mia_relpos_fwd", dtype, out, RpStride{0, 0, 0}))
         return -1;
     rp_fill(a, B, heads, Lq, Lk, D, height, width, q_start, scale, pdrop, seed, seed_offset);
-    int cols = 1;
-    a.splits = rp_fwd_splits(dtype, B, heads, Lq, Lk, D, cols);
+    const int stage = rp_stage(dtype, rp_dp(D));
+    a.tiles = (Lk + stage - 1) / stage;
+    const RpPlan plan = rp_plan(RP_FWD, dtype, B, heads, Lq, Lk, D);
+    const int cols = plan.cols;
+    a.splits = plan.splits;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const long long rows = (long long)B * heads * Lq;
     if (a.splits > 1) {
@@ -1270,11 +1403,7 @@ extern "C" int mia_relpos_fwd(int dtype, const void* q, const void* k, const voi
     const size_t lds = rp_query_lds(a, dtype, DP, cols, tokens);
     const int rc = rp_dispatch(RP_FWD, "mia_relpos_fwd", dtype, cols, rp_grid((long long)B * heads * ((Lq + 64 * cols - 1) / (64 * cols)), a.splits), lds, a, s);
     if (rc || a.splits == 1) return rc;
-    const dim3 threads((D + 63) / 64 * 64);
-    if (dtype == MIA_BF16) MIA_LAUNCH(relpos_join_kernel<bf16_t>, dim3((unsigned)rows), threads, 0, s, a);
-    else MIA_LAUNCH(relpos_join_kernel<float>, dim3((unsigned)rows), threads, 0, s, a);
-    MIA_CHECK_LAUNCH("mia_relpos_fwd");
-    return 0;
+    return rp_join<RP_FWD>("mia_relpos_fwd", dtype, a, s);
 }
 
 // floats of one slab row, and key blocks of one (image, head)
@@ -1282,14 +1411,29 @@ static int rp_slab_ld(const RpArgs& a, int tokens, int cols) {
     return rp_span(a, a.Lq, tokens) + rp_span(a, 64 * cols, tokens) + 1;
 }
 
-extern "C" long long mia_relpos_bwd_ws_floats(int dtype, int B, int heads, int Lq, int Lk, int D, int height, int width, int want_bias) {
-    const long long rows = ((long long)B * heads * Lq + 3) / 4 * 4;
-    if (!want_bias) return rows;
+// The backward's workspace: D of every row | the bias gradient per offset | slab rows | partial results (those of dQ are
+// joined before the dK / dV kernel writes its own over them)
+struct RpWs {
+    long long per_off, slab, part, total;
+};
+static RpWs rp_bwd_ws(int dtype, int B, int heads, int Lq, int Lk, int D, int height, int width, int want_bias) {
     RpArgs a = {};
     rp_fill(a, B, heads, Lq, Lk, D, height, width, 0, 1.f, 0.f, 0, nullptr);
-    const int cols = rp_kv_cols(dtype, D, (long long)B * heads, Lk);
-    return rows + (long long)heads * a.n_off +
-           (long long)B * heads * ((Lk + 64 * cols - 1) / (64 * cols)) * rp_slab_ld(a, height * width, cols);
+    const RpPlan q = rp_plan(RP_BWD_Q, dtype, B, heads, Lq, Lk, D), kv = rp_plan(RP_BWD_KV, dtype, B, heads, Lq, Lk, D);
+    const long long bh = (long long)B * heads, kt = 64 * kv.cols;
+    RpWs w;
+    w.per_off = (bh * Lq + 3) / 4 * 4;
+    w.slab = w.per_off + (want_bias ? (long long)heads * a.n_off : 0);
+    w.part = w.slab + (want_bias ? bh * ((Lk + kt - 1) / kt) * kv.splits * rp_slab_ld(a, height * width, kv.cols) : 0);
+    w.part = (w.part + 3) / 4 * 4;
+    const long long pq = rp_part_floats(RP_BWD_Q, q, B, heads, Lq, Lk, D), pk = rp_part_floats(RP_BWD_KV, kv, B, heads, Lq, Lk, D);
+    w.total = w.part + (pq > pk ? pq : pk);
+    return w;
+}
+
+extern "C" long long mia_relpos_bwd_ws_floats(int dtype, int B, int heads, int Lq, int Lk, int D, int height, int width, int want_bias) {
+    const RpWs w = rp_bwd_ws(dtype, B, heads, Lq, Lk, D, height, width, want_bias);
+    return w.total;
 }
 
 extern "C" int mia_relpos_bwd(int dtype, const void* q, const void* k, const void* v, const long long* strides, const void* dout,
@@ -1303,8 +1447,9 @@ extern "C" int mia_relpos_bwd(int dtype, const void* q, const void* k, const voi
     MIA_CHECK_ARG(((uintptr_t)stat & 7) == 0, "mia_relpos_bwd: stat must start at a multiple of 8 bytes");
     MIA_CHECK_ARG(!dtable || (order && start && buckets > 0), "mia_relpos_bwd: the bias gradient needs the bucket lists");
     MIA_CHECK_ARG(heads <= 65535, "mia_relpos_bwd: %d heads are too many", heads);
-    const long long need = mia_relpos_bwd_ws_floats(dtype, B, heads, Lq, Lk, D, height, width, dtable != nullptr);
-    MIA_CHECK_ARG(ws_floats >= need, "mia_relpos_bwd: workspace of %lld floats is too small (%lld needed)", ws_floats, need);
+    const RpWs w = rp_bwd_ws(dtype, B, heads, Lq, Lk, D, height, width, dtable != nullptr);
+    MIA_CHECK_ARG(ws_floats >= w.total, "mia_relpos_bwd: workspace of %lld floats is too small (%lld needed)", ws_floats, w.total);
+    MIA_CHECK_ARG(((uintptr_t)ws & 15) == 0, "mia_relpos_bwd: the workspace must start at a multiple of 16 bytes");
     RpArgs a = {};
     a.q = q; a.k = k; a.v = v; a.dout = dout; a.out = out; a.bias = bias; a.mask = key_mask;
     a.stat = reinterpret_cast<float2*>(const_cast<float*>(stat));
@@ -1320,23 +1465,33 @@ extern "C" int mia_relpos_bwd(int dtype, const void* q, const void* k, const voi
     const long long bh = (long long)B * heads;
     const int tokens = height * width, DP = rp_dp(D);
     const size_t tile = (size_t)RP_TILE * rp_ld(dtype, DP) * rp_es(dtype);
-    const int qc = rp_cols(dtype, DP, bh, Lq, 64);
-    const size_t q_lds = rp_query_lds(a, dtype, DP, qc, tokens);
-    if (int rc = rp_dispatch(RP_BWD_Q, "mia_relpos_bwd", dtype, qc, rp_grid(bh * ((Lq + 64 * qc - 1) / (64 * qc)), 1), q_lds, a, s)) return rc;
-    const int kc = rp_kv_cols(dtype, D, bh, Lk), ktiles = (Lk + 64 * kc - 1) / (64 * kc);
+    const RpPlan qp = rp_plan(RP_BWD_Q, dtype, B, heads, Lq, Lk, D), kp = rp_plan(RP_BWD_KV, dtype, B, heads, Lq, Lk, D);
+    const int stage = rp_stage(dtype, DP), kt = 64 * kp.cols, ktiles = (Lk + kt - 1) / kt;
+    a.tiles = (Lk + stage - 1) / stage;
+    a.splits = qp.splits;
+    a.po = ws + w.part;
+    a.pml = a.po + (long long)qp.splits * bh * Lq * D;
+    if (int rc = rp_dispatch(RP_BWD_Q, "mia_relpos_bwd", dtype, qp.cols, rp_grid(bh * ((Lq + 64 * qp.cols - 1) / (64 * qp.cols)), qp.splits),
+                             rp_query_lds(a, dtype, DP, qp.cols, tokens), a, s))
+        return rc;
+    if (qp.splits > 1)
+        if (int rc = rp_join<RP_BWD_Q>("mia_relpos_bwd", dtype, a, s)) return rc;
     int ring = 64;
-    while (ring < rp_span(a, RP_TILE, tokens) + rp_span(a, 64 * kc, tokens) + 1) ring *= 2;
+    while (ring < rp_span(a, RP_TILE, tokens) + rp_span(a, kt, tokens) + 1) ring *= 2;
     MIA_CHECK_ARG(ring <= RP_RING_MAX, "mia_relpos_bwd: ring of %d offsets", ring);
     a.acc_mask = ring - 1;
-    float* per_off = ws + (bh * Lq + 3) / 4 * 4;
+    a.splits = kp.splits;
+    float* per_off = ws + w.per_off;
     if (dtable) {
-        a.slab_ld = rp_slab_ld(a, tokens, kc);
-        a.slab = per_off + (long long)heads * a.n_off;
+        a.slab_ld = rp_slab_ld(a, tokens, kp.cols);
+        a.slab = ws + w.slab;
     }
     const size_t kv_lds = 2 * (tile + 256) + 5 * RP_TILE * 4 + (size_t)ring * (dtable ? 4 + 4 * 8 : 4);
-    if (int rc = rp_dispatch(RP_BWD_KV, "mia_relpos_bwd", dtype, kc, rp_grid(bh * ktiles, 1), kv_lds, a, s)) return rc;
+    if (int rc = rp_dispatch(RP_BWD_KV, "mia_relpos_bwd", dtype, kp.cols, rp_grid(bh * ktiles, kp.splits), kv_lds, a, s)) return rc;
+    if (kp.splits > 1)
+        if (int rc = rp_join<RP_BWD_KV>("mia_relpos_bwd", dtype, a, s)) return rc;
     if (!dtable) return 0;
-    MIA_LAUNCH(relpos_offsets_kernel, dim3(cdiv(a.n_off, 64), heads), dim3(256), 0, s, a.slab, a, ktiles, 64 * kc, per_off);
+    MIA_LAUNCH(relpos_offsets_kernel, dim3(cdiv(a.n_off, 64), heads), dim3(1024), 0, s, a, ktiles, kt, per_off);
     MIA_CHECK_LAUNCH("mia_relpos_bwd");
     MIA_LAUNCH(relpos_buckets_kernel, dim3(buckets, heads), dim3(256), 0, s, per_off, a.n_off, heads, order, start, dtable);
     MIA_CHECK_LAUNCH("mia_relpos_bwd");
