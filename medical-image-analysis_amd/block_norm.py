@@ -12,14 +12,13 @@ class GatedResidualNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, f, scale, gate, w1, b1, w2, b2, post, pre, eps):
         x, f = x.contiguous(), f.contiguous()
-        scale, gate, w1, b1, w2, b2 = (t.contiguous() if t is not None else None for t in (scale, gate, w1, b1, w2, b2))
-        C = x.shape[-1]
-        images = gate.shape[0] if gate is not None else 1
-        rows = x.numel() // (images * C) if x.numel() else 0
+        scale, gate, w1, b1, w2, b2 = [t if t is None else t.contiguous() for t in (scale, gate, w1, b1, w2, b2)]
+        C, n = x.shape[-1], x.numel()
+        images = 1 if gate is None else gate.shape[0]
+        rows = n // (images * C) if n else 0
         y = torch.empty_like(x)
         z = torch.empty_like(x) if pre else None
-        keep = any(ctx.needs_input_grad)
-        stats = torch.empty((images * rows, 4), dtype=torch.float32, device=x.device) if keep else None
+        stats = torch.empty((images * rows, 4), dtype=torch.float32, device=x.device) if any(ctx.needs_input_grad) else None
         if rows:
             with on_device(x.device):
                 lib().mia_blocknorm_fwd(_DT[x.dtype], _p(x), _p(f), images, rows, C, _p(scale), _p(gate), post, _p(w1), _p(b1),
@@ -33,18 +32,22 @@ class GatedResidualNormFn(torch.autograd.Function):
     def backward(ctx, dy, dz):
         x, f, scale, gate, w1, b1, w2, b2, stats = ctx.saved_tensors
         images, rows, C, post, pre = ctx.meta
-        grads = [torch.empty_like(t) if t is not None else None for t in (scale, gate, w1, b1, w2, b2)]
+        ds, dg, dw1, db1, dw2, db2 = [t if t is None else torch.empty_like(t) for t in (scale, gate, w1, b1, w2, b2)]
         dx, df = torch.empty_like(x), torch.empty_like(f)
         if rows == 0 or (dy is None and dz is None):
-            return (dx.zero_(), df.zero_(), *[g.zero_() if g is not None else None for g in grads], None, None, None)
-        dy, dz = (t.contiguous() if t is not None else None for t in (dy, dz))
-        nws = lib().mia_blocknorm_ws_floats(images, rows, C, 1 if gate is not None else 0)
+            return (*[t if t is None else t.zero_() for t in (dx, df, ds, dg, dw1, db1, dw2, db2)], None, None, None)
+        if dy is not None:
+            dy = dy.contiguous()
+        if dz is not None:
+            dz = dz.contiguous()
+        lb = lib()
+        nws = lb.mia_blocknorm_ws_floats(images, rows, C, 1 if gate is not None else 0)
         ws = torch.empty((nws,), dtype=torch.float32, device=x.device)
         with on_device(x.device):
-            lib().mia_blocknorm_bwd(_DT[x.dtype], _p(dy), _p(dz), _p(x), _p(f), _p(stats), images, rows, C, _p(scale), _p(gate),
-                                    post, _p(w1), _p(b1), pre, _p(w2), _p(ws), nws, _p(dx), _p(df), *[_p(g) for g in grads],
-                                    _stream())
-        return (dx, df, *grads, None, None, None)
+            lb.mia_blocknorm_bwd(_DT[x.dtype], _p(dy), _p(dz), _p(x), _p(f), _p(stats), images, rows, C, _p(scale), _p(gate), post,
+                                 _p(w1), _p(b1), pre, _p(w2), _p(ws), nws, _p(dx), _p(df), _p(ds), _p(dg), _p(dw1), _p(db1),
+                                 _p(dw2), _p(db2), _stream())
+        return dx, df, ds, dg, dw1, db1, dw2, db2, None, None, None
 
 
 def gated_residual_norm(x, f, scale=None, gate=None, post=None, post_weight=None, post_bias=None, pre="rms", pre_weight=None,
@@ -60,32 +63,33 @@ def gated_residual_norm(x, f, scale=None, gate=None, post=None, post_weight=None
     "layer", each with a weight [C] and optionally a bias [C] (population variance over C, eps added to it). Parameters and
     gate are fp32. All arithmetic is fp32: z is formed from y before y is rounded to the tensors' type. Returns (y, z);
     differentiable in every tensor. C <= 8192."""
-    named = (("scale", scale), ("gate", gate), ("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight),
-             ("pre_bias", pre_bias))
     if post not in _KINDS or pre not in _KINDS:
         raise ValueError(f"norms are 'rms', 'layer' or None (got post={post!r}, pre={pre!r})")
-    if x.dtype not in _DT or f.dtype != x.dtype:
-        raise TypeError(f"x and f are both fp32 or both bf16 (got {x.dtype}, {f.dtype})")
-    if x.dim() < 1 or x.shape != f.shape:
-        raise ValueError(f"x and f have one shape [..., C] (got {tuple(x.shape)}, {tuple(f.shape)})")
-    C = x.shape[-1]
+    dtype, shape = x.dtype, x.shape
+    if dtype not in _DT or f.dtype != dtype:
+        raise TypeError(f"x and f are both fp32 or both bf16 (got {dtype}, {f.dtype})")
+    if len(shape) < 1 or f.shape != shape:
+        raise ValueError(f"x and f have one shape [..., C] (got {tuple(shape)}, {tuple(f.shape)})")
+    C = shape[-1]
     if not 1 <= C <= 8192:
         raise ValueError(f"C must be 1..8192 (got {C})")
     for kind, w, b, which in ((post, post_weight, post_bias, "post"), (pre, pre_weight, pre_bias, "pre")):
         if (kind is None) != (w is None) or (kind is None and b is not None):
             raise ValueError(f"{which}={kind!r} needs {'no weight and no bias' if kind is None else which + '_weight'}")
-    for name, t in named:
+    if gate is not None and len(shape) < 2:
+        raise ValueError("a gate needs x of at least two dimensions")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative (got {eps})")
+    device = x.get_device()
+    for name, t, want in (("scale", scale, (C,)), ("gate", gate, (shape[0], C)), ("post_weight", post_weight, (C,)), ("post_bias", post_bias, (C,)),
+                          ("pre_weight", pre_weight, (C,)), ("pre_bias", pre_bias, (C,))):
         if t is None:
             continue
-        want = (x.shape[0], C) if name == "gate" else (C,)
-        if name == "gate" and x.dim() < 2:
-            raise ValueError("a gate needs x of at least two dimensions")
-        if tuple(t.shape) != want or t.dtype != torch.float32:
+        if t.shape != want or t.dtype != torch.float32:
             raise ValueError(f"{name} must be fp32 {want} (got {t.dtype} {tuple(t.shape)})")
-    if not float(eps) >= 0:
-        raise ValueError(f"eps must not be negative (got {eps})")
-    for name, t in (("x", x), ("f", f), *named):
-        if t is not None and (not t.is_cuda or t.device != x.device):
-            raise RuntimeError(f"gated_residual_norm needs its tensors on one MI355X device; there is no CPU path ({name} is on {t.device})")
+        if t.get_device() != device:
+            raise RuntimeError(f"gated_residual_norm needs its tensors on one MI355X device; there is no CPU path ({name} on {t.device}, x on {x.device})")
+    if device < 0 or f.get_device() != device:
+        raise RuntimeError(f"gated_residual_norm needs its tensors on one MI355X device; there is no CPU path (x on {x.device}, f on {f.device})")
     return GatedResidualNormFn.apply(x, f, scale, gate, post_weight, post_bias, pre_weight, pre_bias, _KINDS[post], _KINDS[pre],
                                      float(eps))

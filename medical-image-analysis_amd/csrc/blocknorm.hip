@@ -487,11 +487,16 @@ extern "C" int mia_blocknorm_bwd(int dtype, const void* dy, const void* dz, cons
     if (dtype == MIA_BF16) bn_dispatch<bf16_t>(false, vec, a, s);
     else bn_dispatch<float>(false, vec, a, s);
     MIA_CHECK_LAUNCH("mia_blocknorm_bwd");
-    const int rows = a.N * a.S, groups = bn_groups(gate != nullptr, a.N, a.S);
-    float* sums = ws + (size_t)rows * 4 * C;
-    MIA_LAUNCH(blocknorm_fold_kernel, dim3(cdiv(C, 64), groups), dim3(1024), 0, s, ws, rows, gate ? a.S : 16, C, scale, post_w,
-               post_b, sums, gate ? dgate : nullptr);
-    MIA_CHECK_LAUNCH("mia_blocknorm_bwd");
+    // up to 64 slab rows without a gate are added up by the parameter kernel itself (four to a lane): one launch less
+    const int rows = a.N * a.S;
+    const bool fold = gate || rows > 64;
+    const int groups = fold ? bn_groups(gate != nullptr, a.N, a.S) : rows;
+    float* sums = fold ? ws + (size_t)rows * 4 * C : ws;
+    if (fold) {
+        MIA_LAUNCH(blocknorm_fold_kernel, dim3(cdiv(C, 64), groups), dim3(1024), 0, s, ws, rows, gate ? a.S : 16, C, scale, post_w,
+                   post_b, sums, gate ? dgate : nullptr);
+        MIA_CHECK_LAUNCH("mia_blocknorm_bwd");
+    }
     MIA_LAUNCH(blocknorm_params_kernel, dim3(cdiv(C, 64)), dim3(1024), 0, s, sums, groups, C, gate, scale, post_w, post_b, dscale,
                dpost_w, dpost_b, dpre_w, dpre_b);
     MIA_CHECK_LAUNCH("mia_blocknorm_bwd");

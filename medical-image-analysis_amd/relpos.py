@@ -89,35 +89,51 @@ def _rows(t):
     return t, st
 
 
+def _packed_rows(qkv):
+    """Addresses of q, k and v inside a packed [B, L, 3, heads, D] tensor and their common (batch, token, head) strides."""
+    sb, st, s3, sh, _ = qkv.stride()
+    at, step = qkv.data_ptr(), s3 * qkv.element_size()
+    return (at, at + step, at + 2 * step), (sb, st, sh) * 3
+
+
 class RelPosAttentionFn(torch.autograd.Function):
+    """q, k, v or one packed tensor in the place of q (k and v None)."""
+
     @staticmethod
     def forward(ctx, q, k, v, table, plan, mask, scale, q_start, pdrop, seed):
-        ctx.packed = k is None
-        if ctx.packed:
-            q, k, v = q.unbind(2)
-        B, Lq, heads, D = q.shape
-        Lk = k.shape[1]
-        dev, f32 = q.device, dict(dtype=torch.float32, device=q.device)
+        dev, dtype = q.device, q.dtype
+        f32 = dict(dtype=torch.float32, device=dev)
+        if k is None:
+            B, Lq, _, heads, D = q.shape
+            Lk = Lq
+            if not q.is_contiguous() or q.data_ptr() % 16:
+                q = q.clone(memory_format=torch.contiguous_format)
+            ptrs, strides = _packed_rows(q)
+        else:
+            B, Lq, heads, D = q.shape
+            Lk = k.shape[1]
+            (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
+            ptrs, strides = (_p(q), _p(k), _p(v)), sq + sk + sv
         ctx.meta = (B, heads, Lq, Lk, D, plan, scale, q_start, pdrop, seed, ops.seed_offset())
         ctx.empty = 0 in (B, Lq, Lk, heads)
         if ctx.empty:
-            out = torch.zeros((B, Lq, heads, D), dtype=q.dtype, device=dev)
             ctx.save_for_backward(q, k, v, table)
-            return out
-        out = torch.empty((B, Lq, heads, D), dtype=q.dtype, device=dev)
-        (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
-        table, mask = table.contiguous(), mask.contiguous() if mask is not None else None
-        strides = array("q", sq + sk + sv)
+            return torch.zeros((B, Lq, heads, D), dtype=dtype, device=dev)
+        out = torch.empty((B, Lq, heads, D), dtype=dtype, device=dev)
+        table = table.contiguous()
+        if mask is not None:
+            mask = mask.contiguous()
+        strides = array("q", strides)
         bias = torch.empty((heads, plan.index.numel()), **f32)
         stat = torch.empty((B, heads, Lq, 2), **f32) if any(ctx.needs_input_grad) else None
-        dt = _DT[q.dtype]
-        nws = lib().mia_relpos_fwd_ws_floats(dt, B, heads, Lq, Lk, D)
+        C, dt = lib(), _DT[dtype]
+        nws = C.mia_relpos_fwd_ws_floats(dt, B, heads, Lq, Lk, D)
         ws = torch.empty((nws,), **f32) if nws else None
         with on_device(dev):
-            lib().mia_relpos_bias(_p(table), _p(plan.index), plan.height, plan.width, heads, scale, _p(bias), _stream())
-            lib().mia_relpos_fwd(dt, _p(q), _p(k), _p(v), strides.buffer_info()[0], B, heads, Lq, Lk, D, _p(bias), plan.height,
-                                 plan.width, q_start, _p(mask), scale, pdrop, seed, ops.seed_offset(), _p(ws), nws, _p(out),
-                                 _p(stat), _stream())
+            stream = _stream()
+            C.mia_relpos_bias(_p(table), _p(plan.index), plan.height, plan.width, heads, scale, _p(bias), stream)
+            C.mia_relpos_fwd(dt, *ptrs, strides.buffer_info()[0], B, heads, Lq, Lk, D, _p(bias), plan.height, plan.width, q_start,
+                             _p(mask), scale, pdrop, seed, ops.seed_offset(), _p(ws), nws, _p(out), _p(stat), stream)
         ctx.strides = strides
         ctx.save_for_backward(q, k, v, bias, mask, out, stat)
         return out
@@ -127,47 +143,48 @@ class RelPosAttentionFn(torch.autograd.Function):
         B, heads, Lq, Lk, D, plan, scale, q_start, pdrop, seed, soff = ctx.meta
         if ctx.empty:
             q, k, v, table = ctx.saved_tensors
-            dt = torch.zeros_like(table)
-            if ctx.packed:
-                return (torch.zeros((B, Lq, 3, heads, D), dtype=q.dtype, device=q.device), None, None, dt) + (None,) * 6
-            return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), dt) + (None,) * 6
+            zeros = [torch.zeros_like(t) if t is not None else None for t in (q, k, v, table)]
+            return (*zeros, None, None, None, None, None, None)
         q, k, v, bias, mask, out, stat = ctx.saved_tensors
-        if ctx.packed:
-            dqkv = torch.empty((B, Lq, 3, heads, D), dtype=q.dtype, device=q.device)
-            dq, dk, dv = dqkv.unbind(2)
+        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if k is None:
+            dk = dv = None
+            ptrs = _packed_rows(q)[0]
+            gptrs, gst = _packed_rows(dq)
         else:
-            dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
-        dout = _rows(dout.contiguous())[0]
-        f32 = dict(dtype=torch.float32, device=q.device)
+            dk, dv = torch.empty(k.shape, dtype=k.dtype, device=k.device), torch.empty(v.shape, dtype=v.dtype, device=v.device)
+            ptrs, gptrs = (_p(q), _p(k), _p(v)), (_p(dq), _p(dk), _p(dv))
+            gst = (*dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3])
+        dout = dout.contiguous()
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
         want = ctx.needs_input_grad[3]
+        f32 = dict(dtype=torch.float32, device=q.device)
         dtable = torch.empty((plan.num_buckets, heads), **f32) if want else None
-        nws = lib().mia_relpos_bwd_ws_floats(_DT[q.dtype], B, heads, Lq, Lk, D, plan.height, plan.width, 1 if want else 0)
+        C, dt = lib(), _DT[q.dtype]
+        nws = C.mia_relpos_bwd_ws_floats(dt, B, heads, Lq, Lk, D, plan.height, plan.width, 1 if want else 0)
         ws = torch.empty((nws,), **f32)
-        gst = array("q", [s for t in (dq, dk, dv) for s in (0 if n == 1 else st for n, st in zip(t.shape[:3], t.stride()))])
+        gst = array("q", gst)
         with on_device(q.device):
-            lib().mia_relpos_bwd(_DT[q.dtype], _p(q), _p(k), _p(v), ctx.strides.buffer_info()[0], _p(dout), _p(out), _p(stat), B,
-                                 heads, Lq, Lk, D, _p(bias), plan.height, plan.width, q_start, _p(mask), scale, pdrop, seed, soff,
-                                 _p(plan.order), _p(plan.start), plan.num_buckets, _p(ws), nws, _p(dq), _p(dk), _p(dv),
-                                 gst.buffer_info()[0], _p(dtable), _stream())
-        if ctx.packed:
-            return (dqkv, None, None, dtable) + (None,) * 6
-        return (dq, dk, dv, dtable) + (None,) * 6
+            C.mia_relpos_bwd(dt, *ptrs, ctx.strides.buffer_info()[0], _p(dout), _p(out), _p(stat), B, heads, Lq, Lk, D, _p(bias),
+                             plan.height, plan.width, q_start, _p(mask), scale, pdrop, seed, soff, _p(plan.order), _p(plan.start),
+                             plan.num_buckets, _p(ws), nws, *gptrs, gst.buffer_info()[0], _p(dtable), _stream())
+        return dq, dk, dv, dtable, None, None, None, None, None, None
 
 
-def _attend(name, q, k, v, table, buckets, key_mask, scale, q_start, dropout_p, seed, packed):
-    B, Lq, heads, D = q.shape
-    Lk = k.shape[1]
-    if q.dtype not in _DT or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"{name}: queries, keys and values are all fp32 or all bf16 (got {q.dtype}, {k.dtype}, {v.dtype})")
+def _attend(name, q, k, v, B, Lq, Lk, heads, D, table, buckets, key_mask, scale, q_start, dropout_p, seed):
+    dtype = q.dtype
+    if dtype not in _DT or (k is not None and (k.dtype != dtype or v.dtype != dtype)):
+        raise TypeError(f"{name}: queries, keys and values are all fp32 or all bf16 (got {', '.join(str(t.dtype) for t in (q, k, v) if t is not None)})")
     if D % 8 or not 8 <= D <= 128:
         raise ValueError(f"{name}: the head width must be a multiple of 8 up to 128 (got {D})")
     tokens = buckets.height * buckets.width
     q_start = int(q_start)
     if Lk > tokens or q_start < 0 or q_start + Lq > tokens:
         raise ValueError(f"{name}: {Lk} keys and {Lq} queries from {q_start} on do not fit a map of {buckets.height} x {buckets.width}")
-    if tuple(table.shape) != (buckets.num_buckets, heads) or table.dtype != torch.float32:
+    if table.shape != (buckets.num_buckets, heads) or table.dtype != torch.float32:
         raise ValueError(f"{name}: the table must be fp32 {(buckets.num_buckets, heads)} (got {table.dtype} {tuple(table.shape)})")
-    if key_mask is not None and (tuple(key_mask.shape) != (B, Lk) or key_mask.dtype not in (torch.bool, torch.uint8)):
+    if key_mask is not None and (key_mask.shape != (B, Lk) or key_mask.dtype not in (torch.bool, torch.uint8)):
         raise ValueError(f"{name}: key_mask must be bool {(B, Lk)}, true where a key counts (got {key_mask.dtype} {tuple(key_mask.shape)})")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 1e-30 < scale < 1e30:
@@ -175,14 +192,14 @@ def _attend(name, q, k, v, table, buckets, key_mask, scale, q_start, dropout_p, 
     dropout_p = float(dropout_p)
     if not 0.0 <= dropout_p < 1.0:
         raise ValueError(f"{name}: dropout must be in [0, 1) (got {dropout_p})")
-    for what, t in (("queries", q), ("keys", k), ("values", v), ("table", table), ("buckets", buckets.index), ("key_mask", key_mask)):
-        if t is not None and (not t.is_cuda or t.device != q.device):
-            raise RuntimeError(f"{name} needs its tensors on one MI355X device; there is no CPU path ({what}: {t.device})")
+    device = q.get_device()
+    for t in (q, k, v, table, buckets.index, key_mask):
+        if t is not None and (device < 0 or t.get_device() != device):
+            raise RuntimeError(f"{name} needs its tensors (and its buckets) on one MI355X device; there is no CPU path (got {t.device})")
     if dropout_p > 0.0 and seed is None:
         from .head_ops import _seed
         seed = _seed()
-    first = (packed, None, None) if packed is not None else (q, k, v)
-    return RelPosAttentionFn.apply(*first, table, buckets, key_mask, scale, q_start, dropout_p, int(seed or 0))
+    return RelPosAttentionFn.apply(q, k, v, table, buckets, key_mask, scale, q_start, dropout_p, int(seed or 0))
 
 
 def relpos_attention(q, k, v, table, buckets, key_mask=None, scale=None, q_start=0, dropout_p=0.0, seed=None):
@@ -200,7 +217,8 @@ def relpos_attention(q, k, v, table, buckets, key_mask=None, scale=None, q_start
             raise ValueError(f"relpos_attention: {what} must be [batch, tokens, heads, D] (got {tuple(t.shape)})")
     if k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
         raise ValueError(f"relpos_attention: shapes do not belong together: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    return _attend("relpos_attention", q, k, v, table, buckets, key_mask, scale, q_start, dropout_p, seed, None)
+    B, Lq, heads, D = q.shape
+    return _attend("relpos_attention", q, k, v, B, Lq, k.shape[1], heads, D, table, buckets, key_mask, scale, q_start, dropout_p, seed)
 
 
 def relpos_self_attention(qkv, table, buckets, key_mask=None, scale=None, dropout_p=0.0, seed=None):
@@ -208,5 +226,5 @@ def relpos_self_attention(qkv, table, buckets, key_mask=None, scale=None, dropou
     back packed as well."""
     if qkv.dim() != 5 or qkv.shape[2] != 3:
         raise ValueError(f"relpos_self_attention: qkv must be [batch, tokens, 3, heads, D] (got {tuple(qkv.shape)})")
-    q, k, v = qkv.detach().unbind(2)
-    return _attend("relpos_self_attention", q, k, v, table, buckets, key_mask, scale, 0, dropout_p, seed, qkv)
+    B, L, _, heads, D = qkv.shape
+    return _attend("relpos_self_attention", qkv, None, None, B, L, L, heads, D, table, buckets, key_mask, scale, 0, dropout_p, seed)
