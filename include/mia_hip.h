@@ -231,20 +231,21 @@ int mia_relpos_bias(const float* table, const int* bucket, int height, int width
 /* q [B][Lq][heads][D], k, v [B][Lk][heads][D] with element strides {batch, token, head} of q, k, v in that order (HOST array of
  * 9; every row starts at a multiple of 16 bytes), D a multiple of 8 up to 128. key_mask (nullable): [B][Lk] bytes, 0 = the key
  * does not exist; a query without keys gives zeros. Dropout as in mia_attention_fwd, on element ((b*heads+h)*Lq+i)*Lk+j.
- * out: [B][Lq][heads][D] contiguous; stat (nullable): [B][heads][Lq][2], kept for the backward pass (the row's maximum and the
+ * out: [B][Lq][heads][D] contiguous; out_low (nullable): the same of what rounding took off out, kept for the backward pass in bf16
+ * (not written in fp32); stat (nullable): [B][heads][Lq][2], kept for the backward pass (the row's maximum and the
  * log2 of its sum of exponentials, +inf for a row without keys). ws: mia_relpos_fwd_ws_floats floats (0: none; few queries against many keys
  * are split over the keys and joined). */
 int mia_relpos_fwd(int dtype, const void* q, const void* k, const void* v, const long long* strides, int B, int heads, int Lq,
                    int Lk, int D, const float* bias, int height, int width, int q_start, const uint8_t* key_mask, float scale,
                    float pdrop, unsigned long long seed, const unsigned long long* seed_offset, float* ws,
-                   long long ws_floats, void* out, float* stat, void* stream);
+                   long long ws_floats, void* out, void* out_low, float* stat, void* stream);
 long long mia_relpos_fwd_ws_floats(int dtype, int B, int heads, int Lq, int Lk, int D);
-/* dout, out: [B][Lq][heads][D] contiguous; dq, dk, dv with their own strides (HOST array of 9); dtable [buckets][heads]
+/* dout, out, out_low (fp32: not read): [B][Lq][heads][D] contiguous; dq, dk, dv with their own strides (HOST array of 9); dtable [buckets][heads]
  * (nullable: not wanted), for which order lists the offsets sorted by bucket and start[buckets + 1] where each bucket's
  * begin in it. Nothing is added atomically across waves: the same bits every time. */
 int mia_relpos_bwd(int dtype, const void* q, const void* k, const void* v, const long long* strides, const void* dout,
-                   const void* out, const float* stat, int B, int heads, int Lq, int Lk, int D, const float* bias, int height,
-                   int width, int q_start, const uint8_t* key_mask, float scale, float pdrop, unsigned long long seed,
+                   const void* out, const void* out_low, const float* stat, int B, int heads, int Lq, int Lk, int D,
+                   const float* bias, int height, int width, int q_start, const uint8_t* key_mask, float scale, float pdrop, unsigned long long seed,
                    const unsigned long long* seed_offset, const int* order, const int* start, int buckets, float* ws,
                    long long ws_floats, void* dq, void* dk, void* dv, const long long* grad_strides, float* dtable,
                    void* stream);

@@ -14,12 +14,13 @@
 // softmax runs down registers plus two lane exchanges, and the four values are already the B operand of O^T = V^T P^T (V^T
 // read from the row-major tile by the transposing LDS read). fp32 runs the same code on 16x16x4. No L x L array exists in
 // memory; the backward recomputes P from the row statistics, once with queries as columns (dQ) and once with keys as
-// columns (dK, dV, dtable). P and dS are rounded to bf16 only as operands of bf16 products; statistics, D and the bias
-// gradient stay fp32.
+// columns (dK, dV, dtable). P and dS become bf16 only as operands of bf16 products (two numbers each for O and dQ);
+// statistics, D and the bias gradient stay fp32.
 //
 // D is needed to fp32 accuracy because the rows of dS sum to zero and a bucket's gradient is what is left of many terms. The
-// output a bf16 caller holds is too coarse for it. The dQ kernel therefore starts from D~ = dO . out, adds up
-// sum_j P_ij (dP_ij - D~_i) = D_i - D~_i in fp32 on the way, and leaves the exact D for the dK / dV / dtable kernel.
+// output a bf16 caller holds is too coarse for it: the forward keeps what its rounding took off beside it, the dQ kernel starts from
+// D~ = dO . (out + out_low), good to 2^-16, and leaves D~ + sum_j P_ij (dP_ij - D~_i) = D_i, added up in fp32 on the way, for
+// the dK / dV / dtable kernel.
 #include "common.h"
 
 typedef __attribute__((ext_vector_type(4))) float rp_f32x4;
@@ -39,8 +40,8 @@ struct RpStride {
     long long b, t, h;   // elements
 };
 struct RpArgs {
-    const void *q, *k, *v, *dout, *out;
-    void *o, *dq, *dk, *dv;
+    const void *q, *k, *v, *dout, *out, *out_low;
+    void *o, *o_low, *dq, *dk, *dv;   // o_low: what rounding o to bf16 took off it, for the backward's D; nullable
     RpStride sq, sk, sv, sdq, sdk, sdv;
     const float* bias;            // [heads][n_off]
     float2* stat;                 // [B][heads][Lq]: maximum of acc, log2 of the sum of exponentials
@@ -93,6 +94,12 @@ struct RpOp<bf16_t> {
     static __device__ __forceinline__ Pair pack(const rp_f32x4& x, const rp_f32x4& y) {
         return __builtin_bit_cast(Pair, make_uint4(pack_bf16x2(v2f{x[0], x[1]}), pack_bf16x2(v2f{x[2], x[3]}),
                                                    pack_bf16x2(v2f{y[0], y[1]}), pack_bf16x2(v2f{y[2], y[3]})));
+    }
+    // what pack rounded off x and y
+    static __device__ __forceinline__ Pair rest(const rp_f32x4& x, const rp_f32x4& y, const Pair& p) {
+        const uint4 w = __builtin_bit_cast(uint4, p);
+        const v2f a = unpack_bf16x2(w.x), b = unpack_bf16x2(w.y), c = unpack_bf16x2(w.z), d = unpack_bf16x2(w.w);
+        return pack(rp_f32x4{x[0] - a.x, x[1] - a.y, x[2] - b.x, x[3] - b.y}, rp_f32x4{y[0] - c.x, y[1] - c.y, y[2] - d.x, y[3] - d.y});
     }
     // A operand of a product over rows: rows ra .. ra+3 and rb .. rb+3 (per 16-lane group) of columns col0 .. col0+15.
     // ra_ptr / rb_ptr: element [ra][col0] of this lane's group.
@@ -239,6 +246,18 @@ __device__ __forceinline__ void rp_settle(V& v) {
     asm volatile("" : "+v"(v));
 }
 
+// Four channels of the output, and of what rounding took off them where the backward will want it.
+template <typename T>
+__device__ __forceinline__ void rp_store_out(const RpArgs& a, size_t at, rp_f32x4 x) {
+    store4<T>((T*)a.o + at, {x[0], x[1], x[2], x[3]});
+    if (sizeof(T) == 2 && a.o_low) {
+        rp_f32x4 y;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = x[r] - to_f32<T>(from_f32<T>(x[r]));
+        store4<T>((T*)a.o_low + at, {y[0], y[1], y[2], y[3]});
+    }
+}
+
 // Barrier between the waves' LDS work on one tile and the next. The wait is explicit because LDS additions return nothing that a
 // later instruction would wait for, and the compiler has been seen to leave none of its own in front of the barrier at a loop's
 // top: the ring below was then read before the last additions had arrived.
@@ -248,9 +267,9 @@ __device__ __forceinline__ void rp_barrier() {
 }
 
 enum { RP_FWD, RP_BWD_Q, RP_BWD_KV };
-// Waves a SIMD has room for: the most that leave a kernel without scratch. Asking for two already keeps the compiler from
-// spreading over the accumulation registers, whose moves cost issue slots (38x38 maps, batch 4, 8 heads of 64: forward 50 -> 45
-// us, dK/dV 140 -> 107).
+// Waves a SIMD has room for: the most that leave a kernel with at most a few registers in scratch (36 bytes at most). Asking for two
+// already keeps the compiler from spreading over the accumulation registers, whose moves cost issue slots (38x38 maps, batch
+// 4, 8 heads of 64: dK/dV 140 -> 103 us, forward unchanged).
 constexpr int rp_waves(int what, bool half, int DP, int cols) {
     if (what == RP_FWD)
         return half ? (cols == 1 ? (DP <= 32 ? 4 : DP <= 64 ? 3 : 2) : (DP <= 16 ? 3 : 2)) : (DP <= 32 ? 4 : DP <= 64 ? 3 : 2);
@@ -525,12 +544,20 @@ __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void
             typename Op::Pair p[QB];
 #pragma unroll
             for (int i = 0; i < QB; ++i) p[i] = Op::pack(s[2 * kk][i], s[2 * kk + 1][i]);
+            typename Op::Pair more[QB];
+            if constexpr (sizeof(T) == 2)
+#pragma unroll
+                for (int i = 0; i < QB; ++i) more[i] = Op::rest(s[2 * kk][i], s[2 * kk + 1][i], p[i]);
             if (!Dim::EARLY) values(kk);
             else if (kk == 0) values(1);
 #pragma unroll
-            for (int d = 0; d < Dim::DB; ++d)
+            for (int d = 0; d < Dim::DB; ++d) {
 #pragma unroll
                 for (int i = 0; i < QB; ++i) o[i][d] = Op::dot_t(vf[kk][d], p[i], o[i][d]);
+                if constexpr (sizeof(T) == 2)
+#pragma unroll
+                    for (int i = 0; i < QB; ++i) o[i][d] = Op::dot_t(vf[kk][d], more[i], o[i][d]);
+            }
         }
         }
     }
@@ -554,11 +581,11 @@ __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void
         }
         const float inv = total == 0.f ? 0.f : 1.0f / total;   // a row without keys is zero
         if (a.stat && g == 0) a.stat[row] = rp_stat(m[i], total);
-        T* op = (T*)a.o + (((size_t)b * a.Lq + qi[i]) * a.heads + h) * a.D;
+        const size_t at = (((size_t)b * a.Lq + qi[i]) * a.heads + h) * a.D;
 #pragma unroll
         for (int d = 0; d < Dim::DB; ++d) {
             const int col = d * 16 + g * 4;
-            if (col < a.D) store4<T>(op + col, {o[i][d][0] * inv, o[i][d][1] * inv, o[i][d][2] * inv, o[i][d][3] * inv});
+            if (col < a.D) rp_store_out<T>(a, at + col, o[i][d] * inv);
         }
     }
 }
@@ -600,7 +627,7 @@ __global__ __launch_bounds__(256) void relpos_join_kernel(RpArgs a) {
         }
         if (WHAT == RP_FWD) {
             const float inv = total == 0.f ? 0.f : 1.0f / total;
-            store4<T>((T*)a.o + ((b * a.Lq + t) * a.heads + h) * a.D + d, {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv});
+            rp_store_out<T>(a, ((b * a.Lq + t) * a.heads + h) * a.D + d, acc * inv);
             if (a.stat && d == 0) a.stat[row] = rp_stat(m, total);
         } else {
             store4<T>((T*)a.dq + b * a.sdq.b + t * a.sdq.t + h * a.sdq.h + d,
@@ -612,6 +639,13 @@ __global__ __launch_bounds__(256) void relpos_join_kernel(RpArgs a) {
 
 // ------------------------------------------------------------------------------------------------
 // backward, queries as columns: dQ and the exact D. The same walk as the forward.
+//
+// A row of dS sums to zero, so what the keys have in common drops out of dQ = dS K, but not out of what rounding dS to bf16, or an
+// inexact D~, does to it. dS is therefore multiplied as two bf16 numbers, its rounding and what that took off, and the forward
+// does the same with P (38x38 maps, batch 4, 8 heads of 64: 52 -> 57 us, forward 45 -> 49; 75x75, 4 heads of 32: 74 -> 87,
+// forward 71 -> 86). The error of dQ is then that of its own last rounding, 1.7e-3; with single roundings it was 2.4e-3 for keys
+// with nothing in common, 5.6e-3 for keys of mean 4 and deviation 1. dK and dV are sums over queries with no such
+// cancellation and take P and dS rounded once: 2.4e-3 (1.7e-3 for 103 -> 109 us with both split).
 // ------------------------------------------------------------------------------------------------
 template <typename T, int DP, int QB>
 __global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) void relpos_bwd_q_kernel(RpArgs a) {
@@ -654,6 +688,11 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) vo
         float d = 0.f;
 #pragma unroll
         for (int c = 0; c < Dim::NCH; ++c) d += Op::inner(gf[i][c], of[c]);
+        if (sizeof(T) == 2) {
+            rp_row_frags<T, DP>((const T*)a.out_low + orow, ok, a.D, g, of);
+#pragma unroll
+            for (int c = 0; c < Dim::NCH; ++c) d += Op::inner(gf[i][c], of[c]);
+        }
         D0[i] = rp_xor_sum(d);
         const float2 st = a.stat[(size_t)bh * a.Lq + row];
         mx[i] = st.x;
@@ -803,6 +842,10 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) vo
             typename Op::Pair p[QB];
 #pragma unroll
             for (int i = 0; i < QB; ++i) p[i] = Op::pack(ds[0][i], ds[1][i]);
+            typename Op::Pair more[QB];
+            if constexpr (sizeof(T) == 2)
+#pragma unroll
+                for (int i = 0; i < QB; ++i) more[i] = Op::rest(ds[0][i], ds[1][i], p[i]);
 #pragma unroll
             for (int d = 0; d < Dim::DB; ++d) {
                 if constexpr (!Dim::EARLY) {
@@ -811,6 +854,9 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) vo
                 }
 #pragma unroll
                 for (int i = 0; i < QB; ++i) dq[i][d] = Op::dot_t(kt_[d], p[i], dq[i][d]);
+                if constexpr (sizeof(T) == 2)
+#pragma unroll
+                    for (int i = 0; i < QB; ++i) dq[i][d] = Op::dot_t(kt_[d], more[i], dq[i][d]);
             }
         }
         }
@@ -1214,8 +1260,11 @@ static size_t rp_es(int dtype) { return dtype == MIA_BF16 ? 2 : 4; }
 // cols: 16-wide columns of a wave, so 64 * cols queries (keys) of a workgroup. Two serve more products with every operand read from
 // LDS; they are taken unless only the narrower workgroups fill the chip. fp32 keeps one: its operands are twice as large.
 // splits: ranges of the tokens a workgroup walks, joined afterwards. The grid runs in turns of as many workgroups as are resident
-// (two a CU with two columns, three with one), so s splits take ceil(workgroups * s / resident) / s of an unsplit walk, plus
-// what starting and joining them costs; ranges of at least four rounds.
+// (two a CU with two columns, three with one), so s splits take ceil(workgroups * s / resident) turns of ceil(rounds / s)
+// rounds each, plus about a fiftieth of the walk per split for starting and joining it; ranges of at least four rounds. Measured: 64
+// workgroups over 16384 keys 52 + 6.6 us (kernel + join) at 7 splits, 48 + 7.1 at 8, 61 + 8.4 at 10; the forward on a 75x75
+// map, 4 heads of 32, 120 us unsplit, 84 + 5 at 2, 72 + 5.5 at 4 and 5, 76 + 7 at 6; on 38x38 maps, batch 4, 8 heads of 64,
+// where the workgroups fill the chip, 45 us unsplit and 45 + 9.7 at 3.
 struct RpPlan {
     int cols, splits;
 };
@@ -1226,21 +1275,15 @@ static RpPlan rp_plan(int what, int dtype, int B, int heads, int Lq, int Lk, int
     RpPlan p;
     const long long one = bh * ((owned + 63) / 64), two = bh * ((owned + 127) / 128), rounds = (walked + round - 1) / round;
     p.cols = dtype == MIA_F32 || DP > (what == RP_FWD ? 96 : 64) || owned <= 64 || (two < 512 && one >= 512) ? 1 : 2;
-#ifdef RP_TUNE
-    if (const char* e = getenv(what == RP_FWD ? "RP_CF" : what == RP_BWD_Q ? "RP_CQ" : "RP_CK")) p.cols = atoi(e);
-#endif
     const long long wgs = p.cols == 1 ? one : two;
     const long long resident = 256 * (p.cols == 1 ? 3 : 2), most = rounds / 4 < 64 ? rounds / 4 : 64;
     long long s = 1;
     double best = 1e30;
     for (long long i = 1; i <= most && (i == 1 || wgs < 2 * resident); ++i) {
-        const double t = (double)((wgs * i + resident - 1) / resident) / i + 0.02 * i;
-        if (t < best - 0.1 * (s == 1)) best = t, s = i;
+        const double t = (double)((wgs * i + resident - 1) / resident * ((rounds + i - 1) / i)) + 0.02 * rounds * i;
+        if (t < best - 0.1 * rounds * (s == 1)) best = t, s = i;
     }
-#ifdef RP_TUNE
-    if (const char* e = getenv(what == RP_FWD ? "RP_SF" : what == RP_BWD_Q ? "RP_SQ" : "RP_SK")) s = atoi(e);
-#endif
-    p.splits = (int)(s > most ? (most < 1 ? 1 : most) : s);
+    p.splits = (int)s;
     return p;
 }
 
@@ -1372,16 +1415,17 @@ extern "C" long long mia_relpos_fwd_ws_floats(int dtype, int B, int heads, int L
 extern "C" int mia_relpos_fwd(int dtype, const void* q, const void* k, const void* v, const long long* strides, int B, int heads,
                               int Lq, int Lk, int D, const float* bias, int height, int width, int q_start,
                               const uint8_t* key_mask, float scale, float pdrop, unsigned long long seed,
-                              const unsigned long long* seed_offset, float* ws, long long ws_floats, void* out, float* stat,
-                              void* stream) {
+                              const unsigned long long* seed_offset, float* ws, long long ws_floats, void* out, void* out_low,
+                              float* stat, void* stream) {
     if (rp_checks("mia_relpos_fwd", dtype, B, heads, Lq, Lk, D, height, width, q_start, scale, pdrop)) return -1;
     MIA_CHECK_ARG(q && k && v && strides && bias && out, "mia_relpos_fwd: null");
     MIA_CHECK_ARG(((uintptr_t)stat & 7) == 0, "mia_relpos_fwd: stat must start at a multiple of 8 bytes");
     RpArgs a = {};
-    a.q = q; a.k = k; a.v = v; a.o = out; a.bias = bias; a.mask = key_mask; a.stat = reinterpret_cast<float2*>(stat);
+    a.q = q; a.k = k; a.v = v; a.o = out; a.o_low = out_low; a.bias = bias; a.mask = key_mask; a.stat = reinterpret_cast<float2*>(stat);
     a.sq = rp_stride(strides); a.sk = rp_stride(strides + 3); a.sv = rp_stride(strides + 6);
     if (rp_aligned("mia_relpos_fwd", dtype, q, a.sq) || rp_aligned("mia_relpos_fwd", dtype, k, a.sk) ||
-        rp_aligned("mia_relpos_fwd", dtype, v, a.sv) || rp_aligned("mia_relpos_fwd", dtype, out, RpStride{0, 0, 0}))
+        rp_aligned("mia_relpos_fwd", dtype, v, a.sv) || rp_aligned("mia_relpos_fwd", dtype, out, RpStride{0, 0, 0}) ||
+        rp_aligned("mia_relpos_fwd", dtype, out_low, RpStride{0, 0, 0}))
         return -1;
     rp_fill(a, B, heads, Lq, Lk, D, height, width, q_start, scale, pdrop, seed, seed_offset);
     const int stage = rp_stage(dtype, rp_dp(D));
@@ -1437,13 +1481,14 @@ extern "C" long long mia_relpos_bwd_ws_floats(int dtype, int B, int heads, int L
 }
 
 extern "C" int mia_relpos_bwd(int dtype, const void* q, const void* k, const void* v, const long long* strides, const void* dout,
-                              const void* out, const float* stat, int B, int heads, int Lq, int Lk, int D, const float* bias,
+                              const void* out, const void* out_low, const float* stat, int B, int heads, int Lq, int Lk, int D, const float* bias,
                               int height, int width, int q_start, const uint8_t* key_mask, float scale, float pdrop,
                               unsigned long long seed, const unsigned long long* seed_offset, const int* order, const int* start,
                               int buckets, float* ws, long long ws_floats, void* dq, void* dk, void* dv,
                               const long long* grad_strides, float* dtable, void* stream) {
     if (rp_checks("mia_relpos_bwd", dtype, B, heads, Lq, Lk, D, height, width, q_start, scale, pdrop)) return -1;
     MIA_CHECK_ARG(q && k && v && strides && dout && out && stat && bias && ws && dq && dk && dv && grad_strides, "mia_relpos_bwd: null");
+    MIA_CHECK_ARG(dtype != MIA_BF16 || out_low, "mia_relpos_bwd: bf16 needs the forward's out_low");
     MIA_CHECK_ARG(((uintptr_t)stat & 7) == 0, "mia_relpos_bwd: stat must start at a multiple of 8 bytes");
     MIA_CHECK_ARG(!dtable || (order && start && buckets > 0), "mia_relpos_bwd: the bias gradient needs the bucket lists");
     MIA_CHECK_ARG(heads <= 65535, "mia_relpos_bwd: %d heads are too many", heads);
@@ -1451,14 +1496,14 @@ extern "C" int mia_relpos_bwd(int dtype, const void* q, const void* k, const voi
     MIA_CHECK_ARG(ws_floats >= w.total, "mia_relpos_bwd: workspace of %lld floats is too small (%lld needed)", ws_floats, w.total);
     MIA_CHECK_ARG(((uintptr_t)ws & 15) == 0, "mia_relpos_bwd: the workspace must start at a multiple of 16 bytes");
     RpArgs a = {};
-    a.q = q; a.k = k; a.v = v; a.dout = dout; a.out = out; a.bias = bias; a.mask = key_mask;
+    a.q = q; a.k = k; a.v = v; a.dout = dout; a.out = out; a.out_low = out_low; a.bias = bias; a.mask = key_mask;
     a.stat = reinterpret_cast<float2*>(const_cast<float*>(stat));
     a.dq = dq; a.dk = dk; a.dv = dv; a.dsum = ws;
     a.sq = rp_stride(strides); a.sk = rp_stride(strides + 3); a.sv = rp_stride(strides + 6);
     a.sdq = rp_stride(grad_strides); a.sdk = rp_stride(grad_strides + 3); a.sdv = rp_stride(grad_strides + 6);
-    const void* ptrs[] = {q, k, v, dq, dk, dv, dout, out};
-    const RpStride sts[] = {a.sq, a.sk, a.sv, a.sdq, a.sdk, a.sdv, {0, 0, 0}, {0, 0, 0}};
-    for (int i = 0; i < 8; ++i)
+    const void* ptrs[] = {q, k, v, dq, dk, dv, dout, out, out_low};
+    const RpStride sts[] = {a.sq, a.sk, a.sv, a.sdq, a.sdk, a.sdv, {0, 0, 0}, {0, 0, 0}, {0, 0, 0}};
+    for (int i = 0; i < 9; ++i)
         if (rp_aligned("mia_relpos_bwd", dtype, ptrs[i], sts[i])) return -1;
     rp_fill(a, B, heads, Lq, Lk, D, height, width, q_start, scale, pdrop, seed, seed_offset);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);

@@ -125,7 +125,9 @@ class RelPosAttentionFn(torch.autograd.Function):
             mask = mask.contiguous()
         strides = array("q", strides)
         bias = torch.empty((heads, plan.index.numel()), **f32)
-        stat = torch.empty((B, heads, Lq, 2), **f32) if any(ctx.needs_input_grad) else None
+        grads = any(ctx.needs_input_grad)
+        stat = torch.empty((B, heads, Lq, 2), **f32) if grads else None
+        low = torch.empty_like(out) if grads and dtype == torch.bfloat16 else None
         C, dt = lib(), _DT[dtype]
         nws = C.mia_relpos_fwd_ws_floats(dt, B, heads, Lq, Lk, D)
         ws = torch.empty((nws,), **f32) if nws else None
@@ -133,9 +135,9 @@ class RelPosAttentionFn(torch.autograd.Function):
             stream = _stream()
             C.mia_relpos_bias(_p(table), _p(plan.index), plan.height, plan.width, heads, scale, _p(bias), stream)
             C.mia_relpos_fwd(dt, *ptrs, strides.buffer_info()[0], B, heads, Lq, Lk, D, _p(bias), plan.height, plan.width, q_start,
-                             _p(mask), scale, pdrop, seed, ops.seed_offset(), _p(ws), nws, _p(out), _p(stat), stream)
+                             _p(mask), scale, pdrop, seed, ops.seed_offset(), _p(ws), nws, _p(out), _p(low), _p(stat), stream)
         ctx.strides = strides
-        ctx.save_for_backward(q, k, v, bias, mask, out, stat)
+        ctx.save_for_backward(q, k, v, bias, mask, out, low, stat)
         return out
 
     @staticmethod
@@ -145,7 +147,7 @@ class RelPosAttentionFn(torch.autograd.Function):
             q, k, v, table = ctx.saved_tensors
             zeros = [torch.zeros_like(t) if t is not None else None for t in (q, k, v, table)]
             return (*zeros, None, None, None, None, None, None)
-        q, k, v, bias, mask, out, stat = ctx.saved_tensors
+        q, k, v, bias, mask, out, low, stat = ctx.saved_tensors
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         if k is None:
             dk = dv = None
@@ -166,7 +168,7 @@ class RelPosAttentionFn(torch.autograd.Function):
         ws = torch.empty((nws,), **f32)
         gst = array("q", gst)
         with on_device(q.device):
-            C.mia_relpos_bwd(dt, *ptrs, ctx.strides.buffer_info()[0], _p(dout), _p(out), _p(stat), B, heads, Lq, Lk, D, _p(bias),
+            C.mia_relpos_bwd(dt, *ptrs, ctx.strides.buffer_info()[0], _p(dout), _p(out), _p(low), _p(stat), B, heads, Lq, Lk, D, _p(bias),
                              plan.height, plan.width, q_start, _p(mask), scale, pdrop, seed, soff, _p(plan.order), _p(plan.start),
                              plan.num_buckets, _p(ws), nws, *gptrs, gst.buffer_info()[0], _p(dtable), _stream())
         return dq, dk, dv, dtable, None, None, None, None, None, None

@@ -2,10 +2,11 @@
 
 Bounds. fp32: every product or sum of n terms is off by at most n 2^-24 of its largest magnitude; a score of at most ~16 in
 size from D products, its exponential, and a sum over L terms give `c32 = 8 (D + 64) + L` roundings of 2^-24 relative to
-the largest output. bf16 inputs are exact; P and dS are rounded once (half a step, 2^-8 of each) as matrix operands, results once
-more, and dQ starts from row sums D of an output that was itself rounded to bf16:
-  out: 2^-8 (P |v| + |out|)              dV: 2^-8 (P^T |dO| + |dV|)
-  dK:  2^-8 (scale |dS|^T |q| + |dK|)    dQ: 2^-8 (scale |dS| |k| + |dQ|) + scale 2^-8 (|dO| . (|out| + P |v|)) (P |k|)
+the largest output. bf16 inputs are exact. P for dV and dS for dK are rounded once (half a step, 2^-8 of each) as matrix
+operands, P for out and dS for dQ to two numbers (2^-16 of each is left), results once; dQ starts from row sums D of an output kept
+to 2^-16 of its terms:
+  out: 2^-16 P |v| + 2^-8 |out|          dV: 2^-8 (P^T |dO| + |dV|)
+  dK:  2^-8 (scale |dS|^T |q| + |dK|)    dQ: 2^-16 scale |dS| |k| + 2^-8 |dQ| + scale 2^-16 (|dO| . (|out| + P |v|)) (P |k|)
 The table's gradient is fp32 in both: c32 2^-24 times the sum of |dS| of its bucket."""
 import numpy as np
 import torch
@@ -58,7 +59,7 @@ def formula(q, k, v, table, plan, mask=None, scale=None, q_start=0, dout=None, d
     back = lambda t: t.permute(0, 2, 1, 3)      # noqa: E731
     got, tol = {"out": back(out)}, {}
     pv = pd @ v.abs()
-    tol["out"] = back((H * (pv + out.abs()) if half else 0.0) + eps * (1e-30 + pv.max()) * torch.ones_like(out))
+    tol["out"] = back((H * (H * pv + out.abs()) if half else 0.0) + eps * (1e-30 + pv.max()) * torch.ones_like(out))
     if dout is None:
         return got, tol
     do = dout.detach().cpu().double().permute(0, 2, 1, 3)
@@ -76,7 +77,7 @@ def formula(q, k, v, table, plan, mask=None, scale=None, q_start=0, dout=None, d
     kk, qq = scale * size @ k.abs(), scale * size.transpose(2, 3) @ q.abs()
     tol["dk"] = back((H * (scale * ds.abs().transpose(2, 3) @ q.abs() + dk.abs()) if half else 0.0) + eq * (1e-30 + qq.max()) * one(dk))
     slack = (do.abs() * (out.abs() + pv)).sum(-1, keepdim=True) * (p @ k.abs()) * scale
-    tol["dq"] = back((H * (scale * ds.abs() @ k.abs() + dq.abs() + slack * (1 + H)) if half else 0.0) + eq * (1e-30 + kk.max()) * one(dq))
+    tol["dq"] = back((H * (H * scale * ds.abs() @ k.abs() + dq.abs() + H * slack * (1 + H)) if half else 0.0) + eq * (1e-30 + kk.max()) * one(dq))
     dt, da = torch.zeros(plan.num_buckets, heads, dtype=torch.float64), torch.zeros(plan.num_buckets, heads, dtype=torch.float64)
     flat = bucket.reshape(-1)
     dt.index_add_(0, flat, ds.sum(0).reshape(heads, -1).t())

@@ -75,7 +75,7 @@ def test_formula_against_autograd():
 def _fwd(dtype=0, q=P, strides=None, B=1, heads=2, Lq=5, Lk=9, D=16, bias=P, height=3, width=3, q_start=0, scale=0.25, pdrop=0.0, ws=None, n=0):
     st = array("q", strides or [80, 32, 16] * 3)
     mia_amd.lib().mia_relpos_fwd(dtype, q, P, P, st.buffer_info()[0], B, heads, Lq, Lk, D, bias, height, width, q_start, None, scale, pdrop, 0,
-                                 None, ws, n, P, None, None)
+                                 None, ws, n, P, None, None, None)
 
 
 @pytest.mark.parametrize("kw,match", [
@@ -96,12 +96,12 @@ def test_backward_entry_refuses():
     need = lib.mia_relpos_bwd_ws_floats(0, 1, 2, 5, 9, 16, 3, 3, 1)
     assert need > lib.mia_relpos_bwd_ws_floats(0, 1, 2, 5, 9, 16, 3, 3, 0) > 0
 
-    def bwd(dout=P, stat=P, order=P, buckets=3, n=need, dq=P):
+    def bwd(dout=P, stat=P, order=P, buckets=3, n=need, dq=P, dtype=0, low=None):
         a = st.buffer_info()[0]
-        lib.mia_relpos_bwd(0, P, P, P, a, dout, P, stat, 1, 2, 5, 9, 16, P, 3, 3, 0, None, 0.25, 0.0, 0, None, order, P, buckets, P, n, dq, P, P, a,
+        lib.mia_relpos_bwd(dtype, P, P, P, a, dout, P, low, stat, 1, 2, 5, 9, 16, P, 3, 3, 0, None, 0.25, 0.0, 0, None, order, P, buckets, P, n, dq, P, P, a,
                            P, None)
     for kw, match in ((dict(dout=None), "null"), (dict(stat=None), "null"), (dict(order=None), "bucket lists"), (dict(buckets=0), "bucket lists"),
-                      (dict(n=need - 1), "too small"), (dict(dq=ctypes.c_void_p(4100)), "16 bytes")):
+                      (dict(n=need - 1), "too small"), (dict(dtype=1), "out_low"), (dict(dtype=1, low=ctypes.c_void_p(4100)), "16 bytes"), (dict(dq=ctypes.c_void_p(4100)), "16 bytes")):
         with pytest.raises(mia_amd.MiaError, match=match):
             bwd(**kw)
     with pytest.raises(mia_amd.MiaError, match="null"):

@@ -147,6 +147,35 @@ def test_memory_layouts(dtype):
         _check(plan, D=24, dtype=dtype, place=place, packed=True)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("height,width,D", [(1, 2, 8), (10, 10, 48), (1, 300, 32)])
+def test_keys_with_a_common_part(height, width, D, dtype):
+    """What all keys share drops out of the gradient of the queries: it must not come back through rounded weights."""
+    plan = RelativePositionBuckets(height, width, 8, 16)
+    n = height * width
+    q, k, v, table, dout = _inputs(3, n, n, 2, D, dtype, plan.num_buckets, 16)
+    k = (k.float() + 20.0).to(dtype)
+    q = (q.float() * 0.05).to(dtype)
+    mine = [t.cuda().requires_grad_() for t in (q, k, v, table)]
+    want, tol = formula(q, k, v, table, plan, dout=dout)
+    out = relpos_attention(*mine, plan)
+    for name, value in zip(("out", "dq", "dk", "dv", "dtable"), (out.detach(), *torch.autograd.grad(out, mine, dout.cuda()))):
+        _compare(value, want[name], tol[name], name)
+
+
+@pytest.mark.parametrize("height,width", [(7, 30), (1, 500), (3, 97)])
+def test_bias_gradient_repeats(height, width):
+    """One bucket per offset over several tiles of queries: every single sum has the same bits each time."""
+    plan = RelativePositionBuckets.from_index(height, width, torch.arange((2 * height - 1) * (2 * width - 1)))
+    n = height * width
+    q, k, v, table, dout = _inputs(8, n, n, 4, 32, BF16, plan.num_buckets, 17)
+    mine = [t.cuda().requires_grad_() for t in (q, k, v, table)]
+    dout = dout.cuda()
+    first = torch.autograd.grad(relpos_attention(*mine, plan), mine, dout)
+    for _ in range(6):
+        assert all(torch.equal(a, b) for a, b in zip(first, torch.autograd.grad(relpos_attention(*mine, plan), mine, dout)))
+
+
 def test_custom_buckets():
     """One bucket for every offset, one for all, and buckets that no offset falls into."""
     g = torch.Generator().manual_seed(5)
