@@ -8,6 +8,8 @@ import torch.nn.functional as F
 
 from . import ops
 from ._lib import lib
+from .block_norm import gated_residual_norm
+from .relpos import relpos_self_attention
 from .ops import ACT_NONE, ACT_RELU, _DT, _p, _stream
 
 
@@ -217,8 +219,19 @@ def mha_head_forward(m, x):
     bqkv = torch.cat((m.query.bias, m.key.bias, m.value.bias), 0)
     qkv = LinearFn.apply(t, wqkv, bqkv, None, ACT_NONE)
     p_att = m.attention_dropout.p if training else 0.0
-    a = AttentionFn.apply(qkv, B, HW, C, m.num_heads, p_att, _seed() if p_att > 0 else 0)
-    x3 = LinearFn.apply(a, m.output_projection.weight, m.output_projection.bias, t, ACT_NONE).view(B, H, W, C)
+    if m.relative_position_table is not None:
+        a = relpos_self_attention(qkv.view(B, HW, 3, m.num_heads, C // m.num_heads), m.relative_position_table,
+                                  m.position_plan(H, W, x2.device), dropout_p=p_att).view(B * HW, C)
+    else:
+        a = AttentionFn.apply(qkv, B, HW, C, m.num_heads, p_att, _seed() if p_att > 0 else 0)
+    proj = m.output_projection
+    if m.residual_norm:
+        branch = LinearFn.apply(a, proj.weight, proj.bias, None, ACT_NONE)
+        _, x3 = gated_residual_norm(t, branch, scale=m.residual_scale, pre=m.residual_norm, pre_weight=m.residual_norm_weight,
+                                    pre_bias=m.residual_norm_bias)
+        x3 = x3.view(B, H, W, C)
+    else:
+        x3 = LinearFn.apply(a, proj.weight, proj.bias, t, ACT_NONE).view(B, H, W, C)
     c = m.classifier
     p1 = c[3].p if training else 0.0
     z = PoolNormFn.apply(x3, c[2].weight, c[2].bias, c[2].eps, p1, _seed() if p1 > 0 else 0)

@@ -9,7 +9,9 @@ Differences that a caller can observe:
   * the trunk is this package's EfficientNetB3Features (timm is not needed); `pretrained=True`
     cannot download weights (no network) and raises unless MIA_ALLOW_RANDOM_INIT=1 is set;
   * segmentation heads are the reference's two decoders on this package's kernels (mia_amd.decoders);
-  * new optional `compute_dtype` ('fp32' | 'bf16'; config key runtime.dtype), default fp32 as in the reference.
+  * new optional `compute_dtype` ('fp32' | 'bf16'; config key runtime.dtype), default fp32 as in the reference;
+  * new optional attention-head settings (config keys model.relative_position_buckets, model.relative_position_distance,
+    model.residual_norm), off by default: see heads.MultiHeadAttentionClassifier.
 """
 import logging
 import os
@@ -43,8 +45,11 @@ class FoundationModel(nn.Module):
     def __init__(self, backbone: str = "efficientnet-b3", pretrained: bool = True, dropout: float = 0.2,
                  classification_heads: Optional[Dict[str, int]] = None,
                  segmentation_heads: Optional[Dict[str, int]] = None, use_attention: bool = True,
-                 num_attention_heads: int = 8, compute_dtype="fp32"):
+                 num_attention_heads: int = 8, compute_dtype="fp32", relative_position_buckets: int = 0,
+                 relative_position_distance: int = 128, residual_norm: Optional[str] = None):
         super().__init__()
+        if not use_attention and (relative_position_buckets or residual_norm):
+            raise ValueError("relative_position_buckets and residual_norm belong to the attention heads (use_attention=True)")
         if backbone not in _BACKBONES:
             raise ValueError(f"Unsupported backbone {backbone!r}: this build implements {_BACKBONES[0]} only")
         if pretrained and os.environ.get("MIA_ALLOW_RANDOM_INIT") != "1":
@@ -56,6 +61,8 @@ class FoundationModel(nn.Module):
         self.segmentation_heads = segmentation_heads or {}
         self.use_attention = use_attention
         self.num_attention_heads = num_attention_heads
+        self.attention_options = dict(relative_position_buckets=relative_position_buckets or 0,
+                                      relative_position_distance=relative_position_distance, residual_norm=residual_norm)
         dt = compute_dtype if isinstance(compute_dtype, torch.dtype) else _DTYPES[compute_dtype]
         self.backbone = EfficientNetB3Features(compute_dtype=dt)
         self.feature_dims = list(self.backbone.feature_dims)
@@ -68,7 +75,8 @@ class FoundationModel(nn.Module):
 
     def _make_cls_head(self, num_classes, dropout):
         if self.use_attention:
-            return MultiHeadAttentionClassifier(self.feature_dims[-1], self.num_attention_heads, num_classes, dropout)
+            return MultiHeadAttentionClassifier(self.feature_dims[-1], self.num_attention_heads, num_classes, dropout,
+                                                **self.attention_options)
         return SimpleHead(self.feature_dims[-1], num_classes, dropout)
 
     def _make_seg_head(self, num_classes, dropout):
@@ -125,7 +133,8 @@ class FoundationModel(nn.Module):
 def create_foundation_model(config: dict = None, backbone: str = None, pretrained: bool = None, dropout: float = None,
                             classification_heads: dict = None, segmentation_heads: dict = None,
                             use_attention: bool = None, num_attention_heads: int = None,
-                            compute_dtype=None) -> FoundationModel:
+                            compute_dtype=None, relative_position_buckets: int = 0,
+                            relative_position_distance: int = 128, residual_norm: str = None) -> FoundationModel:
     """model.py:497-546. The config form reads config['model'][...] and the two dataset lists."""
     if config is not None:
         classification_heads = {}
@@ -141,13 +150,18 @@ def create_foundation_model(config: dict = None, backbone: str = None, pretraine
                                segmentation_heads=segmentation_heads,
                                use_attention=config["model"].get("use_attention", True),
                                num_attention_heads=config["model"].get("num_attention_heads", 8),
-                               compute_dtype=compute_dtype)
+                               compute_dtype=compute_dtype,
+                               relative_position_buckets=config["model"].get("relative_position_buckets", relative_position_buckets),
+                               relative_position_distance=config["model"].get("relative_position_distance", relative_position_distance),
+                               residual_norm=config["model"].get("residual_norm", residual_norm))
     return FoundationModel(backbone=backbone or "efficientnet-b3",
                            pretrained=pretrained if pretrained is not None else True, dropout=dropout or 0.2,
                            classification_heads=classification_heads or {},
                            segmentation_heads=segmentation_heads or {},
                            use_attention=use_attention if use_attention is not None else True,
-                           num_attention_heads=num_attention_heads or 8, compute_dtype=compute_dtype)
+                           num_attention_heads=num_attention_heads or 8, compute_dtype=compute_dtype,
+                           relative_position_buckets=relative_position_buckets,
+                           relative_position_distance=relative_position_distance, residual_norm=residual_norm)
 
 
 def load_model_weights_safely(model, checkpoint, logger=None, suppress_warnings=False):

@@ -1,0 +1,71 @@
+"""The attention head's optional position bias and residual norm: what they add to a model, and what they refuse."""
+import pytest
+
+import mia_amd  # noqa: F401
+from mia_amd.heads import MultiHeadAttentionClassifier
+from mia_amd.src.model import FoundationModel, create_foundation_model
+
+NEW = ["relative_position_table", "residual_norm_bias", "residual_norm_weight", "residual_scale"]
+
+
+def _keys(head):
+    return [k for k in head.state_dict() if not k.startswith(("cbam", "classifier", "query", "key", "value", "output_projection"))]
+
+
+def test_state_dict_keys():
+    assert _keys(MultiHeadAttentionClassifier(64, 8, 2)) == []
+    assert _keys(MultiHeadAttentionClassifier(64, 8, 2, relative_position_buckets=8)) == NEW[:1]
+    assert sorted(_keys(MultiHeadAttentionClassifier(64, 8, 2, residual_norm="rms"))) == NEW[2:]
+    full = MultiHeadAttentionClassifier(64, 8, 2, relative_position_buckets=8, residual_norm="layer")
+    assert sorted(_keys(full)) == NEW
+    assert full.relative_position_table.shape == (64, 8) and not full.relative_position_table.any()
+    assert bool((full.residual_scale == 1).all())
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(relative_position_buckets=6), "multiple of 4"), (dict(relative_position_buckets=2), "multiple of 4"),
+    (dict(relative_position_buckets=16, relative_position_distance=4), "beyond its quarter"), (dict(residual_norm="batch"), "residual_norm")])
+def test_refusals(kw, match):
+    with pytest.raises(ValueError, match=match):
+        MultiHeadAttentionClassifier(64, 8, 2, **kw)
+
+
+def test_head_width_is_refused_only_with_the_bias():
+    MultiHeadAttentionClassifier(60, 5, 2)
+    with pytest.raises(ValueError, match="multiple of 8"):
+        MultiHeadAttentionClassifier(60, 5, 2, relative_position_buckets=8)
+
+
+def test_model_options():
+    kw = dict(pretrained=False, classification_heads={"a": 2})
+    m = FoundationModel(relative_position_buckets=8, residual_norm="rms", **kw)
+    m.add_classification_head("b", 3)
+    for name in "ab":
+        assert sorted(_keys(m.classification_layers[name])) == [NEW[0], *NEW[2:]]
+    assert _keys(FoundationModel(**kw).classification_layers["a"]) == []
+    with pytest.raises(ValueError, match="use_attention"):
+        FoundationModel(use_attention=False, residual_norm="rms", **kw)
+    config = {"model": {"backbone": "efficientnet_b3", "pretrained": False, "dropout": 0.2, "relative_position_buckets": 16, "residual_norm": "layer"},
+              "classification_datasets": [{"name": "a", "classes": ["x", "y"]}]}
+    m = create_foundation_model(config)
+    assert sorted(_keys(m.classification_layers["a"])) == NEW
+    assert m.classification_layers["a"].relative_position_table.shape == (256, 8)
+    del config["model"]["relative_position_buckets"], config["model"]["residual_norm"]
+    assert _keys(create_foundation_model(config).classification_layers["a"]) == []
+
+
+@pytest.mark.parametrize("height,width", [(1, 5), (4, 1), (3, 7), (12, 2)])
+def test_plan_of_a_map(height, width):
+    """One table serves maps of every size, a single row among them; the buckets are those of a loop over the pairs."""
+    import torch
+    from position_head import PositionHead
+    head = MultiHeadAttentionClassifier(64, 8, 2, relative_position_buckets=8, relative_position_distance=9)
+    ref = PositionHead(64, 8, 2, buckets=8, distance=9)
+    with torch.no_grad():
+        ref.relative_position_table.copy_(torch.arange(64 * 8, dtype=torch.float32).reshape(64, 8))
+    plan = head.position_plan(height, width, "cpu")
+    assert plan is head.position_plan(height, width, "cpu") and plan.num_buckets == 64
+    from relpos_formula import offsets
+    n = height * width
+    bucket = plan.index.long()[offsets(height, width, n, n, 0)]
+    assert torch.equal(ref.relative_position_table[bucket].permute(2, 0, 1), ref.bias(height, width))

@@ -1,0 +1,151 @@
+"""The new operators together, as the attention head and a training step use them, against plain torch on the CPU in float64.
+
+Bounds: an output or gradient passes through about ten fp32 products of at most 512 terms, each off by at most 512 * 2^-24 =
+3e-5 of its largest magnitude: 3e-4 of each tensor's largest magnitude for outputs; gradients pass through twice as many, 1e-3
+with the sums over the batch's tokens."""
+import copy
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import mia_amd  # noqa: E402,F401
+from mia_amd.graphs import GraphedForward, GraphedTrainStep  # noqa: E402
+from mia_amd.head_ops import CrossEntropyLoss  # noqa: E402
+from mia_amd.heads import MultiHeadAttentionClassifier  # noqa: E402
+from mia_amd.optim import AdamW, clip_grad_norm_  # noqa: E402
+from mia_amd.src.model import FoundationModel  # noqa: E402
+from position_head import PositionHead  # noqa: E402
+from seeding import randn, seeded_state_dict  # noqa: E402
+
+
+def rel(a, b):
+    a, b = a.detach().double().cpu(), b.detach().double().cpu()
+    return float((a - b).abs().max() / b.abs().max().clamp_min(1e-30))
+
+
+def _pair(C, heads, n, buckets, norm, seed, distance=16):
+    ref = PositionHead(C, heads, n, buckets=buckets, distance=distance, norm=norm)
+    sd = seeded_state_dict(ref, seed)
+    if buckets:
+        sd["relative_position_table"] = randn(seed + 1, buckets * buckets, heads)
+    if norm:
+        sd["residual_scale"] = 1 + 0.3 * randn(seed + 2, C)
+    mine = MultiHeadAttentionClassifier(C, heads, n, 0.0, relative_position_buckets=buckets, relative_position_distance=distance, residual_norm=norm)
+    assert set(mine.state_dict()) == set(sd)
+    ref.load_state_dict(sd)
+    mine.load_state_dict(sd)
+    return ref.double().train(), mine.cuda().train()
+
+
+@pytest.mark.parametrize("C,heads,hw,buckets,norm", [
+    (384, 8, (10, 10), 16, "rms"), (64, 8, (3, 5), 8, "layer"), (96, 3, (1, 9), 8, None), (64, 1, (5, 1), 0, "rms"), (64, 4, (19, 17), 8, "layer")])
+def test_head_and_clipped_step(C, heads, hw, buckets, norm):
+    """Forward, backward, gradients clipped to a norm, in one run; the last map has more tokens than the default path takes."""
+    ref, mine = _pair(C, heads, 4, buckets, norm, 51)
+    x = randn(52, 3, C, *hw)
+    xr, xm = x.double().requires_grad_(), x.permute(0, 2, 3, 1).contiguous().cuda().requires_grad_()
+    out_r, out_m = ref(xr), mine(xm)
+    assert rel(out_m, out_r) < 3e-4
+    g = randn(53, *out_r.shape)
+    out_r.backward(g.double())
+    out_m.backward(g.cuda())
+    assert rel(xm.grad.permute(0, 3, 1, 2), xr.grad) < 1e-3
+    want = dict(ref.named_parameters())
+    for k, p in mine.named_parameters():
+        if k == "key.bias" and not buckets:
+            assert p.grad.abs().max().item() < 1e-5
+        elif k != "key.bias":
+            assert rel(p.grad, want[k].grad) < 1e-3, k
+    # the key bias has no gradient (a softmax does not see it): both sides hold noise there
+    mine.key.bias.grad.zero_()
+    ref.key.bias.grad.zero_()
+    norm_r = torch.nn.utils.clip_grad_norm_(ref.parameters(), 0.5)
+    keep = [p.grad.clone() for p in mine.parameters()]
+    opt = AdamW(mine.parameters(), lr=1e-3, max_grad_norm=0.5)
+    other = copy.deepcopy(mine)
+    for p, grad in zip(other.parameters(), keep):
+        p.grad = grad.clone()
+    opt_other = AdamW(other.parameters(), lr=1e-3)
+    norm_m = clip_grad_norm_(list(other.parameters()), 0.5)
+    assert abs(float(norm_m) / float(norm_r) - 1) < 1e-3 and float(norm_r) > 0.5
+    for p, q in zip(other.parameters(), ref.parameters()):
+        assert rel(p.grad, q.grad) < 2e-3 or float(q.grad.abs().max()) == 0
+    opt.step()          # scales inside the update: the gradients stay, the parameters are those of a clipped step
+    opt_other.step()
+    assert all(torch.equal(p.grad, grad) for p, grad in zip(mine.parameters(), keep))
+    assert torch.equal(opt.grad_norm, norm_m)
+    for p, q in zip(mine.parameters(), other.parameters()):
+        assert rel(p, q) < 1e-6
+
+
+def test_zero_table_is_the_default_head():
+    """A head loaded from a checkpoint without a table starts as it was."""
+    torch.manual_seed(3)
+    plain = MultiHeadAttentionClassifier(384, 8, 4, 0.0).cuda().eval()
+    biased = MultiHeadAttentionClassifier(384, 8, 4, 0.0, relative_position_buckets=16).cuda().eval()
+    missing, unexpected = biased.load_state_dict(plain.state_dict(), strict=False)
+    assert missing == ["relative_position_table"] and not unexpected
+    x = torch.randn(4, 10, 10, 384, device="cuda")
+    with torch.no_grad():
+        assert rel(biased(x), plain(x)) < 1e-4
+        assert rel(biased(x.bfloat16()), plain(x)) < 3e-2
+
+
+def _model(dtype, dropout):
+    torch.manual_seed(0)
+    m = FoundationModel(pretrained=False, dropout=dropout, classification_heads={"d": 4}, compute_dtype=dtype, relative_position_buckets=16,
+                        residual_norm="rms").cuda().train()
+    for mod in m.modules():
+        if isinstance(mod, torch.nn.Dropout):
+            mod.p = dropout
+    return m
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_training_step_captured(dtype):
+    """Captured and replayed with eager steps of the same model in between, on three learning rates: bit for bit the eager run."""
+    eager = _model(dtype, 0.0)
+    graphed = copy.deepcopy(eager)
+    crit = CrossEntropyLoss()
+    opt_e = AdamW(eager.parameters(), lr=1e-3, max_grad_norm=1.0)
+    opt_g = AdamW(graphed.parameters(), lr=1e-3, max_grad_norm=1.0)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    xs = [torch.randn(4, 3, 96, 96, generator=g, device="cuda") for _ in range(4)]
+    ys = [torch.randint(0, 4, (4,), generator=g, device="cuda") for _ in range(4)]
+    step = GraphedTrainStep(graphed, "classification", "d", crit, opt_g, xs[0], ys[0])
+    for i, (x, y) in enumerate(zip(xs, ys)):
+        for opt in (opt_e, opt_g):
+            opt.param_groups[0]["lr"] = 1e-3 * (1 + i)
+        opt_e.zero_grad(set_to_none=True)
+        loss = crit(eager(x, "classification", "d"), y)
+        loss.backward()
+        opt_e.step()
+        assert torch.equal(step(x, y), loss.detach()), i
+        torch.cuda.synchronize()
+    for (k, p), q in zip(eager.named_parameters(), graphed.parameters()):
+        assert torch.equal(p, q), k
+    table = eager.classification_layers["d"].relative_position_table
+    assert bool(table.any()) and bool(torch.isfinite(table).all())
+
+
+def test_inference_captured():
+    m = _model("bf16", 0.2).eval()
+    with torch.no_grad():
+        m.classification_layers["d"].relative_position_table.normal_()
+    xs = [torch.randn(2, 3, 96, 96, device="cuda") for _ in range(3)]
+    g = GraphedForward(m, "classification", "d", xs[0])
+    with torch.no_grad():
+        for x in xs:
+            assert torch.equal(g(x), m(x, "classification", "d"))
+
+
+def test_dropout_in_the_head():
+    m = _model("fp32", 0.3)
+    x = torch.randn(2, 3, 96, 96, device="cuda")
+    outs = []
+    for seed in (1, 1, 2):
+        torch.manual_seed(seed)
+        outs.append(m(x, "classification", "d").detach())
+    assert torch.equal(outs[0], outs[1]) and not torch.equal(outs[0], outs[2])
