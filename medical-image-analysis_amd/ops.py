@@ -55,6 +55,12 @@ def _stream():
 _NO_SWITCH = contextlib.nullcontext()
 
 
+def first_derivative_only(name):
+    """Called by a backward pass of kernels: under create_graph=True its results would be taken for constants."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name} has no second derivative (create_graph=True)")
+
+
 def on_device(device):
     """Context in which `device` is the current one (so that _stream() is a stream of it); free when it already is."""
     current = _raw_device() if _raw_device is not None else torch.cuda.current_device()

@@ -3,11 +3,12 @@ number of tokens, masked keys, few queries against many keys, gradients of every
 import math
 from array import array
 
+import numpy as np
 import torch
 
 from . import ops
 from ._lib import lib
-from .ops import _DT, _p, _stream, on_device
+from .ops import _DT, _p, _stream, first_derivative_only, on_device
 
 
 class RelativePositionBuckets:
@@ -60,16 +61,17 @@ class RelativePositionBuckets:
         n = (2 * height - 1) * (2 * width - 1)
         if index.numel() != n:
             raise ValueError(f"a map of {height} x {width} has {n} offsets (got an index of {index.numel()})")
-        low, high = int(index.min()), int(index.max())
+        low, high = map(int, index.aminmax())
         num_buckets = high + 1 if num_buckets is None else int(num_buckets)
         if low < 0 or high >= num_buckets:
             raise ValueError(f"buckets {low}..{high} are not all in 0..{num_buckets - 1}")
         self.height, self.width, self.num_buckets = int(height), int(width), num_buckets
-        start = torch.zeros(num_buckets + 1, dtype=torch.int64)
-        start[1:] = torch.bincount(index, minlength=num_buckets).cumsum(0)
-        self.index = index.to(torch.int32).to(device)
-        self.order = index.argsort(stable=True).to(torch.int32).to(device)
-        self.start = start.to(torch.int32).to(device)
+        count = torch.bincount(index, minlength=num_buckets)
+        # 16-bit keys are sorted by radix: 0.2 ms for the 22201 offsets of a 75 x 75 map, 1.9 ms by torch's sort
+        keys = index.numpy()
+        order = torch.from_numpy((keys.astype(np.int16) if num_buckets <= 1 << 15 else keys).argsort(kind="stable"))
+        packed = torch.cat((index, order, count.cumsum(0) - count, torch.tensor([n]))).to(torch.int32).to(device)
+        self.index, self.order, self.start = packed[:n], packed[n:2 * n], packed[2 * n:]
 
     @property
     def device(self):
@@ -97,10 +99,11 @@ def _packed_rows(qkv):
 
 
 class RelPosAttentionFn(torch.autograd.Function):
-    """q, k, v or one packed tensor in the place of q (k and v None)."""
+    """q, k, v or one packed tensor in the place of q (k and v None). record: whether autograd records the call (forward itself
+    cannot see it); what the backward needs is written only then."""
 
     @staticmethod
-    def forward(ctx, q, k, v, table, plan, mask, scale, q_start, pdrop, seed):
+    def forward(ctx, q, k, v, table, plan, mask, scale, q_start, pdrop, seed, record):
         dev, dtype = q.device, q.dtype
         f32 = dict(dtype=torch.float32, device=dev)
         if k is None:
@@ -125,7 +128,7 @@ class RelPosAttentionFn(torch.autograd.Function):
             mask = mask.contiguous()
         strides = array("q", strides)
         bias = torch.empty((heads, plan.index.numel()), **f32)
-        grads = any(ctx.needs_input_grad)
+        grads = record and any(ctx.needs_input_grad)
         stat = torch.empty((B, heads, Lq, 2), **f32) if grads else None
         low = torch.empty_like(out) if grads and dtype == torch.bfloat16 else None
         C, dt = lib(), _DT[dtype]
@@ -142,11 +145,12 @@ class RelPosAttentionFn(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
+        first_derivative_only("relpos_attention")
         B, heads, Lq, Lk, D, plan, scale, q_start, pdrop, seed, soff = ctx.meta
         if ctx.empty:
             q, k, v, table = ctx.saved_tensors
             zeros = [torch.zeros_like(t) if t is not None else None for t in (q, k, v, table)]
-            return (*zeros, None, None, None, None, None, None)
+            return (*zeros, None, None, None, None, None, None, None)
         q, k, v, bias, mask, out, low, stat = ctx.saved_tensors
         dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
         if k is None:
@@ -171,7 +175,7 @@ class RelPosAttentionFn(torch.autograd.Function):
             C.mia_relpos_bwd(dt, *ptrs, ctx.strides.buffer_info()[0], _p(dout), _p(out), _p(low), _p(stat), B, heads, Lq, Lk, D, _p(bias),
                              plan.height, plan.width, q_start, _p(mask), scale, pdrop, seed, soff, _p(plan.order), _p(plan.start),
                              plan.num_buckets, _p(ws), nws, *gptrs, gst.buffer_info()[0], _p(dtable), _stream())
-        return dq, dk, dv, dtable, None, None, None, None, None, None
+        return dq, dk, dv, dtable, None, None, None, None, None, None, None
 
 
 def _attend(name, q, k, v, B, Lq, Lk, heads, D, table, buckets, key_mask, scale, q_start, dropout_p, seed):
@@ -201,7 +205,8 @@ def _attend(name, q, k, v, B, Lq, Lk, heads, D, table, buckets, key_mask, scale,
     if dropout_p > 0.0 and seed is None:
         from .head_ops import _seed
         seed = _seed()
-    return RelPosAttentionFn.apply(q, k, v, table, buckets, key_mask, scale, q_start, dropout_p, int(seed or 0))
+    return RelPosAttentionFn.apply(q, k, v, table, buckets, key_mask, scale, q_start, dropout_p, int(seed or 0),
+                                 torch.is_grad_enabled())
 
 
 def relpos_attention(q, k, v, table, buckets, key_mask=None, scale=None, q_start=0, dropout_p=0.0, seed=None):

@@ -149,3 +149,38 @@ def test_dropout_in_the_head():
         torch.manual_seed(seed)
         outs.append(m(x, "classification", "d").detach())
     assert torch.equal(outs[0], outs[1]) and not torch.equal(outs[0], outs[2])
+
+
+def test_second_derivatives_are_refused():
+    from mia_amd.block_norm import gated_residual_norm
+    from mia_amd.relpos import RelativePositionBuckets, relpos_self_attention
+    plan = RelativePositionBuckets(2, 3, 8, 16)
+    qkv = torch.randn(1, 6, 3, 2, 8, device="cuda", requires_grad=True)
+    out = relpos_self_attention(qkv, torch.zeros(64, 2, device="cuda"), plan)
+    with pytest.raises(RuntimeError, match="relpos_attention has no second derivative"):
+        torch.autograd.grad(out.sum(), qkv, create_graph=True)
+    x = torch.randn(3, 16, device="cuda", requires_grad=True)
+    _, z = gated_residual_norm(x, x.detach(), pre="rms", pre_weight=torch.ones(16, device="cuda"))
+    with pytest.raises(RuntimeError, match="gated_residual_norm has no second derivative"):
+        torch.autograd.grad(z.square().sum(), x, create_graph=True)
+
+
+def test_nothing_is_kept_without_gradients():
+    """Parameters that ask for gradients under no_grad: the same results and no more memory than the result itself."""
+    from mia_amd.block_norm import gated_residual_norm
+    from mia_amd.relpos import RelativePositionBuckets, relpos_self_attention
+    plan = RelativePositionBuckets(8, 8, 8, 16)
+    qkv = torch.randn(16, 64, 3, 4, 32, device="cuda").bfloat16().requires_grad_()
+    table, w = torch.randn(64, 4, device="cuda", requires_grad=True), torch.ones(128, device="cuda", requires_grad=True)
+    x = torch.randn(16, 64, 128, device="cuda").bfloat16().requires_grad_()
+
+    def run():
+        a = relpos_self_attention(qkv, table, plan)
+        return (a, *gated_residual_norm(x, a.view(16, 64, 128), pre="rms", pre_weight=w))
+    kept = run()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    with torch.no_grad():
+        plain = run()
+    assert torch.cuda.memory_allocated() - before == 3 * 16 * 64 * 128 * 2
+    assert all(torch.equal(a, b) for a, b in zip(kept, plain)) and not any(t.requires_grad for t in plain)
