@@ -1362,14 +1362,15 @@ static int rp_checks(const char* name, int dtype, int B, int heads, int Lq, int 
     MIA_CHECK_ARG(D % 8 == 0 && D <= 128, "%s: head width %d is not a multiple of 8 up to 128", name, D);
     MIA_CHECK_ARG(height > 0 && width > 0 && (height == 1 || width <= RP_MAX_WIDTH), "%s: bad map %d x %d (at most %d wide if of several rows)", name,
                   height, width, RP_MAX_WIDTH);
-    MIA_CHECK_ARG((2ll * height - 1) * (2ll * width - 1) <= (1ll << 28), "%s: a map of %d x %d has too many offsets", name, height, width);
+    MIA_CHECK_ARG((2ll * height - 1) * (2ll * width - 1) <= (1ll << 27), "%s: a map of %d x %d has too many offsets", name, height, width);
     const long long tokens = (long long)height * width;
     MIA_CHECK_ARG(height == 1 || tokens <= (1ll << 22), "%s: a map of %d x %d has too many tokens", name, height, width);
     MIA_CHECK_ARG(Lk <= tokens && q_start >= 0 && (long long)q_start + Lq <= tokens,
                   "%s: %d keys and %d queries from %d on do not fit a map of %lld tokens", name, Lk, Lq, q_start, tokens);
     MIA_CHECK_ARG(scale > 0.f && scale < 1e30f, "%s: scale must be positive (got %g)", name, (double)scale);
     MIA_CHECK_ARG(pdrop >= 0.f && pdrop < 1.f, "%s: dropout %g is not in [0, 1)", name, (double)pdrop);
-    MIA_CHECK_ARG((long long)B * heads * ((Lq + 63ll) / 64) <= 0x3fffffffll && (long long)B * heads * ((Lk + 63ll) / 64) <= 0x3fffffffll,
+    // 256 threads a block of 64 tokens, less than 2^32 of them in a launch
+    MIA_CHECK_ARG((long long)B * heads * ((Lq + 63ll) / 64) < (1ll << 24) - 8 && (long long)B * heads * ((Lk + 63ll) / 64) < (1ll << 24) - 8,
                   "%s: too many workgroups", name);
     return 0;
 }
@@ -1398,7 +1399,7 @@ static RpStride rp_stride(const long long* s) { return {s[0], s[1], s[2]}; }
 extern "C" int mia_relpos_bias(const float* table, const int* bucket, int height, int width, int heads, float scale, float* bias,
                                void* stream) {
     MIA_CHECK_ARG(table && bucket && bias, "mia_relpos_bias: null");
-    MIA_CHECK_ARG(height > 0 && width > 0 && heads > 0 && heads <= 65535 && (2ll * height - 1) * (2ll * width - 1) <= (1ll << 28) && scale > 0.f,
+    MIA_CHECK_ARG(height > 0 && width > 0 && heads > 0 && heads <= 65535 && (2ll * height - 1) * (2ll * width - 1) <= (1ll << 27) && scale > 0.f,
                   "mia_relpos_bias: bad arguments");
     const int n_off = (2 * height - 1) * (2 * width - 1);
     // after the division by scale and the later product with scale * log2(e) everything has to stay finite

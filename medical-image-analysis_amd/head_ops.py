@@ -219,13 +219,13 @@ def mha_head_forward(m, x):
     bqkv = torch.cat((m.query.bias, m.key.bias, m.value.bias), 0)
     qkv = LinearFn.apply(t, wqkv, bqkv, None, ACT_NONE)
     p_att = m.attention_dropout.p if training else 0.0
-    if m.relative_position_table is not None:
+    if getattr(m, "relative_position_table", None) is not None:      # (a head pickled whole before it had the options)
         a = relpos_self_attention(qkv.view(B, HW, 3, m.num_heads, C // m.num_heads), m.relative_position_table,
                                   m.position_plan(H, W, x2.device), dropout_p=p_att).view(B * HW, C)
     else:
         a = AttentionFn.apply(qkv, B, HW, C, m.num_heads, p_att, _seed() if p_att > 0 else 0)
     proj = m.output_projection
-    if m.residual_norm:
+    if getattr(m, "residual_norm", None):
         branch = LinearFn.apply(a, proj.weight, proj.bias, None, ACT_NONE)
         _, x3 = gated_residual_norm(t, branch, scale=m.residual_scale, pre=m.residual_norm, pre_weight=m.residual_norm_weight,
                                     pre_bias=m.residual_norm_bias)

@@ -54,8 +54,8 @@ class RelativePositionBuckets:
 
     @staticmethod
     def _check_map(height, width):
-        if height < 1 or width < 1 or (height > 1 and (width > 896 or height * width > 1 << 22)) or (2 * height - 1) * (2 * width - 1) > 1 << 28:
-            raise ValueError(f"a map of {height} x {width} is not supported (several rows: at most 896 wide and 2 ** 22 tokens; at most 2 ** 28 offsets)")
+        if height < 1 or width < 1 or (height > 1 and (width > 896 or height * width > 1 << 22)) or (2 * height - 1) * (2 * width - 1) > 1 << 27:
+            raise ValueError(f"a map of {height} x {width} is not supported (several rows: at most 896 wide and 2 ** 22 tokens; at most 2 ** 27 offsets)")
 
     def _set(self, height, width, index, num_buckets, device):
         n = (2 * height - 1) * (2 * width - 1)

@@ -10,13 +10,13 @@ from mia_amd.block_norm import gated_residual_norm
 P = ctypes.c_void_p(4096)
 
 
-def _fwd(dtype=0, x=P, f=P, images=2, rows=3, C=16, post=0, w1=None, b1=None, pre=1, w2=P, b2=None, eps=1e-6, y=P, z=P):
-    mia_amd.lib().mia_blocknorm_fwd(dtype, x, f, images, rows, C, None, None, post, w1, b1, pre, w2, b2, eps, y, z, None, None)
+def _fwd(dtype=0, x=P, f=P, images=2, rows=3, C=16, post=0, w1=None, b1=None, pre=1, w2=P, b2=None, eps=1e-6, y=P, z=P, gate=None):
+    mia_amd.lib().mia_blocknorm_fwd(dtype, x, f, images, rows, C, None, gate, post, w1, b1, pre, w2, b2, eps, y, z, None, None)
 
 
 @pytest.mark.parametrize("kw,match", [
     (dict(dtype=2), "bad dtype"), (dict(images=0), "bad shape"), (dict(rows=-1), "bad shape"), (dict(C=8193), "C <= 8192"),
-    (dict(rows=1 << 40), "too many"), (dict(post=3, w1=P), "bad norm kind"), (dict(eps=-1.0), "eps"), (dict(x=None), "null"), (dict(z=None), "null"),
+    (dict(rows=1 << 40), "too many"), (dict(images=1 << 22, rows=1, gate=P), "gates of"), (dict(post=3, w1=P), "bad norm kind"), (dict(eps=-1.0), "eps"), (dict(x=None), "null"), (dict(z=None), "null"),
     (dict(w2=None), "comes with its weight"), (dict(w1=P), "comes with its weight"), (dict(post=1), "comes with its weight"),
     (dict(b1=P), "only then with a bias"), (dict(pre=0, w2=None, b2=P), "only then with a bias")])
 def test_forward_entry_refuses(kw, match):

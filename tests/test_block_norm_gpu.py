@@ -126,6 +126,11 @@ def test_one_output_unused(use, dtype):
     _check((2, 9, 72), dtype, "layer", "rms", gate=True, use=use)
 
 
+def test_gates_of_many_images():
+    """More images than a grid has second or third dimensions."""
+    _check((70000, 1, 8), F32, "rms", "layer", gate=True)
+
+
 def test_views_of_any_layout():
     """Strided inputs and gradients, and rows that are not aligned to 16 bytes."""
     def odd(t):

@@ -80,7 +80,8 @@ def _fwd(dtype=0, q=P, strides=None, B=1, heads=2, Lq=5, Lk=9, D=16, bias=P, hei
 
 @pytest.mark.parametrize("kw,match", [
     (dict(dtype=5), "bad dtype"), (dict(B=0), "bad shape"), (dict(Lk=0), "bad shape"), (dict(D=12), "multiple of 8"), (dict(D=136), "multiple of 8"),
-    (dict(height=0), "bad map"), (dict(height=2, width=1030, Lk=9), "bad map"), (dict(height=1, width=1 << 29), "too many offsets"),
+    (dict(height=0), "bad map"), (dict(height=2, width=1030, Lk=9), "bad map"), (dict(height=1, width=1 << 29), "too many offsets"), (dict(height=1, width=(1 << 26) + 1), "too many offsets"),
+    (dict(B=1 << 20, heads=16, Lq=9), "too many workgroups"),
     (dict(Lk=10), "do not fit"), (dict(q_start=5), "do not fit"), (dict(q_start=-1), "do not fit"), (dict(scale=0.0), "scale"),
     (dict(scale=float("nan")), "scale"), (dict(pdrop=1.0), "dropout"), (dict(bias=None), "null"), (dict(q=ctypes.c_void_p(4104)), "16 bytes"),
     (dict(strides=[80, 32, 16, 80, 32, 16, 80, 33, 16]), "16 bytes"), (dict(dtype=1, strides=[80, 32, 16, 80, 32, 12, 80, 32, 16]), "16 bytes"),
