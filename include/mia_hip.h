@@ -223,9 +223,8 @@ int mia_attention_bwd(int dtype, const void* qkv, const float* P, const void* do
 /* ---- attention with a learned relative position bias (no counterpart in the reference, whose attention over the tokens of
  *      the feature map, model.py:153-163, knows no positions) -----------------------------------------------------------
  * s_ij = scale q_i.k_j + table[bucket(pos_j - pos_i)][head]; P = softmax over the keys that exist; out = P v. Tokens are
- * the positions of an height x width map in row order (a sequence: height 1; several rows: width <= 896 and at most 2^22 tokens; at most 2^27
- * offsets); key j is token j,
- * query i token q_start + i. Offset (dy, dx) has the number (dy + height-1)(2 width-1) + dx + width-1.
+ * the positions of an height x width map in row order (a sequence: height 1; several rows: width <= 896 and at most 2^22
+ * tokens; at most 2^27 offsets); key j is token j, query i token q_start + i. Offset (dy, dx) has the number (dy + height-1)(2 width-1) + dx + width-1.
  * bias[heads][(2 height-1)(2 width-1)] = table[bucket[offset]][head] / scale: made once per table, read by both calls below. */
 int mia_relpos_bias(const float* table, const int* bucket, int height, int width, int heads, float scale, float* bias,
                     void* stream);

@@ -1197,47 +1197,67 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
 // order[start[k]] .. order[start[k + 1] - 1]). Fixed order everywhere.
 // ------------------------------------------------------------------------------------------------
 // Slab rows are [image][head][key block][query range]; the offsets that a row covers depend on the last two alone. A workgroup: 64
-// offsets, 16 waves that share the rows; a row that covers none of the 64 costs two comparisons.
+// * PER offsets, 16 waves that share the rows where there are at least 16 of them (PER = 4: a row's four loads are in flight
+// together), else the images (PER = 1, four images in flight). A lane works out what one row covers, a ballot finds the rows
+// that reach the workgroup's offsets. 75x75 map, 4 heads, 704 rows: 11 us, 18 to 20 with PER = 1 (31 with every row tested by every
+// wave); 38x38, 8 heads, 23 rows, 4 images: 5.5 us, 7.7 with PER = 1.
+template <int PER>
 __global__ __launch_bounds__(1024) void relpos_offsets_kernel(RpArgs a, int ktiles, int kt, float* __restrict__ per_off) {
-    __shared__ float sm[16][64];
-    __shared__ int2 cover[1024];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, o0 = blockIdx.x * 64, o = o0 + lane, h = blockIdx.y;
+    __shared__ float sm[16][64 * PER];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), o0 = blockIdx.x * 64 * PER, h = blockIdx.y;
     const int rows = ktiles * a.splits, qtiles = (a.Lq + RP_TILE - 1) / RP_TILE;
-    const int wb = rows >= 16 ? 1 : 16, b0 = wb == 1 ? 0 : wave, r0 = wb == 1 ? wave : 0, rs = wb == 1 ? 16 : 1;   // waves over rows or images
     const size_t image = (size_t)a.heads * rows * a.slab_ld;
-    float v = 0.f;
-    for (int first = 0; first < rows; first += 1024) {
-        const int n = min(1024, rows - first);
-        __syncthreads();
-        if ((int)threadIdx.x < n) {
-            const int r = first + threadIdx.x, kb = r / a.splits, sp = r - kb * a.splits, k0 = kb * kt;
-            const int q0 = (int)((long long)qtiles * sp / a.splits) * RP_TILE, q1 = min((int)((long long)qtiles * (sp + 1) / a.splits) * RP_TILE, a.Lq) - 1;
-            cover[threadIdx.x] = make_int2(rp_c(a, k0) + a.off - rp_c(a, a.q_start + q1), rp_c(a, min(k0 + kt, a.Lk) - 1) + a.off - rp_c(a, a.q_start + q0));
-        }
-        __syncthreads();
-        for (int i = r0; i < n; i += rs) {
-            const int lo = __builtin_amdgcn_readfirstlane(cover[i].x), hi = __builtin_amdgcn_readfirstlane(cover[i].y);
-            if (hi < o0 || lo > o0 + 63) continue;
-            const bool in = o >= lo && o <= hi;
-            const float* p = a.slab + ((size_t)h * rows + first + i) * a.slab_ld + (in ? o - lo : 0);
-            int b = b0;
-            for (; b + 3 * wb < a.B; b += 4 * wb) {
-                float x[4];
+    float v[PER];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) x[u] = p[(b + u * wb) * image];
-                if (in) v += (x[0] + x[1]) + (x[2] + x[3]);
-            }
-            for (; b < a.B; b += wb) {
-                const float x = p[b * image];
-                if (in) v += x;
+    for (int u = 0; u < PER; ++u) v[u] = 0.f;
+    for (int first = 0; first < rows; first += 1024) {
+        const int r = first + (PER == 4 ? lane * 16 + wave : lane), kb = (int)((unsigned)r / (unsigned)a.splits), sp = r - kb * a.splits, k0 = kb * kt;
+        int lo = 0, hi = -1;
+        if (r < rows) {
+            const unsigned t0 = (unsigned)(qtiles * sp) / (unsigned)a.splits, t1 = (unsigned)(qtiles * (sp + 1)) / (unsigned)a.splits;   // at most 2^21 * 64
+            lo = rp_c(a, k0) + a.off - rp_c(a, a.q_start + min((int)t1 * RP_TILE, a.Lq) - 1);
+            hi = rp_c(a, min(k0 + kt, a.Lk) - 1) + a.off - rp_c(a, a.q_start + (int)t0 * RP_TILE);
+        }
+        unsigned long long reach = __ballot(r < rows && hi >= o0 && lo < o0 + 64 * PER);
+        for (; reach != 0ull; reach &= reach - 1) {
+            const int j = __builtin_ctzll(reach), from = __builtin_amdgcn_readlane(lo, j), to = __builtin_amdgcn_readlane(hi, j);
+            const float* p = a.slab + ((size_t)h * rows + first + (PER == 4 ? j * 16 + wave : j)) * a.slab_ld;
+            if constexpr (PER == 4) {
+                int at[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) at[u] = min(max(o0 + u * 64 + lane, from), to) - from;
+                for (int b = 0; b < a.B; ++b, p += image) {
+                    float x[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) x[u] = p[at[u]];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) v[u] += at[u] == o0 + u * 64 + lane - from ? x[u] : 0.f;
+                }
+            } else {
+                const int o = o0 + lane;
+                const bool in = o >= from && o <= to;
+                p += in ? o - from : 0;
+                int b = wave;
+                for (; b + 48 < a.B; b += 64) {
+                    float x[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) x[u] = p[(b + u * 16) * image];
+                    if (in) v[0] += (x[0] + x[1]) + (x[2] + x[3]);
+                }
+                for (; b < a.B; b += 16) {
+                    const float x = p[b * image];
+                    if (in) v[0] += x;
+                }
             }
         }
     }
-    sm[wave][lane] = v;
+#pragma unroll
+    for (int u = 0; u < PER; ++u) sm[wave][u * 64 + lane] = v[u];
     __syncthreads();
-    if (wave != 0 || o >= a.n_off) return;
-    for (int w = 1; w < 16; ++w) v += sm[w][lane];
-    per_off[(size_t)h * a.n_off + o] = v;
+    if ((int)threadIdx.x >= 64 * PER || o0 + (int)threadIdx.x >= a.n_off) return;
+    float total = sm[0][threadIdx.x];
+    for (int w = 1; w < 16; ++w) total += sm[w][threadIdx.x];
+    per_off[(size_t)h * a.n_off + o0 + threadIdx.x] = total;
 }
 
 __global__ __launch_bounds__(256) void relpos_buckets_kernel(const float* __restrict__ per_off, int n_off, int heads,
@@ -1273,34 +1293,38 @@ static int rp_ld(int dtype, int DP) {   // RpDim::LD
 static int rp_stage(int dtype, int DP) { return dtype == MIA_BF16 && DP <= 64 ? 2 * RP_TILE : RP_TILE; }   // RpDim::STAGE
 static size_t rp_es(int dtype) { return dtype == MIA_BF16 ? 2 : 4; }
 
-// How the kernels are laid out over a problem.
-// cols: 16-wide columns of a wave, so 64 * cols queries (keys) of a workgroup. Two serve more products with every operand read from
-// LDS; they are taken unless only the narrower workgroups fill the chip. fp32 keeps one: its operands are twice as large.
-// splits: ranges of the tokens a workgroup walks, joined afterwards. The grid runs in turns of as many workgroups as are resident
-// (two a CU with two columns, three with one), so s splits take ceil(workgroups * s / resident) turns of ceil(rounds / s)
-// rounds each, plus about a fiftieth of the walk per split for starting and joining it; ranges of at least four rounds. Measured: 64
-// workgroups over 16384 keys 52 + 6.6 us (kernel + join) at 7 splits, 48 + 7.1 at 8, 61 + 8.4 at 10; the forward on a 75x75
-// map, 4 heads of 32, 120 us unsplit, 84 + 5 at 2, 72 + 5.5 at 4 and 5, 76 + 7 at 6; on 38x38 maps, batch 4, 8 heads of 64,
-// where the workgroups fill the chip, 45 us unsplit and 45 + 9.7 at 3.
+// How the kernels are laid out over a problem: the pair with the lowest estimate of
+//   cols: 16-wide columns of a wave, so 64 * cols queries (keys) of a workgroup. Two serve more products with every operand read from
+//     LDS, but a round of them is 1.85 times as long (about twice with short heads, whose two-column kernels have half as many
+//     waves a SIMD). fp32 and wide heads keep one: their operands do not fit.
+//   splits: ranges of the tokens a workgroup walks, of at least four rounds, joined afterwards.
+// The kernels are bound by issue, so what counts is the busiest of the 256 CUs: ceil(workgroups * splits / 256) of them, for
+// ceil(rounds / splits) rounds each; a workgroup alone on its CU takes 1.25 times its share, and joining about 3 rounds plus what the
+// partial results weigh. Measured (us, kernel + join), with the choice first: forward on a 75x75 map, 4 heads of 32: one column, 5
+// splits 73 + 6, 2 splits 82 + 5, 3 splits 85 + 5; two columns, 4 splits 85 + 6. 4096 tokens, 4 heads of 64: two columns, 4 splits
+// 54 + 7, 3 splits 66 + 6, 5 splits 65 + 7; one column, 3 splits 57 + 6. 38x38, batch 4, 8 heads of 64: one column unsplit 50, 3
+// splits 50 + 11; two columns unsplit 58. 10x10, batch 128, 8 heads of 48: two columns 27, one 30. One query, 64 workgroups over
+// 16384 keys: 8 splits 48 + 7, 7 splits 52 + 7, 10 splits 61 + 8.
 struct RpPlan {
     int cols, splits;
 };
 static RpPlan rp_plan(int what, int dtype, int B, int heads, int Lq, int Lk, int D) {
     const int DP = rp_dp(D), owned = what == RP_BWD_KV ? Lk : Lq, walked = what == RP_BWD_KV ? Lq : Lk;
     const int round = what == RP_BWD_KV ? RP_TILE : rp_stage(dtype, DP);
-    const long long bh = (long long)B * heads;
-    RpPlan p;
-    const long long one = bh * ((owned + 63) / 64), two = bh * ((owned + 127) / 128), rounds = (walked + round - 1) / round;
-    p.cols = dtype == MIA_F32 || DP > (what == RP_FWD ? 96 : 64) || owned <= 64 || (two < 512 && one >= 512) ? 1 : 2;
-    const long long wgs = p.cols == 1 ? one : two;
-    const long long resident = 256 * (p.cols == 1 ? 3 : 2), most = rounds / 4 < 64 ? rounds / 4 : 64;
-    long long s = 1;
-    double best = 1e30;
-    for (long long i = 1; i <= most && (i == 1 || wgs < 2 * resident); ++i) {
-        const double t = (double)((wgs * i + resident - 1) / resident * ((rounds + i - 1) / i)) + 0.02 * rounds * i;
-        if (t < best - 0.1 * rounds * (s == 1)) best = t, s = i;
+    const long long rounds = (walked + round - 1) / round, most = rounds / 4 < 1 ? 1 : rounds / 4 < 64 ? rounds / 4 : 64;
+    const int max_cols = dtype == MIA_F32 || DP > (what == RP_FWD ? 96 : 64) || owned <= 64 ? 1 : 2;
+    RpPlan p = {1, 1};
+    double best = 1e300;
+    for (int cols = 1; cols <= max_cols; ++cols) {
+        const long long wgs = (long long)B * heads * ((owned + 64 * cols - 1) / (64 * cols));
+        const double length = cols == 1 ? 1.0 : DP > 32 ? 1.85 : what == RP_FWD ? 2.1 : 1.95;
+        for (long long s = 1; s <= most; ++s) {
+            const long long busiest = (wgs * s + 255) / 256, walk = (rounds + s - 1) / s;
+            double t = length * walk * (busiest == 1 ? 1.25 : (double)busiest);
+            if (s > 1) t += 3.0 + 0.6 * s * wgs * cols / 256;
+            if (t < best) best = t, p.cols = cols, p.splits = (int)s;
+        }
     }
-    p.splits = (int)s;
     return p;
 }
 
@@ -1554,7 +1578,8 @@ extern "C" int mia_relpos_bwd(int dtype, const void* q, const void* k, const voi
     if (kp.splits > 1)
         if (int rc = rp_join<RP_BWD_KV>("mia_relpos_bwd", dtype, a, s)) return rc;
     if (!dtable) return 0;
-    MIA_LAUNCH(relpos_offsets_kernel, dim3(cdiv(a.n_off, 64), heads), dim3(1024), 0, s, a, ktiles, kt, per_off);
+    if (ktiles * a.splits >= 16) MIA_LAUNCH((relpos_offsets_kernel<4>), dim3(cdiv(a.n_off, 256), heads), dim3(1024), 0, s, a, ktiles, kt, per_off);
+    else MIA_LAUNCH((relpos_offsets_kernel<1>), dim3(cdiv(a.n_off, 64), heads), dim3(1024), 0, s, a, ktiles, kt, per_off);
     MIA_CHECK_LAUNCH("mia_relpos_bwd");
     MIA_LAUNCH(relpos_buckets_kernel, dim3(buckets, heads), dim3(256), 0, s, per_off, a.n_off, heads, order, start, dtable);
     MIA_CHECK_LAUNCH("mia_relpos_bwd");
