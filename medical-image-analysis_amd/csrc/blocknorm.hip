@@ -17,9 +17,10 @@
 // A row lives in the registers of one wave (up to 64 * V * 2 channels) or one workgroup, V = channels of a 16-byte access, so
 // every tensor is read once and written once: two in, two out forward; four in, two out backward. The statistics of both
 // norms are kept (16 bytes a row). The next row is requested while one is worked on: a wave has one or two rows in flight instead of
-// waiting out every load (32 images of 1444 rows of 1024 bf16 channels, two RMS norms: forward 91 -> 73 us, 5.2 TB/s; backward
-// 164 -> 131 us, 4.3 TB/s). Long batches of rows are bound by HBM, short ones (a head's 100 tokens) by latency. The backward keeps its column sums in registers over all
-// rows of a workgroup and leaves one slab row; two small kernels add the slab up in a fixed order (no atomics).
+// waiting out every load (32 images of 1444 rows of 1024 bf16 channels, two RMS norms: forward 91 -> 73 us, backward 164 -> 131;
+// now 65, 5.8 TB/s, and 132, 4.3 TB/s). Long batches of rows are bound by HBM, short ones (a head's 100 tokens) by latency.
+// The backward keeps its column sums in registers over all rows of a workgroup and leaves one slab row; two small kernels add
+// the slab up in a fixed order (no atomics).
 #include "common.h"
 
 enum { BNORM_NONE = 0, BNORM_RMS = 1, BNORM_LAYER = 2 };
@@ -489,10 +490,13 @@ static void bn_dispatch(bool fwd, bool vec, const BNormArgs& a, hipStream_t s) {
     }
 }
 
-// Workgroups an image's rows are split over: enough to fill the chip (about 1024 wave-per-row or 512 row-per-workgroup
-// workgroups in all), at least four rows a row lane.
-static int bn_splits(long long images, long long rows, int C) {
-    const long long want = C <= 1024 ? 1024 : 512, per = C <= 512 ? 16 : 4;
+// Workgroups an image's rows are split over: as many in all as are resident at once, so that the rows come out even, and at least four
+// rows a row lane. Backward two a CU (32 images of 1444 rows of 1024 bf16 channels: 134 us, 142 with 1024 workgroups, 132 with
+// 256; 200000 rows of 384: 236, 244 and 354). Forward four a CU with eight channels a lane (200000 rows of 384 bf16 channels: 120
+// us, 143 with 512), three with sixteen (rows of 1024: 65 us, 70 with 1024, 67 with 512), two with a workgroup a row (8000 rows
+// of 2048: 28 us, 45 with 256).
+static int bn_splits(bool fwd, int dtype, long long images, long long rows, int C) {
+    const long long want = !fwd || C > 1024 ? 512 : dtype == MIA_BF16 && C > 512 ? 768 : 1024, per = C <= 512 ? 16 : 4;
     long long s = (want + images - 1) / images;
     if (s > rows / per) s = rows / per;
     return s < 1 ? 1 : (int)s;
@@ -501,7 +505,7 @@ static int bn_splits(long long images, long long rows, int C) {
 static int bn_groups(int gated, int N, int S) { return gated ? N : (N * S + 15) / 16; }
 
 extern "C" long long mia_blocknorm_ws_floats(int images, long long rows_per_image, int C, int gated) {
-    const int S = bn_splits(gated ? images : 1, gated ? rows_per_image : rows_per_image * images, C), N = gated ? images : 1;
+    const int S = bn_splits(false, MIA_F32, gated ? images : 1, gated ? rows_per_image : rows_per_image * images, C), N = gated ? images : 1;
     return ((long long)N * S + bn_groups(gated, N, S)) * 4 * C;
 }
 
@@ -516,10 +520,10 @@ static int bn_checks(const char* name, int dtype, int images, long long rows, in
     return 0;
 }
 
-static void bn_shape(BNormArgs& a, int images, long long rows, int C, int post, int pre, float eps) {
+static void bn_shape(BNormArgs& a, bool fwd, int dtype, int images, long long rows, int C, int post, int pre, float eps) {
     a.N = a.gate ? images : 1;
     a.T = a.gate ? rows : rows * images;
-    a.S = bn_splits(a.N, a.T, C);
+    a.S = bn_splits(fwd, dtype, a.N, a.T, C);
     a.C = C; a.post = post; a.pre = pre; a.eps = eps; a.inv_c = 1.0f / (float)C;
 }
 
@@ -534,7 +538,7 @@ extern "C" int mia_blocknorm_fwd(int dtype, const void* x, const void* f, int im
     BNormArgs a = {};
     a.x = x; a.f = f; a.y = y; a.z = z; a.stats = stats;
     a.scale = scale; a.gate = gate; a.w1 = post_w; a.b1 = post_b; a.w2 = pre_w; a.b2 = pre_b;
-    bn_shape(a, images, rows_per_image, C, post, pre, eps);
+    bn_shape(a, true, dtype, images, rows_per_image, C, post, pre, eps);
     const void* ptrs[] = {x, f, y, pre ? z : y, scale, gate, post_w, post_b, pre_w, pre_b};
     const bool vec = bn_vec(dtype, C, ptrs, 10);
     if (dtype == MIA_BF16) bn_dispatch<bf16_t>(true, vec, a, reinterpret_cast<hipStream_t>(stream));
@@ -559,7 +563,7 @@ extern "C" int mia_blocknorm_bwd(int dtype, const void* dy, const void* dz, cons
     BNormArgs a = {};
     a.dy = dy; a.dz = dz; a.x = x; a.f = f; a.dx = dx; a.df = df; a.stats = const_cast<float*>(stats); a.slab = ws;
     a.scale = scale; a.gate = gate; a.w1 = post_w; a.b1 = post_b; a.w2 = pre_w;
-    bn_shape(a, images, rows_per_image, C, post, pre, 0.f);
+    bn_shape(a, false, dtype, images, rows_per_image, C, post, pre, 0.f);
     const void* ptrs[] = {x, f, dx, df, dy, dz, scale, gate, post_w, post_b, pre_w};
     const bool vec = bn_vec(dtype, C, ptrs, 11);
     if (dtype == MIA_BF16) bn_dispatch<bf16_t>(false, vec, a, s);
