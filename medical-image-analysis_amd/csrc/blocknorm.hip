@@ -490,13 +490,15 @@ static void bn_dispatch(bool fwd, bool vec, const BNormArgs& a, hipStream_t s) {
     }
 }
 
-// Workgroups an image's rows are split over: as many in all as are resident at once, so that the rows come out even, and at least four
-// rows a row lane. Backward two a CU (32 images of 1444 rows of 1024 bf16 channels: 134 us, 142 with 1024 workgroups, 132 with
-// 256; 200000 rows of 384: 236, 244 and 354). Forward four a CU with eight channels a lane (200000 rows of 384 bf16 channels: 120
-// us, 143 with 512), three with sixteen (rows of 1024: 65 us, 70 with 1024, 67 with 512), two with a workgroup a row (8000 rows
-// of 2048: 28 us, 45 with 256).
+// Workgroups an image's rows are split over: as many in all as are resident at once, so that the rows come out even, with at
+// least one row a wave forward and two backward, two where a workgroup has a row (100 rows of 384 bf16 channels: forward 3.6 us,
+// 7.2 with four rows a wave; backward 6.7 and 8.7).
+// Backward two a CU (32 images of 1444 rows of 1024 bf16 channels: 134 us, 142 with 1024 workgroups, 132 with 256; 200000 rows
+// of 384: 236, 244 and 354). Forward four a CU with eight channels a lane (200000 rows of 384 bf16 channels: 120 us, 143 with
+// 512), three with sixteen (rows of 1024: 65 us, 70 with 1024, 67 with 512), two with a workgroup a row (8000 rows of 2048: 28
+// us, 45 with 256).
 static int bn_splits(bool fwd, int dtype, long long images, long long rows, int C) {
-    const long long want = !fwd || C > 1024 ? 512 : dtype == MIA_BF16 && C > 512 ? 768 : 1024, per = C <= 512 ? 16 : 4;
+    const long long want = !fwd || C > 1024 ? 512 : dtype == MIA_BF16 && C > 512 ? 768 : 1024, per = C > 512 ? 2 : fwd ? 4 : 8;
     long long s = (want + images - 1) / images;
     if (s > rows / per) s = rows / per;
     return s < 1 ? 1 : (int)s;

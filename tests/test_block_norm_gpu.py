@@ -77,7 +77,7 @@ def _check(shape, dtype, post, pre, scale=True, gate=False, bias=True, use=("y",
     _close(y.detach(), y64.detach(), eps32 * y64.abs().max(), "y")
     if pre:
         # z divides by the row's deviation, which small rows can make large
-        _close(z.detach(), z64.detach(), eps32 * max(1.0, float(z64.abs().max())), "z")
+        _close(z.detach(), z64.detach(), eps32 * max(1.0, float(z64.detach().abs().max())), "z")
     outs, gs = [], []
     if "y" in use:
         outs.append(y), gs.append(make(dy.cuda()))
