@@ -89,6 +89,26 @@ class _Lib:
         self.fastcall = True
 
 
+_nodes = None
+
+
+def nodes():
+    """The autograd nodes in C++ (csrc/autograd.cpp, built by build.py): relpos.py and block_norm.py call them."""
+    global _nodes
+    if _nodes is None:
+        lib()       # the library first, and torch's HIP runtime before it
+        build = f"build it with `python {os.path.join(HERE, 'build.py')}` (there is no fallback path)"
+        try:
+            from . import _mia_autograd
+        except ImportError as e:
+            raise ImportError(f"_mia_autograd is missing or does not load ({e}): {build}") from e
+        if _mia_autograd.digest() != _proto.autograd_digest():
+            raise ImportError(f"_mia_autograd was built against another header or another torch: {build}")
+        _mia_autograd.bind(MiaError)
+        _nodes = _mia_autograd
+    return _nodes
+
+
 _lib = None
 
 

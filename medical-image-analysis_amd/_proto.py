@@ -42,3 +42,9 @@ def header_digest(path=HEADER) -> str:
     for name in sorted(protos):
         h.update(f"{name}:{protos[name][0]}:{','.join(protos[name][1])};".encode())
     return h.hexdigest()[:16]
+
+
+def autograd_digest() -> str:
+    """What the C++ autograd nodes are compiled against: the prototypes and torch's own classes."""
+    import torch
+    return f"{header_digest()}-{torch.__version__}"

@@ -195,7 +195,40 @@ def build_fast(force: bool = False, verbose: bool = True) -> str:
     return target
 
 
+# ------------------------------------------------------------------------------------------------
+# Autograd nodes in C++ (csrc/autograd.cpp): host code against torch's headers, linked to the library next to it.
+# ------------------------------------------------------------------------------------------------
+def autograd_module_path() -> str:
+    import sysconfig
+    return os.path.join(HERE, "_mia_autograd" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
+
+
+def build_autograd(force: bool = False, verbose: bool = True) -> str:
+    import importlib.util
+    import sysconfig
+    target, src = autograd_module_path(), os.path.join(CSRC, "autograd.cpp")
+    deps = [src, os.path.join(HERE, "..", "include", "mia_hip.h"), os.path.join(HERE, "_proto.py"), os.path.abspath(__file__)]
+    if not force and os.path.exists(target) and all(os.path.getmtime(d) <= os.path.getmtime(target) for d in deps):
+        return target
+    spec = importlib.util.spec_from_file_location("mia_proto", os.path.join(HERE, "_proto.py"))
+    proto = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(proto)
+    import torch
+    home = os.path.dirname(torch.__file__)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-fPIC", "-shared", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", f'-DMIA_HEADER_DIGEST="{proto.autograd_digest()}"',
+           "-isystem", os.path.join(home, "include"), "-isystem", os.path.join(home, "include", "torch", "csrc", "api", "include"),
+           "-isystem", os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"), "-isystem", sysconfig.get_paths()["include"],
+           src, "-o", target, "-L" + os.path.join(home, "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_python",
+           "-L" + HERE, "-lmia_hip", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
+    return target
+
+
 if __name__ == "__main__":
     build(force="--force" in sys.argv)
     build_fast(force="--force" in sys.argv)
+    build_autograd(force="--force" in sys.argv)
     print(LIB)

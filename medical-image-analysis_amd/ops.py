@@ -2,7 +2,6 @@
 Functions built from them. Tensors are torch CUDA tensors used purely as device memory; every
 arithmetic step is a kernel of libmia_hip.so launched on torch's current HIP stream.
 """
-import contextlib
 import ctypes
 import math
 from typing import Optional
@@ -50,21 +49,6 @@ def _stream():
     if _raw_stream is not None and _raw_device is not None:
         return _raw_stream(_raw_device())
     return torch.cuda.current_stream().cuda_stream
-
-
-_NO_SWITCH = contextlib.nullcontext()
-
-
-def first_derivative_only(name):
-    """Called by a backward pass of kernels: under create_graph=True its results would be taken for constants."""
-    if torch.is_grad_enabled():
-        raise RuntimeError(f"{name} has no second derivative (create_graph=True)")
-
-
-def on_device(device):
-    """Context in which `device` is the current one (so that _stream() is a stream of it); free when it already is."""
-    current = _raw_device() if _raw_device is not None else torch.cuda.current_device()
-    return _NO_SWITCH if device.index == current else torch.cuda.device(device)
 
 
 class Replay:

@@ -5,52 +5,16 @@ which the reference builds at train.py:193-197 and finetune.py:232-248, so LR sc
 (ReduceLROnPlateau, train.py:199-201) and optimizer checkpoints (train.py:440) keep working."""
 import ctypes
 import math
-from array import array
 
 import torch
 
-from ._lib import lib
-from .ops import _DT, Side, WeightEpoch, _p, _stream, on_device
-
-
-_data_ptr, _numel, _is_contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
-
-
-def _grad_table(grads):
-    """Host tables of a list of gradients for mia_grad_norm / mia_grad_clip -> (count, addresses, dtypes, sizes, device);
-    the arrays have to outlive the call that reads them. dtypes is None when all are fp32."""
-    # one C call sorts the list by device and type; attribute by attribute a list of 430 gradients costs twice the whole clipping
-    groups = list(torch._C._group_tensors_by_device_and_dtype([grads], False))
-    if len({device for device, _ in groups}) != 1 or not grads[0].is_cuda:
-        raise RuntimeError("gradient norm and clipping need their tensors on one MI355X device; there is no CPU path")
-    kinds = {dtype for _, dtype in groups}
-    if not kinds <= _DT.keys():
-        raise TypeError(f"gradients are fp32 or bf16 (got {', '.join(sorted(str(k) for k in kinds))})")
-    dtypes = None if kinds == {torch.float32} else array("i", [_DT[g.dtype] for g in grads])
-    return len(grads), array("Q", map(_data_ptr, grads)), dtypes, array("q", map(_numel, grads)), grads[0].device
+from ._lib import lib, nodes
+from .ops import Side, WeightEpoch, _p, _stream
 
 
 def _dense(g):
     """Whether the elements fill one run of memory in some order: a norm and a scaling need no more than that."""
-    if g.layout != torch.strided:
-        raise TypeError("gradients are dense tensors")
-    if g.is_contiguous():
-        return True
-    run = 1
-    for stride, size in sorted((st, n) for st, n in zip(g.stride(), g.shape) if n != 1):
-        if stride != run:
-            return False
-        run *= size
-    return True
-
-
-def _addr(a):
-    return a.buffer_info()[0] if a is not None else None
-
-
-def _norm_ws(n, sizes, device):
-    nws = lib().mia_grad_norm_ws_doubles(n, _addr(sizes))
-    return torch.empty((nws,), dtype=torch.float64, device=device), nws
+    return nodes().all_dense([g])
 
 
 def _check_max_norm(max_norm):
@@ -60,44 +24,21 @@ def _check_max_norm(max_norm):
     return max_norm
 
 
-@torch.no_grad()
 def grad_norm(grads):
     """Norm of all elements of the tensors together (fp32 or bf16, any mix, dense), as a 0-d fp32 device tensor: one pass,
     squares summed in double in a fixed order, nothing read back to the host."""
     grads = list(grads)
-    if not all(map(_is_contiguous, grads)):
-        grads = [g if _dense(g) else g.contiguous() for g in grads]
-    if not grads:
-        return torch.zeros(())
-    n, ptrs, dtypes, sizes, device = _grad_table(grads)
-    with on_device(device):
-        ws, nws = _norm_ws(n, sizes, device)
-        out = torch.empty((2,), dtype=torch.float32, device=device)
-        lib().mia_grad_norm(n, _addr(ptrs), _addr(dtypes), _addr(sizes), 1.0, 0.0, _p(ws), nws, _p(out), _stream())
-    return out[0]
+    return nodes().grad_norm(grads) if grads else torch.zeros(())
 
 
-@torch.no_grad()
 def clip_grads_(grads, max_norm):
     """Scales the tensors in place so that their global norm is at most max_norm and returns the norm they had (0-d fp32
     device tensor): g *= min(1, max_norm / (norm + 1e-6)), as torch.nn.utils.clip_grad_norm_ does. No host
-    synchronisation; the tensors must not overlap; may be captured into a HIP graph. A norm that is infinite or NaN makes the gradients zero, NaN or
-    both, as there: look at the returned norm where that can happen."""
+    synchronisation; the tensors must not overlap; may be captured into a HIP graph. A norm that is infinite or NaN makes the
+    gradients zero, NaN or both, as there: look at the returned norm where that can happen."""
     max_norm = _check_max_norm(max_norm)
     grads = list(grads)
-    if not grads:
-        return torch.zeros(())
-    for g in (() if all(map(_is_contiguous, grads)) else grads):
-        if not _dense(g):
-            raise ValueError(f"clip_grads_ scales in place and needs dense tensors (got strides {g.stride()} for {tuple(g.shape)})")
-    n, ptrs, dtypes, sizes, device = _grad_table(grads)
-    if len(set(ptrs)) != n and len({a for a, k in zip(ptrs, sizes) if k}) != sum(1 for k in sizes if k):
-        raise ValueError("a tensor is listed twice: it would be scaled twice")
-    with on_device(device):
-        ws, nws = _norm_ws(n, sizes, device)
-        out = torch.empty((2,), dtype=torch.float32, device=device)
-        lib().mia_grad_clip(n, _addr(ptrs), _addr(dtypes), _addr(sizes), max_norm, _p(ws), nws, _p(out), _stream())
-    return out[0]
+    return nodes().grad_clip(grads, max_norm) if grads else torch.zeros(())
 
 
 @torch.no_grad()
@@ -109,9 +50,10 @@ def clip_grad_norm_(parameters, max_norm):
         parameters = [parameters]
     Side.sync()
     params = [p for p in parameters if p.grad is not None]
-    for p in params:
-        if not _dense(p.grad):
-            p.grad = p.grad.contiguous()
+    if not nodes().all_dense([p.grad for p in params]):
+        for p in params:
+            if not _dense(p.grad):
+                p.grad = p.grad.contiguous()
     return clip_grads_([p.grad for p in params], max_norm)
 
 

@@ -1,14 +1,13 @@
 """Multi-head attention with a learned relative position bias, on the gfx950 kernels of csrc/relpos.hip: no limit on the
 number of tokens, masked keys, few queries against many keys, gradients of everything including the bias table."""
 import math
-from array import array
 
 import numpy as np
 import torch
 
 from . import ops
-from ._lib import lib
-from .ops import _DT, _p, _stream, first_derivative_only, on_device
+from ._lib import nodes
+from .ops import _DT
 
 
 class RelativePositionBuckets:
@@ -78,106 +77,6 @@ class RelativePositionBuckets:
         return self.index.device
 
 
-def _rows(t):
-    """The tensor itself when the kernels can read it where it lies (head elements contiguous, rows at multiples of 16
-    bytes), else a contiguous copy; and its (batch, token, head) strides in elements."""
-    per = 16 // t.element_size()
-    st = [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride())]
-    if (t.stride(3) != 1 and t.shape[3] != 1) or any(s % per or s < 0 for s in st) or st[1] >= 1 << 24 or t.data_ptr() % 16:
-        t = t.contiguous()
-        if t.data_ptr() % 16:       # a contiguous view that starts in between
-            t = t.clone()
-        st = [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride())]
-    return t, st
-
-
-def _packed_rows(qkv):
-    """Addresses of q, k and v inside a packed [B, L, 3, heads, D] tensor and their common (batch, token, head) strides."""
-    sb, st, s3, sh, _ = qkv.stride()
-    at, step = qkv.data_ptr(), s3 * qkv.element_size()
-    return (at, at + step, at + 2 * step), (sb, st, sh) * 3
-
-
-class RelPosAttentionFn(torch.autograd.Function):
-    """q, k, v or one packed tensor in the place of q (k and v None). record: whether autograd records the call (forward itself
-    cannot see it); what the backward needs is written only then."""
-
-    @staticmethod
-    def forward(ctx, q, k, v, table, plan, mask, scale, q_start, pdrop, seed, record):
-        dev, dtype = q.device, q.dtype
-        f32 = dict(dtype=torch.float32, device=dev)
-        if k is None:
-            B, Lq, _, heads, D = q.shape
-            Lk = Lq
-            if not q.is_contiguous() or q.data_ptr() % 16:
-                q = q.clone(memory_format=torch.contiguous_format)
-            ptrs, strides = _packed_rows(q)
-        else:
-            B, Lq, heads, D = q.shape
-            Lk = k.shape[1]
-            (q, sq), (k, sk), (v, sv) = _rows(q), _rows(k), _rows(v)
-            ptrs, strides = (_p(q), _p(k), _p(v)), sq + sk + sv
-        ctx.meta = (B, heads, Lq, Lk, D, plan, scale, q_start, pdrop, seed, ops.seed_offset())
-        ctx.empty = 0 in (B, Lq, Lk, heads)
-        if ctx.empty:
-            ctx.save_for_backward(q, k, v, table)
-            return torch.zeros((B, Lq, heads, D), dtype=dtype, device=dev)
-        out = torch.empty((B, Lq, heads, D), dtype=dtype, device=dev)
-        table = table.contiguous()
-        if mask is not None:
-            mask = mask.contiguous()
-        strides = array("q", strides)
-        bias = torch.empty((heads, plan.index.numel()), **f32)
-        grads = record and any(ctx.needs_input_grad)
-        stat = torch.empty((B, heads, Lq, 2), **f32) if grads else None
-        low = torch.empty_like(out) if grads and dtype == torch.bfloat16 else None
-        C, dt = lib(), _DT[dtype]
-        nws = C.mia_relpos_fwd_ws_floats(dt, B, heads, Lq, Lk, D)
-        ws = torch.empty((nws,), **f32) if nws else None
-        with on_device(dev):
-            stream = _stream()
-            C.mia_relpos_bias(_p(table), _p(plan.index), plan.height, plan.width, heads, scale, _p(bias), stream)
-            C.mia_relpos_fwd(dt, *ptrs, strides.buffer_info()[0], B, heads, Lq, Lk, D, _p(bias), plan.height, plan.width, q_start,
-                             _p(mask), scale, pdrop, seed, ops.seed_offset(), _p(ws), nws, _p(out), _p(low), _p(stat), stream)
-        ctx.strides = strides
-        ctx.save_for_backward(q, k, v, bias, mask, out, low, stat)
-        return out
-
-    @staticmethod
-    def backward(ctx, dout):
-        first_derivative_only("relpos_attention")
-        B, heads, Lq, Lk, D, plan, scale, q_start, pdrop, seed, soff = ctx.meta
-        if ctx.empty:
-            q, k, v, table = ctx.saved_tensors
-            zeros = [torch.zeros_like(t) if t is not None else None for t in (q, k, v, table)]
-            return (*zeros, None, None, None, None, None, None, None)
-        q, k, v, bias, mask, out, low, stat = ctx.saved_tensors
-        dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if k is None:
-            dk = dv = None
-            ptrs = _packed_rows(q)[0]
-            gptrs, gst = _packed_rows(dq)
-        else:
-            dk, dv = torch.empty(k.shape, dtype=k.dtype, device=k.device), torch.empty(v.shape, dtype=v.dtype, device=v.device)
-            ptrs, gptrs = (_p(q), _p(k), _p(v)), (_p(dq), _p(dk), _p(dv))
-            gst = (*dq.stride()[:3], *dk.stride()[:3], *dv.stride()[:3])
-        dout = dout.contiguous()
-        if dout.data_ptr() % 16:
-            dout = dout.clone()
-        want = ctx.needs_input_grad[3]
-        f32 = dict(dtype=torch.float32, device=q.device)
-        dtable = torch.empty((plan.num_buckets, heads), **f32) if want else None
-        C, dt = lib(), _DT[q.dtype]
-        nws = C.mia_relpos_bwd_ws_floats(dt, B, heads, Lq, Lk, D, plan.height, plan.width, 1 if want else 0)
-        ws = torch.empty((nws,), **f32)
-        gst = array("q", gst)
-        with on_device(q.device):
-            C.mia_relpos_bwd(dt, *ptrs, ctx.strides.buffer_info()[0], _p(dout), _p(out), _p(low), _p(stat), B, heads, Lq, Lk, D, _p(bias),
-                             plan.height, plan.width, q_start, _p(mask), scale, pdrop, seed, soff, _p(plan.order), _p(plan.start),
-                             plan.num_buckets, _p(ws), nws, *gptrs, gst.buffer_info()[0], _p(dtable), _stream())
-        return dq, dk, dv, dtable, None, None, None, None, None, None, None
-
-
 def _attend(name, q, k, v, B, Lq, Lk, heads, D, table, buckets, key_mask, scale, q_start, dropout_p, seed):
     dtype = q.dtype
     if dtype not in _DT or (k is not None and (k.dtype != dtype or v.dtype != dtype)):
@@ -205,8 +104,8 @@ def _attend(name, q, k, v, B, Lq, Lk, heads, D, table, buckets, key_mask, scale,
     if dropout_p > 0.0 and seed is None:
         from .head_ops import _seed
         seed = _seed()
-    return RelPosAttentionFn.apply(q, k, v, table, buckets, key_mask, scale, q_start, dropout_p, int(seed or 0),
-                                 torch.is_grad_enabled())
+    return nodes().relpos(q, k, v, table, buckets.index, buckets.order, buckets.start, key_mask, buckets.height, buckets.width, buckets.num_buckets,
+                          scale, q_start, dropout_p, int(seed or 0) & 0xFFFFFFFFFFFFFFFF, ops.seed_offset() or 0)
 
 
 def relpos_attention(q, k, v, table, buckets, key_mask=None, scale=None, q_start=0, dropout_p=0.0, seed=None):

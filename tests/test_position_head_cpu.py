@@ -54,6 +54,17 @@ def test_model_options():
     assert _keys(create_foundation_model(config).classification_layers["a"]) == []
 
 
+def test_nodes_are_those_of_this_tree(monkeypatch):
+    """The C++ module that makes the operators' calls was compiled against this header and this torch, or is refused."""
+    import mia_amd._lib as _lib
+    from mia_amd import _proto
+    assert _lib.nodes().digest() == _proto.autograd_digest()
+    monkeypatch.setattr(_lib, "_nodes", None)
+    monkeypatch.setattr(_proto, "autograd_digest", lambda: "another")
+    with pytest.raises(ImportError, match="another header or another torch"):
+        _lib.nodes()
+
+
 @pytest.mark.parametrize("height,width", [(1, 5), (4, 1), (3, 7), (12, 2)])
 def test_plan_of_a_map(height, width):
     """One table serves maps of every size, a single row among them; the buckets are those of a loop over the pairs."""
