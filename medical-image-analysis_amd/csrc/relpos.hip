@@ -51,7 +51,7 @@ struct RpArgs {
     float *po, *pml;              // split forward: [splits][B * heads * Lq][D], [..][2]
     int B, heads, Lq, Lk, D, W, off, n_off, q_start;
     unsigned inv_w;               // ceil(2^32 / W)
-    int tiles, splits, acc_mask, slab_ld;
+    int tiles, splits, acc_mask, slab_ld, few;
     float scale, sl2, pdrop;
     unsigned long long seed;
     const unsigned long long* seed_off;
@@ -592,6 +592,223 @@ __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void
             if (col < a.D) rp_store_out<T>(a, at + col, o[i][d] * inv);
         }
     }
+}
+
+// ------------------------------------------------------------------------------------------------
+// forward of at most 16 queries (one new token against a long series): reading the keys and values is all the work. Waves take
+// chunks of KEYS keys in turn and never wait for each other: a wave's keys go from memory into the operand registers, its values
+// through a piece of LDS of its own for the transposing read, and the next chunk is requested before the softmax of this one. The four
+// waves of a workgroup share one head's keys or read four neighbouring heads (rp_plan); the waves of a head are joined in LDS at the end,
+// workgroups by relpos_join_few_kernel. One query against 16384 keys, batch 8, 8 heads of 64 in bf16, keys and values not in any
+// cache: 52 us = 5.2 TB/s with four heads a workgroup, 56 with two, 62 with one (128-byte pieces of memory), 64 with the tiled kernel
+// above, of whose four waves one works; 155 keys, 8 heads of 48 in fp32: 7.5 us, 11.6 with that kernel.
+// ------------------------------------------------------------------------------------------------
+#define RP_FEW 16
+template <typename T, int DP>
+struct RpFew {
+    static constexpr int KEYS = DP * (int)sizeof(T) <= 128 ? 64 : 32, LD = RpDim<T, DP>::LD, PIECES = KEYS * RpDim<T, DP>::CPR / 64;
+    static constexpr size_t LDS = 4 * (size_t)KEYS * LD * sizeof(T);
+    static_assert(LDS >= 4 * RP_FEW * (DP + 2) * sizeof(float), "the joining of the waves does not fit");
+};
+static int rp_few_keys(int dtype, int DP) { return DP * (dtype == MIA_BF16 ? 2 : 4) <= 128 ? 64 : 32; }
+
+// LDS that only this wave's lanes share: its accesses are carried out in order, the compiler has to keep the order too
+__device__ __forceinline__ void rp_wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, DP * (int)sizeof(T) <= 64 ? 3 : DP * (int)sizeof(T) <= 384 ? 2 : 1) void relpos_few_kernel(RpArgs a) {
+    typedef RpOp<T> Op;
+    typedef RpDim<T, DP> Dim;
+    typedef RpFew<T, DP> Few;
+    constexpr int LD = Dim::LD, KEYS = Few::KEYS, KB = KEYS / 16, CPR = Dim::CPR;
+    __shared__ __attribute__((aligned(16))) char sm[Few::LDS];
+    const int groups = a.heads / a.few, ranks = 4 / a.few, split = blockIdx.x / (a.B * groups), id = blockIdx.x - split * a.B * groups;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = lane & 15, g = lane >> 4;
+    const int b = id / groups, h0 = (id - b * groups) * a.few, h = h0 + wave % a.few;
+    const T* kp = (const T*)a.k + b * a.sk.b + h * a.sk.h;
+    const T* vp = (const T*)a.v + b * a.sv.b + h * a.sv.h;
+    T* Vs = reinterpret_cast<T*>(sm) + wave * KEYS * LD;
+    const int query = min(l, a.Lq - 1);
+    const float* bias = a.bias + (size_t)h * a.n_off + (a.off - rp_c(a, a.q_start + query));   // of this lane's query, by c(key)
+    typename Op::Frag qf[Dim::NCH];
+    rp_row_frags<T, DP>((const T*)a.q + b * a.sq.b + (long long)query * a.sq.t + h * a.sq.h, l < a.Lq, a.D, g, qf);
+    const unsigned long long seed = a.pdrop > 0.f ? rp_seed(a) : 0ull;
+
+    typename Op::Frag kf[KB][Dim::NCH];
+    uint4 vr[Few::PIECES];
+    float br[KB][4];
+    int byte = 0;
+    auto fetch = [&](int t) {
+        const int k0 = t * KEYS;
+        byte = rp_mask_byte(a, b, k0);
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            const T* row = kp + (long long)min(k0 + kb * 16 + l, a.Lk - 1) * a.sk.t;
+#pragma unroll
+            for (int c = 0; c < Dim::NCH; ++c) {
+                const int col = c * Op::CHUNK + g * Op::PER;
+                kf[kb][c] = *reinterpret_cast<const typename Op::Frag*>(row + (col < a.D ? col : 0));
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < Few::PIECES; ++i) {
+            const int piece = i * 64 + lane, row = piece / CPR, col = (piece - row * CPR) * Op::PER;
+            vr[i] = *reinterpret_cast<const uint4*>(vp + (long long)min(k0 + row, a.Lk - 1) * a.sv.t + (col < a.D ? col : 0));
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) br[kb][r] = bias[rp_c(a, min(k0 + kb * 16 + g * 4 + r, a.Lk - 1))];
+    };
+    float m = -INFINITY, sum = 0.f;
+    rp_f32x4 o[Dim::DB];
+#pragma unroll
+    for (int d = 0; d < Dim::DB; ++d) o[d] = rp_f32x4{0.f, 0.f, 0.f, 0.f};
+    const int t1 = (int)((long long)a.tiles * (split + 1) / a.splits);
+    int t = (int)((long long)a.tiles * split / a.splits) + wave / a.few;
+    if (t < t1) fetch(t);
+    for (; t < t1; t += ranks) {
+        const unsigned long long all = KEYS == 64 ? ~0ull : (1ull << KEYS) - 1, here = rp_valid(a, t * KEYS, byte) & all;
+        rp_f32x4 s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) s[kb] = rp_f32x4{br[kb][0], br[kb][1], br[kb][2], br[kb][3]};
+        // columns past D are zero in the query's operand; in the keys' they repeat the first ones, which may not be finite
+#pragma unroll
+        for (int c = 0; c < Dim::NCH; ++c)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                if (c * Op::CHUNK + g * Op::PER >= a.D) kf[kb][c] = typename Op::Frag{};
+                s[kb] = Op::dot(kf[kb][c], qf[c], s[kb]);
+            }
+        rp_wave_sync();
+#pragma unroll
+        for (int i = 0; i < Few::PIECES; ++i) {
+            const int piece = i * 64 + lane, row = piece / CPR;
+            *reinterpret_cast<uint4*>(Vs + row * LD + (piece - row * CPR) * Op::PER) = (here >> row) & 1 ? vr[i] : make_uint4(0u, 0u, 0u, 0u);
+        }
+        rp_wave_sync();
+        if (t + ranks < t1) fetch(t + ranks);
+        if (here == 0ull) continue;
+        if (here != all) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[kb][r] = (here >> (kb * 16 + g * 4 + r)) & 1 ? s[kb][r] : -INFINITY;
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[kb][r]);
+        mx = fmaxf(m, rp_xor_max(mx));
+        const float use = mx == -INFINITY ? 0.f : mx, alpha = __builtin_amdgcn_exp2f((m - use) * a.sl2);
+        sum *= alpha;
+#pragma unroll
+        for (int d = 0; d < Dim::DB; ++d) o[d] *= alpha;
+        m = mx;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[kb][r] = __builtin_amdgcn_exp2f((s[kb][r] - use) * a.sl2);
+            sum += (s[kb][0] + s[kb][1]) + (s[kb][2] + s[kb][3]);
+        }
+        if (a.pdrop > 0.f) {
+            const unsigned long long at = ((unsigned long long)(b * a.heads + h) * a.Lq + query) * a.Lk + (unsigned)(t * KEYS) + g * 4;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[kb][r] *= rp_drop(seed, at + kb * 16 + r, a.pdrop);
+        }
+#pragma unroll
+        for (int kk = 0; kk < KB / 2; ++kk) {
+            const typename Op::Pair p = Op::pack(s[2 * kk], s[2 * kk + 1]);
+            typename Op::Pair more;
+            if constexpr (sizeof(T) == 2) more = Op::rest(s[2 * kk], s[2 * kk + 1], p);
+#pragma unroll
+            for (int d = 0; d < Dim::DB; ++d) {
+                const T* v0 = Vs + (kk * 32 + g * 4) * LD + d * 16;
+                const typename Op::TFrag vf = Op::load_t(v0, v0 + 16 * LD, LD, l);
+                o[d] = Op::dot_t(vf, p, o[d]);
+                if constexpr (sizeof(T) == 2) o[d] = Op::dot_t(vf, more, o[d]);
+            }
+        }
+    }
+    // maxima, sums and outputs of the waves of a head, joined in wave order
+    sum = rp_xor_sum(sum);
+    float* os = reinterpret_cast<float*>(sm);      // [wave][query][DP]
+    float2* ml = reinterpret_cast<float2*>(os + 4 * RP_FEW * DP);
+    __syncthreads();
+    if (g == 0) ml[wave * RP_FEW + l] = make_float2(m, sum);
+#pragma unroll
+    for (int d = 0; d < Dim::DB; ++d) *reinterpret_cast<rp_f32x4*>(os + (wave * RP_FEW + l) * DP + d * 16 + g * 4) = o[d];
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.few * a.Lq * (DP / 4); i += 256) {
+        const int hq = i / (DP / 4), col = (i - hq * (DP / 4)) * 4, hh = hq / a.Lq, q = hq - hh * a.Lq;
+        if (col >= a.D) continue;
+        float top = -INFINITY, total = 0.f;
+        for (int w = hh; w < 4; w += a.few) top = fmaxf(top, ml[w * RP_FEW + q].x);
+        const float use = top == -INFINITY ? 0.f : top;
+        rp_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int w = hh; w < 4; w += a.few) {
+            const float2 x = ml[w * RP_FEW + q];
+            const float weight = __builtin_amdgcn_exp2f((x.x - use) * a.sl2);
+            total = fmaf(x.y, weight, total);
+            acc += *reinterpret_cast<const rp_f32x4*>(os + (w * RP_FEW + q) * DP + col) * weight;
+        }
+        const size_t row = ((size_t)b * a.heads + h0 + hh) * a.Lq + q;
+        if (a.splits > 1) {
+            const size_t prow = (size_t)split * a.B * a.heads * a.Lq + row;
+            if (col == 0) reinterpret_cast<float2*>(a.pml)[prow] = make_float2(top, total);
+            *reinterpret_cast<rp_f32x4*>(a.po + prow * a.D + col) = acc;
+        } else {
+            const float inv = total == 0.f ? 0.f : 1.0f / total;
+            rp_store_out<T>(a, (((size_t)b * a.Lq + q) * a.heads + h0 + hh) * a.D + col, acc * inv);
+            if (a.stat && col == 0) a.stat[row] = rp_stat(top, total);
+        }
+    }
+}
+
+// Joins the partial results of relpos_few_kernel: few rows in many splits, so a workgroup per row, whose threads share the splits
+// (64 rows of 64 in 16 splits: 5 us; 12 with a thread per four channels that walks the splits).
+template <typename T, int DP>
+__global__ __launch_bounds__(256) void relpos_join_few_kernel(RpArgs a) {
+    constexpr int QUADS = DP <= 16 ? 4 : DP <= 32 ? 8 : DP <= 64 ? 16 : 32, LANES = 256 / QUADS;
+    __shared__ rp_f32x4 os[LANES][QUADS];
+    __shared__ float2 ml[LANES];
+    const size_t rows = (size_t)a.B * a.heads * a.Lq, row = blockIdx.x;
+    const int quad = threadIdx.x % QUADS, sl = threadIdx.x / QUADS, d = quad * 4;
+    const float2* pml = reinterpret_cast<const float2*>(a.pml);
+    float m = -INFINITY, total = 0.f;
+    for (int s = sl; s < a.splits; s += LANES) m = fmaxf(m, pml[s * rows + row].x);
+    float use = m == -INFINITY ? 0.f : m;
+    rp_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = sl; s < a.splits; s += LANES) {
+        const float2 x = pml[s * rows + row];
+        const float w = __builtin_amdgcn_exp2f((x.x - use) * a.sl2);
+        total = fmaf(x.y, w, total);
+        if (d < a.D) acc += *reinterpret_cast<const rp_f32x4*>(a.po + (s * rows + row) * a.D + d) * w;
+    }
+    os[sl][quad] = acc;
+    if (quad == 0) ml[sl] = make_float2(m, total);
+    __syncthreads();
+    if (sl != 0 || d >= a.D) return;
+    const int n = min(LANES, a.splits);
+    m = -INFINITY;
+    for (int i = 0; i < n; ++i) m = fmaxf(m, ml[i].x);
+    use = m == -INFINITY ? 0.f : m;
+    total = 0.f;
+    acc = rp_f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < n; ++i) {
+        const float w = __builtin_amdgcn_exp2f((ml[i].x - use) * a.sl2);
+        total = fmaf(ml[i].y, w, total);
+        acc += os[i][quad] * w;
+    }
+    const size_t bh = row / a.Lq, b = bh / a.heads, h = bh - b * a.heads, t = row - bh * a.Lq;
+    rp_store_out<T>(a, ((b * a.Lq + t) * a.heads + h) * a.D + d, acc * (total == 0.f ? 0.f : 1.0f / total));
+    if (a.stat && d == 0) a.stat[row] = rp_stat(m, total);
 }
 
 // Joins the partial results of kernels that were split over the tokens they walk: a thread per four channels of a row, the
@@ -1303,17 +1520,33 @@ static size_t rp_es(int dtype) { return dtype == MIA_BF16 ? 2 : 4; }
 // partial results weigh. Measured (us, kernel + join), with the choice first: forward on a 75x75 map, 4 heads of 32: one column, 5
 // splits 73 + 6, 2 splits 82 + 5, 3 splits 85 + 5; two columns, 4 splits 85 + 6. 4096 tokens, 4 heads of 64: two columns, 4 splits
 // 54 + 7, 3 splits 66 + 6, 5 splits 65 + 7; one column, 3 splits 57 + 6. 38x38, batch 4, 8 heads of 64: one column unsplit 50, 3
-// splits 50 + 11; two columns unsplit 58. 10x10, batch 128, 8 heads of 48: two columns 27, one 30. One query, 64 workgroups over
-// 16384 keys: 8 splits 48 + 7, 7 splits 52 + 7, 10 splits 61 + 8.
+// splits 50 + 11; two columns unsplit 58. 10x10, batch 128, 8 heads of 48: two columns 27, one 30.
+// At most 16 queries (cols = 0): `few` heads of a workgroup's four waves. With enough keys for 2048 waves of four chunks or more, the
+// waves read neighbouring heads, whose rows are one piece of memory, in ranges that make about 2048 waves; else the waves share one
+// head's keys, four chunks each, which is what a second workgroup and the joining would cost.
+#define RP_FEW_WAVES 2048
 struct RpPlan {
-    int cols, splits;
+    int cols, splits, few;
 };
 static RpPlan rp_plan(int what, int dtype, int B, int heads, int Lq, int Lk, int D) {
     const int DP = rp_dp(D), owned = what == RP_BWD_KV ? Lk : Lq, walked = what == RP_BWD_KV ? Lq : Lk;
     const int round = what == RP_BWD_KV ? RP_TILE : rp_stage(dtype, DP);
     const long long rounds = (walked + round - 1) / round, most = rounds / 4 < 1 ? 1 : rounds / 4 < 64 ? rounds / 4 : 64;
     const int max_cols = dtype == MIA_F32 || DP > (what == RP_FWD ? 96 : 64) || owned <= 64 ? 1 : 2;
-    RpPlan p = {1, 1};
+    RpPlan p = {1, 1, 0};
+    if (what == RP_FWD && Lq <= RP_FEW) {
+        const int keys = rp_few_keys(dtype, DP);
+        const long long bh = (long long)B * heads, chunks = (Lk + keys - 1) / keys;
+        p.cols = 0;
+        p.few = 1;
+        long long s = (chunks + 15) / 16;
+        if (bh * chunks >= 4 * RP_FEW_WAVES) {
+            p.few = heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1;
+            s = (RP_FEW_WAVES * p.few / 4 + bh - 1) / bh;
+        }
+        p.splits = (int)(s < 1 ? 1 : s > 256 ? 256 : s);
+        return p;
+    }
     double best = 1e300;
     for (int cols = 1; cols <= max_cols; ++cols) {
         const long long wgs = (long long)B * heads * ((owned + 64 * cols - 1) / (64 * cols));
@@ -1340,6 +1573,17 @@ static int rp_launch(const char* name, K kernel, dim3 grid, size_t lds, const Rp
 }
 
 // cols: 16-wide columns of a wave
+template <typename T, int DP>
+static int rp_few(const char* name, dim3 grid, const RpArgs& a, hipStream_t s) {
+    MIA_LAUNCH((relpos_few_kernel<T, DP>), grid, dim3(256), 0, s, a);
+    MIA_CHECK_LAUNCH(name);
+    if (a.splits > 1) {
+        MIA_LAUNCH((relpos_join_few_kernel<T, DP>), dim3(a.B * a.heads * a.Lq), dim3(256), 0, s, a);
+        MIA_CHECK_LAUNCH(name);
+    }
+    return 0;
+}
+
 template <typename T, int DP, int COLS>
 static int rp_run(int what, const char* name, dim3 grid, size_t lds, const RpArgs& a, hipStream_t s) {
     if constexpr (COLS == 1 || DP <= 96) {
@@ -1356,6 +1600,7 @@ static int rp_run(int what, const char* name, dim3 grid, size_t lds, const RpArg
 static int rp_dispatch(int what, const char* name, int dtype, int cols, dim3 grid, size_t lds, const RpArgs& a, hipStream_t s) {
 #define RP_CASE(DP_)                                                                                      \
     case DP_:                                                                                             \
+        if (cols == 0) return dtype == MIA_F32 ? rp_few<float, DP_>(name, grid, a, s) : rp_few<bf16_t, DP_>(name, grid, a, s); \
         if (dtype == MIA_F32) return rp_run<float, DP_, 1>(what, name, grid, lds, a, s);          \
         return cols == 2 ? rp_run<bf16_t, DP_, 2>(what, name, grid, lds, a, s)                    \
                          : rp_run<bf16_t, DP_, 1>(what, name, grid, lds, a, s);
@@ -1470,10 +1715,9 @@ extern "C" int mia_relpos_fwd(int dtype, const void* q, const void* k, const voi
         rp_aligned("mia_relpos_fwd", dtype, out_low, RpStride{0, 0, 0}))
         return -1;
     rp_fill(a, B, heads, Lq, Lk, D, height, width, q_start, scale, pdrop, seed, seed_offset);
-    const int stage = rp_stage(dtype, rp_dp(D));
-    a.tiles = (Lk + stage - 1) / stage;
     const RpPlan plan = rp_plan(RP_FWD, dtype, B, heads, Lq, Lk, D);
-    const int cols = plan.cols;
+    const int cols = plan.cols, tile = cols == 0 ? rp_few_keys(dtype, rp_dp(D)) : rp_stage(dtype, rp_dp(D));
+    a.tiles = (Lk + tile - 1) / tile;
     a.splits = plan.splits;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const long long rows = (long long)B * heads * Lq;
@@ -1486,9 +1730,12 @@ extern "C" int mia_relpos_fwd(int dtype, const void* q, const void* k, const voi
         a.pml = ws + (long long)a.splits * rows * D;
     }
     const int tokens = height * width, DP = rp_dp(D);
-    const size_t lds = rp_query_lds(a, dtype, DP, cols, tokens);
-    const int rc = rp_dispatch(RP_FWD, "mia_relpos_fwd", dtype, cols, rp_grid((long long)B * heads * ((Lq + 64 * cols - 1) / (64 * cols)), a.splits), lds, a, s);
-    if (rc || a.splits == 1) return rc;
+    const size_t lds = cols == 0 ? 0 : rp_query_lds(a, dtype, DP, cols, tokens);
+    a.few = plan.few;
+    const long long blocks = cols == 0 ? (long long)B * heads / a.few : (long long)B * heads * ((Lq + 64 * cols - 1) / (64 * cols));
+    const dim3 grid = cols == 0 ? dim3((unsigned)(blocks * a.splits)) : rp_grid(blocks, a.splits);
+    const int rc = rp_dispatch(RP_FWD, "mia_relpos_fwd", dtype, cols, grid, lds, a, s);
+    if (rc || a.splits == 1 || cols == 0) return rc;
     return rp_join<RP_FWD>("mia_relpos_fwd", dtype, a, s);
 }
 

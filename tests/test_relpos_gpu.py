@@ -114,6 +114,30 @@ def test_split_over_the_keys(Lq, Lk, B, heads, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("D", [8, 32, 40, 64, 96, 128])
+@pytest.mark.parametrize("Lq", [1, 2, 15, 16, 17])
+def test_few_queries(Lq, D, dtype):
+    """Both sides of the border between the two forward kernels, over ends inside a chunk of keys, on maps of several rows."""
+    plan = RelativePositionBuckets(9, 37, 8, 16)
+    g = torch.Generator().manual_seed(Lq)
+    for Lk, q_start in ((333, 316), (65, 0)):
+        _check(plan, Lq=Lq, Lk=Lk, q_start=q_start, D=D, dtype=dtype)
+        mask = torch.rand(3, Lk, generator=g) < 0.5
+        mask[0] = False
+        mask[1, :64] = False
+        _check(plan, B=3, Lq=Lq, Lk=Lk, q_start=q_start, D=D, dtype=dtype, mask=mask, drop=0.2)
+
+
+@pytest.mark.parametrize("heads,D,dtype", [(8, 64, BF16), (6, 64, BF16), (7, 32, BF16), (4, 64, F32)])
+def test_few_queries_of_neighbouring_heads(heads, D, dtype):
+    """Enough keys for the variants whose waves read several heads."""
+    B, Lk = -(-9000 // (heads * (4100 // (64 if dtype == BF16 else 32)))), 4100
+    mask = torch.arange(Lk)[None, :] < torch.randint(1, Lk + 1, (B, 1), generator=torch.Generator().manual_seed(18))
+    mask[0] = False
+    _check(RelativePositionBuckets(1, 4200, 32, 128), B=B, heads=heads, Lq=2, Lk=Lk, q_start=Lk - 2, D=D, dtype=dtype, mask=mask)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_scale_and_dropout(dtype):
     plan = RelativePositionBuckets(8, 12, 8, 16)
     _check(plan, scale=1.0, D=16, dtype=dtype)
