@@ -11,6 +11,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
+#include <mutex>
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
@@ -104,9 +105,11 @@ struct RelPosAttentionBackward : torch::autograd::Node {
 
     std::string name() const override { return "RelPosAttentionBackward"; }
     void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
         for (SavedVariable* s : {&q, &k, &v, &bias, &mask, &out, &low, &stat}) s->reset_data();
     }
     variable_list apply(variable_list&& grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
         first_derivative_only("relpos_attention");
         variable_list got(4);
         if (!grads[0].defined()) return got;
@@ -233,10 +236,12 @@ struct GatedResidualNormBackward : torch::autograd::Node {
 
     std::string name() const override { return "GatedResidualNormBackward"; }
     void release_variables() override {
+        const std::lock_guard<std::mutex> lock(mutex_);
         x.reset_data(), f.reset_data(), stats.reset_data();
         for (SavedVariable& p : parameter) p.reset_data();
     }
     variable_list apply(variable_list&& grads) override {
+        const std::lock_guard<std::mutex> lock(mutex_);
         first_derivative_only("gated_residual_norm");
         variable_list got(8);
         Tensor dy = grads[0], dz = pre ? grads[1] : Tensor();

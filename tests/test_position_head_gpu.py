@@ -184,3 +184,71 @@ def test_nothing_is_kept_without_gradients():
         plain = run()
     assert torch.cuda.memory_allocated() - before == 3 * 16 * 64 * 128 * 2
     assert all(torch.equal(a, b) for a, b in zip(kept, plain)) and not any(t.requires_grad for t in plain)
+
+
+def _block(dtype):
+    from mia_amd.block_norm import gated_residual_norm
+    from mia_amd.relpos import RelativePositionBuckets, relpos_attention
+    plan = RelativePositionBuckets(5, 7, 8, 16)
+    g = torch.Generator().manual_seed(5)
+    x = torch.randn(3, 35, 64, generator=g).cuda().to(dtype).requires_grad_()
+    table, w, s = (t.cuda().requires_grad_() for t in (torch.randn(64, 4, generator=g), 1 + torch.randn(64, generator=g), torch.randn(64, generator=g)))
+
+    def run(x):
+        h = x.view(3, 35, 4, 16)
+        a = relpos_attention(h, h * 0.5, h + 1, table, plan)
+        y, z = gated_residual_norm(x, a.reshape(3, 35, 64), scale=s, pre="layer", pre_weight=w)
+        return y + z
+    return run, x, (x, table, w, s)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_inside_checkpoints_and_hooks(dtype):
+    """Recomputed in the backward, with saved tensors moved to the host and back, and twice through one graph: the same bits."""
+    from torch.utils.checkpoint import checkpoint
+    run, x, leaves = _block(dtype)
+    dout = torch.randn(3, 35, 64, device="cuda").to(dtype)
+    out = run(x)
+    want = torch.autograd.grad(out, leaves, dout, retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(out, leaves, dout)))
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(out, leaves, dout)
+    for reentrant in (False, True):
+        for t in leaves:
+            t.grad = None
+        checkpoint(run, x, use_reentrant=reentrant).backward(dout)
+        assert all(torch.equal(a, t.grad) for a, t in zip(want, leaves)), reentrant
+    with torch.autograd.graph.save_on_cpu():
+        out = run(x)
+    assert all(torch.equal(a, b) for a, b in zip(want, torch.autograd.grad(out, leaves, dout)))
+
+
+def test_inputs_changed_in_between_are_noticed():
+    run, x, leaves = _block(torch.float32)
+    out = run(x)
+    with torch.no_grad():
+        leaves[2].mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_two_threads_backward():
+    """Two backward passes at once, each of its own graph over the same leaves."""
+    import threading
+    run, x, leaves = _block(torch.bfloat16)
+    dout = torch.randn(3, 35, 64, device="cuda").bfloat16()
+    want = torch.autograd.grad(run(x), leaves, dout)
+    torch.cuda.synchronize()
+    got = {}
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(8):
+                got[i] = torch.autograd.grad(run(x), leaves, dout)
+        torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(torch.equal(a, b) for i in range(2) for a, b in zip(want, got[i]))
