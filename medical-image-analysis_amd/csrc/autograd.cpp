@@ -367,6 +367,15 @@ Tensor grad_clip(const std::vector<Tensor>& grads, double max_norm) {
     return t.out.select(0, 0);
 }
 
+// Whether AdamW's kernel can take every parameter and its gradient as they are: dense fp32 on the device
+bool update_ready(const std::vector<Tensor>& params) {
+    return std::all_of(params.begin(), params.end(), [](const Tensor& p) {
+        const Tensor& g = p.grad();
+        return g.defined() && p.is_cuda() && g.is_cuda() && p.scalar_type() == at::kFloat && g.scalar_type() == at::kFloat &&
+               g.layout() == at::kStrided && p.is_contiguous() && g.is_contiguous();
+    });
+}
+
 PyObject* refusal = nullptr;   // the library's exception class
 
 }  // namespace
@@ -377,6 +386,7 @@ PYBIND11_MODULE(_mia_autograd, m) {
     m.def("relpos", &relpos, py::call_guard<py::gil_scoped_release>());
     m.def("residual", &residual, py::call_guard<py::gil_scoped_release>());
     m.def("all_dense", &all_dense);
+    m.def("update_ready", &update_ready);
     m.def("grad_norm", &grad_norm, py::call_guard<py::gil_scoped_release>());
     m.def("grad_clip", &grad_clip, py::call_guard<py::gil_scoped_release>());
     py::register_exception_translator([](std::exception_ptr e) {

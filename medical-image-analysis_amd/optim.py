@@ -136,7 +136,8 @@ class AdamW(torch.optim.Optimizer):
             ps = [p for p in group["params"] if p.grad is not None]
             if not ps:
                 continue
-            for p in ps:
+            # attribute by attribute in Python the check is a fifth of a step of 22 parameters
+            for p in (() if nodes().update_ready(ps) else ps):
                 if (not p.is_cuda or not p.grad.is_cuda or p.dtype != torch.float32 or p.grad.dtype != torch.float32
                         or not p.is_contiguous() or p.grad.is_sparse):
                     raise RuntimeError("mia_amd.optim.AdamW needs contiguous fp32 parameters on an MI355X device")

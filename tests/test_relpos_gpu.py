@@ -325,6 +325,22 @@ def test_offsets_past_32_bits():
         _compare(o, want["out"], tol["out"])
 
 
+@pytest.mark.parametrize("Lq", [2, 40])
+def test_tokens_past_32_bits(Lq):
+    """Tokens so far apart that the last ones lie more than 2^31 elements (2^32 bytes) behind the first."""
+    plan = RelativePositionBuckets(1, 150, 8, 16)
+    q, k, v, table, dout = _inputs(1, Lq, 150, 1, 16, BF16, 8, 19)
+    apart = (1 << 24) - 8
+    store = torch.empty(149 * apart + 32, dtype=BF16, device="cuda")
+    kc, vc = (store[i:].as_strided((1, 150, 1, 16), (16, apart, 16, 1)) for i in (0, 16))
+    kc.copy_(k), vc.copy_(v)
+    mine = [q.cuda().requires_grad_(), kc.requires_grad_(), vc.requires_grad_(), table.cuda().requires_grad_()]
+    want, tol = formula(q, k, v, table, plan, q_start=100, dout=dout)
+    out = relpos_attention(*mine, plan, q_start=100)
+    for name, value in zip(("out", "dq", "dk", "dv", "dtable"), (out.detach(), *torch.autograd.grad(out, mine, dout.cuda()))):
+        _compare(value, want[name], tol[name], name)
+
+
 def test_repeatable_streams_and_capture():
     plan = RelativePositionBuckets(12, 12, 16, 32)
     q, k, v, table, dout = _inputs(4, 144, 144, 4, 48, BF16, plan.num_buckets, 14)
