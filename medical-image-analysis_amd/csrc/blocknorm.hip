@@ -18,7 +18,7 @@
 // every tensor is read once and written once: two in, two out forward; four in, two out backward. The statistics of both
 // norms are kept (16 bytes a row). The next row is requested while one is worked on: a wave has one or two rows in flight instead of
 // waiting out every load (32 images of 1444 rows of 1024 bf16 channels, two RMS norms: forward 91 -> 73 us, backward 164 -> 131;
-// now 65, 5.8 TB/s, and 132, 4.3 TB/s). Long batches of rows are bound by HBM, short ones (a head's 100 tokens) by latency.
+// now 65, 5.8 TB/s, and 125, 4.5 TB/s). Long batches of rows are bound by HBM, short ones (a head's 100 tokens) by latency.
 // The backward keeps its column sums in registers over all rows of a workgroup and leaves one slab row; two small kernels add
 // the slab up in a fixed order (no atomics).
 #include "common.h"
@@ -162,6 +162,25 @@ __device__ __forceinline__ void bn_stats(const float (&t)[R * V], int kind, int 
     r = 1.0f / sqrtf(fmaf(s, a.inv_c, a.eps));
 }
 
+// The branch's affine part as it is used, y = x + (mul * fhat + add): mul = scale * gate * w1, add = scale * gate * b1. Two vectors
+// instead of three, and both directions form the same y; 200000 rows of 384 bf16 channels, two RMS norms: backward 236 -> 194 us.
+template <int V, int R, int TPR>
+__device__ __forceinline__ void bn_affine(const BNormArgs& a, int n, int lane, float (&mul)[R * V], float (&add)[R * V]) {
+    float t[R * V];
+    bn_param<V, R, TPR>(a.scale, 1.f, lane, a.C, mul);
+    if (a.gate) {
+        bn_param<V, R, TPR>(a.gate + (size_t)n * a.C, 1.f, lane, a.C, t);
+#pragma unroll
+        for (int i = 0; i < R * V; ++i) mul[i] *= t[i];
+    }
+    bn_param<V, R, TPR>(a.b1, 0.f, lane, a.C, t);
+#pragma unroll
+    for (int i = 0; i < R * V; ++i) add[i] = mul[i] * t[i];
+    bn_param<V, R, TPR>(a.w1, 1.f, lane, a.C, t);
+#pragma unroll
+    for (int i = 0; i < R * V; ++i) mul[i] *= t[i];
+}
+
 template <typename T, int V, int R, int TPR, int WG>
 __global__ __launch_bounds__(WG) void blocknorm_fwd_kernel(BNormArgs a) {
     __shared__ float2 sm[2 * (WG / 64)];
@@ -169,15 +188,8 @@ __global__ __launch_bounds__(WG) void blocknorm_fwd_kernel(BNormArgs a) {
     const int n = blockIdx.x / a.S, s = blockIdx.x % a.S;
     const int lane = threadIdx.x % TPR, row_of = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);   // a row is whole waves: scalar addresses
     const long long lo = a.T * s / a.S, hi = a.T * (s + 1) / a.S;
-    float amp[R * V], w1[R * V], b1[R * V], w2[R * V], b2[R * V];
-    bn_param<V, R, TPR>(a.scale, 1.f, lane, a.C, amp);
-    if (a.gate) {
-        bn_param<V, R, TPR>(a.gate + (size_t)n * a.C, 1.f, lane, a.C, w1);
-#pragma unroll
-        for (int i = 0; i < R * V; ++i) amp[i] *= w1[i];
-    }
-    bn_param<V, R, TPR>(a.w1, 1.f, lane, a.C, w1);
-    bn_param<V, R, TPR>(a.b1, 0.f, lane, a.C, b1);
+    float mul[R * V], add[R * V], w2[R * V], b2[R * V];
+    bn_affine<V, R, TPR>(a, n, lane, mul, add);
     bn_param<V, R, TPR>(a.w2, 1.f, lane, a.C, w2);
     bn_param<V, R, TPR>(a.b2, 0.f, lane, a.C, b2);
     BNormRow<T, V, R, TPR> fr, xr;
@@ -199,10 +211,10 @@ __global__ __launch_bounds__(WG) void blocknorm_fwd_kernel(BNormArgs a) {
         if (a.post) {
             bn_stats<V, R, TPR>(f, a.post, lane, a, sum, m1, r1);
 #pragma unroll
-            for (int i = 0; i < R * V; ++i) f[i] = fmaf((f[i] - m1) * r1, w1[i], b1[i]);
+            for (int i = 0; i < R * V; ++i) f[i] = (f[i] - m1) * r1;
         }
 #pragma unroll
-        for (int i = 0; i < R * V; ++i) y[i] = fmaf(amp[i], f[i], y[i]);
+        for (int i = 0; i < R * V; ++i) y[i] += fmaf(mul[i], f[i], add[i]);
         if (TPR * R * V != a.C) {   // channels behind the last one stay zero for the statistics' plain sum
 #pragma unroll
             for (int r = 0; r < R; ++r)
@@ -243,23 +255,10 @@ __global__ __launch_bounds__(WG) void blocknorm_bwd_kernel(BNormArgs a) {
     // parameters, but read those again (from L2) where a row needs them (2048 rows of 8192, two RMS norms: 169 -> 97 us in
     // bf16, 251 -> 167 us in fp32). Single elements spill either way (353 us, 517 us so).
     constexpr bool SLIM = TPR == 1024 && V > 1 && R * V == 8;
-    float amp[R * V], w1[R * V], b1[R * V], w2[R * V];
-    auto load_amp = [&]() {
-        bn_param<V, R, TPR>(a.scale, 1.f, lane, a.C, amp);
-        if (a.gate) {
-            float t[R * V];
-            bn_param<V, R, TPR>(a.gate + (size_t)n * a.C, 1.f, lane, a.C, t);
-#pragma unroll
-            for (int i = 0; i < R * V; ++i) amp[i] *= t[i];
-        }
-    };
-    auto load_w1 = [&]() { bn_param<V, R, TPR>(a.w1, 1.f, lane, a.C, w1); };
-    auto load_b1 = [&]() { bn_param<V, R, TPR>(a.b1, 0.f, lane, a.C, b1); };
+    float mul[R * V], add[R * V], w2[R * V];
     auto load_w2 = [&]() { bn_param<V, R, TPR>(a.w2, 1.f, lane, a.C, w2); };
     if constexpr (!SLIM) {
-        load_amp();
-        load_w1();
-        load_b1();
+        bn_affine<V, R, TPR>(a, n, lane, mul, add);
         load_w2();
     }
     float s1[R * V], s2[R * V], s3[R * V], s4[R * V];
@@ -300,14 +299,12 @@ __global__ __launch_bounds__(WG) void blocknorm_bwd_kernel(BNormArgs a) {
         if (a.dz) {
             float p = 0.f, q = 0.f;
             if constexpr (SLIM) {
-                load_amp();
-                load_w1();
-                load_b1();
+                bn_affine<V, R, TPR>(a, n, lane, mul, add);
                 load_w2();
             }
 #pragma unroll
             for (int i = 0; i < R * V; ++i) {
-                y[i] = (fmaf(amp[i], fmaf(f[i], w1[i], b1[i]), y[i]) - st.z) * st.w;
+                y[i] = (y[i] + fmaf(mul[i], f[i], add[i]) - st.z) * st.w;
                 const float d = z[i] * w2[i];   // zero behind the last channel, where dz was not loaded
                 p += d;
                 q = fmaf(d, y[i], q);
@@ -327,22 +324,21 @@ __global__ __launch_bounds__(WG) void blocknorm_bwd_kernel(BNormArgs a) {
             const int c = (r * TPR + lane) * V;
             if (c < a.C) bn_store<T, V>((T*)a.dx + at + c, g + r * V);
         }
-        if constexpr (SLIM) load_amp();
+        if constexpr (SLIM) bn_affine<V, R, TPR>(a, n, lane, mul, add);
 #pragma unroll
         for (int i = 0; i < R * V; ++i) {
             s1[i] = fmaf(g[i], f[i], s1[i]);
             s2[i] += g[i];
-            g[i] *= amp[i];
+            g[i] *= mul[i];
         }
         if (a.post) {
             float p = 0.f, q = 0.f;
-            if constexpr (SLIM) load_w1();
 #pragma unroll
             for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int k = 0; k < V; ++k) {
                     const int i = r * V + k;
-                    g[i] = (r * TPR + lane) * V + k < a.C ? g[i] * w1[i] : 0.f;
+                    if ((r * TPR + lane) * V + k >= a.C) g[i] = 0.f;
                     p += g[i];
                     q = fmaf(g[i], f[i], q);
                 }
@@ -493,12 +489,13 @@ static void bn_dispatch(bool fwd, bool vec, const BNormArgs& a, hipStream_t s) {
 // Workgroups an image's rows are split over: as many in all as are resident at once, so that the rows come out even, with at
 // least one row a wave forward and two backward, two where a workgroup has a row (100 rows of 384 bf16 channels: forward 3.6 us,
 // 7.2 with four rows a wave; backward 6.7 and 8.7).
-// Backward two a CU (32 images of 1444 rows of 1024 bf16 channels: 134 us, 142 with 1024 workgroups, 132 with 256; 200000 rows
-// of 384: 236, 244 and 354). Forward four a CU with eight channels a lane (200000 rows of 384 bf16 channels: 120 us, 143 with
-// 512), three with sixteen (rows of 1024: 65 us, 70 with 1024, 67 with 512), two with a workgroup a row (8000 rows of 2048: 28
-// us, 45 with 256).
+// Backward three a CU up to 512 channels (100000 rows of 256 fp32 channels: 126 us, 134 with 512 workgroups; 200000 of 384 in bf16:
+// 194 and 196), else two (32 images of 1444 rows of 1024 bf16 channels: 125 us; 142 with 1024 workgroups and 134 with 512
+// before the affine part was kept as two vectors). Forward four a CU with eight channels a lane (200000 rows of 384 bf16 channels:
+// 120 us, 143 with 512), three with sixteen (rows of 1024: 65 us, 70 with 1024, 67 with 512), two with a workgroup a row (8000
+// rows of 2048: 28 us, 45 with 256).
 static int bn_splits(bool fwd, int dtype, long long images, long long rows, int C) {
-    const long long want = !fwd || C > 1024 ? 512 : dtype == MIA_BF16 && C > 512 ? 768 : 1024, per = C > 512 ? 2 : fwd ? 4 : 8;
+    const long long want = !fwd ? (C <= 512 ? 768 : 512) : C > 1024 ? 512 : dtype == MIA_BF16 && C > 512 ? 768 : 1024, per = C > 512 ? 2 : fwd ? 4 : 8;
     long long s = (want + images - 1) / images;
     if (s > rows / per) s = rows / per;
     return s < 1 ? 1 : (int)s;
