@@ -330,7 +330,8 @@ __device__ __forceinline__ unsigned long long rp_valid(const RpArgs& a, int k0, 
 // the XCDs in turn when their number is a multiple of eight (the heads of a packed token share cache lines: 10x10 maps, batch 128,
 // 8 heads of 48: forward 20 us, 23 with heads dealt out), else (image, head)s are (an image that is masked out then costs
 // every XCD the same: 38x38 maps, batch 4, one of them empty: forward 46 us, 48 with a run for each XCD), else each XCD gets an
-// equal run of blocks. The grid is a multiple of 8; ids past the last block have nothing to do.
+// equal run of blocks. (Times from before P was split in two numbers.) The grid is a multiple of 8; ids past the last block have
+// nothing to do.
 __device__ __forceinline__ int rp_block(const RpArgs& a, int per) {
     const int id = blockIdx.x, bhs = a.B * a.heads;
     if (bhs & 7) return (id & 7) * ((int)gridDim.x >> 3) + (id >> 3);
@@ -460,109 +461,109 @@ __global__ __launch_bounds__(256, rp_waves(RP_FWD, sizeof(T) == 2, DP, QB)) void
         if (idle) continue;
 #pragma unroll 1
         for (int hv = 0; hv < HV; ++hv) {
-        const unsigned long long here = HV == 1 || hv == 0 ? valid[0] : valid[HV - 1];
-        if (here == 0ull) continue;
-        const T *Kh = Ks + hv * RP_TILE * LD, *Vh = Vs + hv * RP_TILE * LD;
-        const int* ckh = ck + hv * RP_TILE;
-        rp_f32x4 s[4][QB];
-#pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-            const int4 c4 = *reinterpret_cast<const int4*>(ckh + kb * 16 + g * 4);
-#pragma unroll
-            for (int i = 0; i < QB; ++i) s[kb][i] = rp_bias4(bw, c4, cq[i]);
-        }
-#pragma unroll
-        for (int c = 0; c < Dim::NCH; ++c)
+            const unsigned long long here = HV == 1 || hv == 0 ? valid[0] : valid[HV - 1];
+            if (here == 0ull) continue;
+            const T *Kh = Ks + hv * RP_TILE * LD, *Vh = Vs + hv * RP_TILE * LD;
+            const int* ckh = ck + hv * RP_TILE;
+            rp_f32x4 s[4][QB];
 #pragma unroll
             for (int kb = 0; kb < 4; ++kb) {
-                const typename Op::Frag kf = *reinterpret_cast<const typename Op::Frag*>(Kh + (kb * 16 + l) * LD + c * Op::CHUNK + g * Op::PER);
+                const int4 c4 = *reinterpret_cast<const int4*>(ckh + kb * 16 + g * 4);
 #pragma unroll
-                for (int i = 0; i < QB; ++i) s[kb][i] = Op::dot(kf, qf[i][c], s[kb][i]);
+                for (int i = 0; i < QB; ++i) s[kb][i] = rp_bias4(bw, c4, cq[i]);
             }
-        // the value operands are requested here, so that they arrive while the softmax runs
-        typename Op::TFrag vf[2][Dim::DB];
-        auto values = [&](int kk) {
 #pragma unroll
-            for (int d = 0; d < Dim::DB; ++d) {
-                const T* v0 = Vh + (kk * 32 + g * 4) * LD + d * 16;
-                vf[kk][d] = Op::load_t(v0, v0 + 16 * LD, LD, l);
+            for (int c = 0; c < Dim::NCH; ++c)
+#pragma unroll
+                for (int kb = 0; kb < 4; ++kb) {
+                    const typename Op::Frag kf = *reinterpret_cast<const typename Op::Frag*>(Kh + (kb * 16 + l) * LD + c * Op::CHUNK + g * Op::PER);
+#pragma unroll
+                    for (int i = 0; i < QB; ++i) s[kb][i] = Op::dot(kf, qf[i][c], s[kb][i]);
+                }
+            // the value operands are requested here, so that they arrive while the softmax runs
+            typename Op::TFrag vf[2][Dim::DB];
+            auto values = [&](int kk) {
+#pragma unroll
+                for (int d = 0; d < Dim::DB; ++d) {
+                    const T* v0 = Vh + (kk * 32 + g * 4) * LD + d * 16;
+                    vf[kk][d] = Op::load_t(v0, v0 + 16 * LD, LD, l);
+                }
+            };
+            if constexpr (Dim::EARLY) {
+                values(0);
+                __builtin_amdgcn_sched_barrier(0);
             }
-        };
-        if constexpr (Dim::EARLY) {
-            values(0);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        if (here != ~0ull) {
+            if (here != ~0ull) {
 #pragma unroll
-            for (int kb = 0; kb < 4; ++kb) {
-                const rp_f32x4 c4 = *reinterpret_cast<const rp_f32x4*>(cap + hv * RP_TILE + kb * 16 + g * 4);
+                for (int kb = 0; kb < 4; ++kb) {
+                    const rp_f32x4 c4 = *reinterpret_cast<const rp_f32x4*>(cap + hv * RP_TILE + kb * 16 + g * 4);
 #pragma unroll
-                for (int i = 0; i < QB; ++i)
+                    for (int i = 0; i < QB; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[kb][i][r] = fminf(s[kb][i][r], c4[r]);
+                        for (int r = 0; r < 4; ++r) s[kb][i][r] = fminf(s[kb][i][r], c4[r]);
+                }
             }
-        }
 #pragma unroll
-        for (int i = 0; i < QB; ++i) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[kb][i][r]);
-            mx = fmaxf(m[i], rp_xor_max(mx));
-            const float use = mx == -INFINITY ? 0.f : mx;
-            if (__any(mx > m[i])) {
-                const float alpha = __builtin_amdgcn_exp2f((m[i] - use) * a.sl2);
-                sum[i] *= alpha;
-#pragma unroll
-                for (int d = 0; d < Dim::DB; ++d) o[i][d] *= alpha;
-            }
-            m[i] = mx;
-            // one FMA where the rounding of use * sl2 cannot matter, the difference first where it would
-            if (!__any(fabsf(use) * a.sl2 > RP_FAR)) {
-                const float shift = use * a.sl2;
+            for (int i = 0; i < QB; ++i) {
+                float mx = -INFINITY;
 #pragma unroll
                 for (int kb = 0; kb < 4; ++kb)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[kb][i][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][i][r], a.sl2, -shift));
-            } else {
+                    for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[kb][i][r]);
+                mx = fmaxf(m[i], rp_xor_max(mx));
+                const float use = mx == -INFINITY ? 0.f : mx;
+                if (__any(mx > m[i])) {
+                    const float alpha = __builtin_amdgcn_exp2f((m[i] - use) * a.sl2);
+                    sum[i] *= alpha;
 #pragma unroll
-                for (int kb = 0; kb < 4; ++kb)
+                    for (int d = 0; d < Dim::DB; ++d) o[i][d] *= alpha;
+                }
+                m[i] = mx;
+                // one FMA where the rounding of use * sl2 cannot matter, the difference first where it would
+                if (!__any(fabsf(use) * a.sl2 > RP_FAR)) {
+                    const float shift = use * a.sl2;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) s[kb][i][r] = __builtin_amdgcn_exp2f((s[kb][i][r] - use) * a.sl2);
+                    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[kb][i][r] = __builtin_amdgcn_exp2f(fmaf(s[kb][i][r], a.sl2, -shift));
+                } else {
+#pragma unroll
+                    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[kb][i][r] = __builtin_amdgcn_exp2f((s[kb][i][r] - use) * a.sl2);
+                }
+                float part[4];
+#pragma unroll
+                for (int kb = 0; kb < 4; ++kb) part[kb] = (s[kb][i][0] + s[kb][i][1]) + (s[kb][i][2] + s[kb][i][3]);
+                sum[i] += (part[0] + part[1]) + (part[2] + part[3]);
+                if (a.pdrop > 0.f) {
+                    const unsigned long long at = ((unsigned long long)bh * a.Lq + qi[i]) * a.Lk + t * ST + hv * RP_TILE + g * 4;
+#pragma unroll
+                    for (int kb = 0; kb < 4; ++kb)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) s[kb][i][r] *= rp_drop(seed, at + kb * 16 + r, a.pdrop);
+                }
             }
-            float part[4];
 #pragma unroll
-            for (int kb = 0; kb < 4; ++kb) part[kb] = (s[kb][i][0] + s[kb][i][1]) + (s[kb][i][2] + s[kb][i][3]);
-            sum[i] += (part[0] + part[1]) + (part[2] + part[3]);
-            if (a.pdrop > 0.f) {
-                const unsigned long long at = ((unsigned long long)bh * a.Lq + qi[i]) * a.Lk + t * ST + hv * RP_TILE + g * 4;
+            for (int kk = 0; kk < 2; ++kk) {
+                typename Op::Pair p[QB];
 #pragma unroll
-                for (int kb = 0; kb < 4; ++kb)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) s[kb][i][r] *= rp_drop(seed, at + kb * 16 + r, a.pdrop);
-            }
-        }
-#pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            typename Op::Pair p[QB];
-#pragma unroll
-            for (int i = 0; i < QB; ++i) p[i] = Op::pack(s[2 * kk][i], s[2 * kk + 1][i]);
-            typename Op::Pair more[QB];
-            if constexpr (sizeof(T) == 2)
-#pragma unroll
-                for (int i = 0; i < QB; ++i) more[i] = Op::rest(s[2 * kk][i], s[2 * kk + 1][i], p[i]);
-            if (!Dim::EARLY) values(kk);
-            else if (kk == 0) values(1);
-#pragma unroll
-            for (int d = 0; d < Dim::DB; ++d) {
-#pragma unroll
-                for (int i = 0; i < QB; ++i) o[i][d] = Op::dot_t(vf[kk][d], p[i], o[i][d]);
+                for (int i = 0; i < QB; ++i) p[i] = Op::pack(s[2 * kk][i], s[2 * kk + 1][i]);
+                typename Op::Pair more[QB];
                 if constexpr (sizeof(T) == 2)
 #pragma unroll
-                    for (int i = 0; i < QB; ++i) o[i][d] = Op::dot_t(vf[kk][d], more[i], o[i][d]);
+                    for (int i = 0; i < QB; ++i) more[i] = Op::rest(s[2 * kk][i], s[2 * kk + 1][i], p[i]);
+                if (!Dim::EARLY) values(kk);
+                else if (kk == 0) values(1);
+#pragma unroll
+                for (int d = 0; d < Dim::DB; ++d) {
+#pragma unroll
+                    for (int i = 0; i < QB; ++i) o[i][d] = Op::dot_t(vf[kk][d], p[i], o[i][d]);
+                    if constexpr (sizeof(T) == 2)
+#pragma unroll
+                        for (int i = 0; i < QB; ++i) o[i][d] = Op::dot_t(vf[kk][d], more[i], o[i][d]);
+                }
             }
-        }
         }
     }
 #pragma unroll
@@ -976,110 +977,110 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) vo
         if (idle) continue;
 #pragma unroll 1
         for (int hv = 0; hv < HV; ++hv) {
-        const unsigned long long here = HV == 1 || hv == 0 ? valid[0] : valid[HV - 1];
-        if (here == 0ull) continue;
-        const T *Kh = Ks + hv * RP_TILE * LD, *Vh = Vs + hv * RP_TILE * LD;
-        const int* ckh = ck + hv * RP_TILE;
+            const unsigned long long here = HV == 1 || hv == 0 ? valid[0] : valid[HV - 1];
+            if (here == 0ull) continue;
+            const T *Kh = Ks + hv * RP_TILE * LD, *Vh = Vs + hv * RP_TILE * LD;
+            const int* ckh = ck + hv * RP_TILE;
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            rp_f32x4 s[2][QB], ds[2][QB];   // ds: dP, then dS
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int4 c4 = *reinterpret_cast<const int4*>(ckh + (2 * kk + e) * 16 + g * 4);
-#pragma unroll
-                for (int i = 0; i < QB; ++i) {
-                    s[e][i] = rp_bias4(bw, c4, cq[i]);
-                    ds[e][i] = rp_f32x4{0.f, 0.f, 0.f, 0.f};
-                }
-            }
-#pragma unroll
-            for (int c = 0; c < Dim::NCH; ++c)
+            for (int kk = 0; kk < 2; ++kk) {
+                rp_f32x4 s[2][QB], ds[2][QB];   // ds: dP, then dS
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const int at = ((2 * kk + e) * 16 + l) * LD + c * Op::CHUNK + g * Op::PER;
-                    const typename Op::Frag kf = *reinterpret_cast<const typename Op::Frag*>(Kh + at);
-                    const typename Op::Frag vf = *reinterpret_cast<const typename Op::Frag*>(Vh + at);
+                    const int4 c4 = *reinterpret_cast<const int4*>(ckh + (2 * kk + e) * 16 + g * 4);
 #pragma unroll
                     for (int i = 0; i < QB; ++i) {
-                        s[e][i] = Op::dot(kf, qf[i][c], s[e][i]);
-                        ds[e][i] = Op::dot(vf, gf[i][c], ds[e][i]);
+                        s[e][i] = rp_bias4(bw, c4, cq[i]);
+                        ds[e][i] = rp_f32x4{0.f, 0.f, 0.f, 0.f};
                     }
                 }
-            typename Op::TFrag kt_[Dim::DB];   // requested ahead of the exponentials
-            if constexpr (Dim::EARLY) {
 #pragma unroll
-                for (int d = 0; d < Dim::DB; ++d) {
-                    const T* k0 = Kh + (kk * 32 + g * 4) * LD + d * 16;
-                    kt_[d] = Op::load_t(k0, k0 + 16 * LD, LD, l);
+                for (int c = 0; c < Dim::NCH; ++c)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int at = ((2 * kk + e) * 16 + l) * LD + c * Op::CHUNK + g * Op::PER;
+                        const typename Op::Frag kf = *reinterpret_cast<const typename Op::Frag*>(Kh + at);
+                        const typename Op::Frag vf = *reinterpret_cast<const typename Op::Frag*>(Vh + at);
+#pragma unroll
+                        for (int i = 0; i < QB; ++i) {
+                            s[e][i] = Op::dot(kf, qf[i][c], s[e][i]);
+                            ds[e][i] = Op::dot(vf, gf[i][c], ds[e][i]);
+                        }
+                    }
+                typename Op::TFrag kt_[Dim::DB];   // requested ahead of the exponentials
+                if constexpr (Dim::EARLY) {
+#pragma unroll
+                    for (int d = 0; d < Dim::DB; ++d) {
+                        const T* k0 = Kh + (kk * 32 + g * 4) * LD + d * 16;
+                        kt_[d] = Op::load_t(k0, k0 + 16 * LD, LD, l);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if (here != ~0ull) {
+                if (here != ~0ull) {
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const rp_f32x4 c4 = *reinterpret_cast<const rp_f32x4*>(cap + hv * RP_TILE + (2 * kk + e) * 16 + g * 4);
+                    for (int e = 0; e < 2; ++e) {
+                        const rp_f32x4 c4 = *reinterpret_cast<const rp_f32x4*>(cap + hv * RP_TILE + (2 * kk + e) * 16 + g * 4);
 #pragma unroll
-                    for (int i = 0; i < QB; ++i)
+                        for (int i = 0; i < QB; ++i)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[e][i][r] = fminf(s[e][i][r], c4[r]);
+                            for (int r = 0; r < 4; ++r) s[e][i][r] = fminf(s[e][i][r], c4[r]);
+                    }
                 }
-            }
-            if (a.pdrop > 0.f) {
+                if (a.pdrop > 0.f) {
 #pragma unroll
-                for (int i = 0; i < QB; ++i) {
-                    const unsigned long long at = ((unsigned long long)bh * a.Lq + qi[i]) * a.Lk + t * ST + hv * RP_TILE + kk * 32 + g * 4;
+                    for (int i = 0; i < QB; ++i) {
+                        const unsigned long long at = ((unsigned long long)bh * a.Lq + qi[i]) * a.Lk + t * ST + hv * RP_TILE + kk * 32 + g * 4;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) ds[e][i][r] *= rp_drop(seed, at + e * 16 + r, a.pdrop);
+                    }
+                }
+                if (far) {
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) ds[e][i][r] *= rp_drop(seed, at + e * 16 + r, a.pdrop);
-                }
-            }
-            if (far) {
+                        for (int i = 0; i < QB; ++i)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
+                            for (int r = 0; r < 4; ++r) s[e][i][r] = __builtin_amdgcn_exp2f(fmaf(s[e][i][r] - mx[i], a.sl2, -lg[i]));
+                } else {
 #pragma unroll
-                    for (int i = 0; i < QB; ++i)
+                    for (int e = 0; e < 2; ++e)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) s[e][i][r] = __builtin_amdgcn_exp2f(fmaf(s[e][i][r] - mx[i], a.sl2, -lg[i]));
-            } else {
+                        for (int i = 0; i < QB; ++i)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int i = 0; i < QB; ++i)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) s[e][i][r] = __builtin_amdgcn_exp2f(fmaf(s[e][i][r], a.sl2, -shift[i]));
-            }
-#pragma unroll
-            for (int i = 0; i < QB; ++i) {
-                float part[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) ds[e][i][r] = s[e][i][r] * (ds[e][i][r] - D0[i]);
-                    part[e] = (ds[e][i][0] + ds[e][i][1]) + (ds[e][i][2] + ds[e][i][3]);
-                }
-                extra[i] += part[0] + part[1];
-            }
-            typename Op::Pair p[QB];
-#pragma unroll
-            for (int i = 0; i < QB; ++i) p[i] = Op::pack(ds[0][i], ds[1][i]);
-            typename Op::Pair more[QB];
-            if constexpr (sizeof(T) == 2)
-#pragma unroll
-                for (int i = 0; i < QB; ++i) more[i] = Op::rest(ds[0][i], ds[1][i], p[i]);
-#pragma unroll
-            for (int d = 0; d < Dim::DB; ++d) {
-                if constexpr (!Dim::EARLY) {
-                    const T* k0 = Kh + (kk * 32 + g * 4) * LD + d * 16;
-                    kt_[d] = Op::load_t(k0, k0 + 16 * LD, LD, l);
+                            for (int r = 0; r < 4; ++r) s[e][i][r] = __builtin_amdgcn_exp2f(fmaf(s[e][i][r], a.sl2, -shift[i]));
                 }
 #pragma unroll
-                for (int i = 0; i < QB; ++i) dq[i][d] = Op::dot_t(kt_[d], p[i], dq[i][d]);
+                for (int i = 0; i < QB; ++i) {
+                    float part[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) ds[e][i][r] = s[e][i][r] * (ds[e][i][r] - D0[i]);
+                        part[e] = (ds[e][i][0] + ds[e][i][1]) + (ds[e][i][2] + ds[e][i][3]);
+                    }
+                    extra[i] += part[0] + part[1];
+                }
+                typename Op::Pair p[QB];
+#pragma unroll
+                for (int i = 0; i < QB; ++i) p[i] = Op::pack(ds[0][i], ds[1][i]);
+                typename Op::Pair more[QB];
                 if constexpr (sizeof(T) == 2)
 #pragma unroll
-                    for (int i = 0; i < QB; ++i) dq[i][d] = Op::dot_t(kt_[d], more[i], dq[i][d]);
+                    for (int i = 0; i < QB; ++i) more[i] = Op::rest(ds[0][i], ds[1][i], p[i]);
+#pragma unroll
+                for (int d = 0; d < Dim::DB; ++d) {
+                    if constexpr (!Dim::EARLY) {
+                        const T* k0 = Kh + (kk * 32 + g * 4) * LD + d * 16;
+                        kt_[d] = Op::load_t(k0, k0 + 16 * LD, LD, l);
+                    }
+#pragma unroll
+                    for (int i = 0; i < QB; ++i) dq[i][d] = Op::dot_t(kt_[d], p[i], dq[i][d]);
+                    if constexpr (sizeof(T) == 2)
+#pragma unroll
+                        for (int i = 0; i < QB; ++i) dq[i][d] = Op::dot_t(kt_[d], more[i], dq[i][d]);
+                }
             }
-        }
         }
     }
 #pragma unroll
