@@ -14,8 +14,8 @@
 // softmax runs down registers plus two lane exchanges, and the four values are already the B operand of O^T = V^T P^T (V^T
 // read from the row-major tile by the transposing LDS read). fp32 runs the same code on 16x16x4. No L x L array exists in
 // memory; the backward recomputes P from the row statistics, once with queries as columns (dQ) and once with keys as
-// columns (dK, dV, dtable). P and dS become bf16 only as operands of bf16 products (two numbers each for O and dQ);
-// statistics, D and the bias gradient stay fp32.
+// columns (dK, dV, dtable). P and dS become bf16 only as operands of bf16 products, as two numbers each (what the first
+// rounding took off is the second); statistics, D and the bias gradient stay fp32.
 //
 // D is needed to fp32 accuracy because the rows of dS sum to zero and a bucket's gradient is what is left of many terms. The
 // output a bf16 caller holds is too coarse for it: the forward keeps what its rounding took off beside it, the dQ kernel starts from
@@ -866,8 +866,8 @@ __global__ __launch_bounds__(256) void relpos_join_kernel(RpArgs a) {
 // inexact D~, does to it. dS is therefore multiplied as two bf16 numbers, its rounding and what that took off, and the forward
 // does the same with P (38x38 maps, batch 4, 8 heads of 64: 52 -> 57 us, forward 45 -> 49; 75x75, 4 heads of 32: 74 -> 87,
 // forward 71 -> 86). The error of dQ is then that of its own last rounding, 1.7e-3; with single roundings it was 2.4e-3 for keys
-// with nothing in common, 5.6e-3 for keys of mean 4 and deviation 1. dK and dV are sums over queries with no such
-// cancellation and take P and dS rounded once: 2.4e-3 (1.7e-3 for 103 -> 109 us with both split).
+// with nothing in common, 5.6e-3 for keys of mean 4 and deviation 1. dK and dV are sums over queries that cancel too, by
+// chance: their products take P and dS as two numbers as well (2.4e-3 -> 1.7e-3 for 103 -> 109 us).
 // ------------------------------------------------------------------------------------------------
 template <typename T, int DP, int QB>
 __global__ __launch_bounds__(256, rp_waves(RP_BWD_Q, sizeof(T) == 2, DP, QB)) void relpos_bwd_q_kernel(RpArgs a) {
@@ -1355,11 +1355,15 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
 #pragma unroll
                         for (int r = 0; r < 4; ++r) p[e][j][r] = (kept >> ((e * KB + j) * 4 + r)) & 1 ? p[e][j][r] * up : 0.f;
             }
-            typename Op::Pair pp[KB], pd[KB];
+            typename Op::Pair pp[KB], pd[KB], pp2[KB], pd2[KB];
 #pragma unroll
             for (int j = 0; j < KB; ++j) {
                 pp[j] = Op::pack(p[0][j], p[1][j]);
                 pd[j] = Op::pack(ds[0][j], ds[1][j]);
+                if constexpr (sizeof(T) == 2) {
+                    pp2[j] = Op::rest(p[0][j], p[1][j], pp[j]);
+                    pd2[j] = Op::rest(ds[0][j], ds[1][j], pd[j]);
+                }
             }
             const int trow = g * (16 * LD + INS) + kk * 8 * LD;
 #pragma unroll
@@ -1371,6 +1375,12 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
                     dk[j][d] = Op::dot_t(qa, pd[j], dk[j][d]);
                     dv[j][d] = Op::dot_t(ga, pp[j], dv[j][d]);
                 }
+                if constexpr (sizeof(T) == 2)
+#pragma unroll
+                    for (int j = 0; j < KB; ++j) {
+                        dk[j][d] = Op::dot_t(qa, pd2[j], dk[j][d]);
+                        dv[j][d] = Op::dot_t(ga, pp2[j], dv[j][d]);
+                    }
             }
         }
     }

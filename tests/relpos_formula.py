@@ -2,11 +2,13 @@
 
 Bounds. fp32: every product or sum of n terms is off by at most n 2^-24 of its largest magnitude; a score of at most ~16 in
 size from D products, its exponential, and a sum over L terms give `c32 = 8 (D + 64) + L` roundings of 2^-24 relative to
-the largest output. bf16 inputs are exact. P for dV and dS for dK are rounded once (half a step, 2^-8 of each) as matrix
-operands, P for out and dS for dQ to two numbers (2^-16 of each is left), results once; dQ starts from row sums D of an output kept
+the largest output. bf16 inputs are exact. `dv` and `dk` allow for P and dS rounded once (half a step, 2^-8 of each) as matrix
+operands, `out` and `dq` to two numbers (2^-16 of each is left), results are rounded once; dQ starts from row sums D of an output kept
 to 2^-16 of its terms:
   out: 2^-16 P |v| + 2^-8 |out|          dV: 2^-8 (P^T |dO| + |dV|)
   dK:  2^-8 (scale |dS|^T |q| + |dK|)    dQ: 2^-16 scale |dS| |k| + 2^-8 |dQ| + scale 2^-16 (|dO| . (|out| + P |v|)) (P |k|)
+dV and dK of weights held as two numbers have 2^-8 of their first term again, `dv_split` and `dk_split`:
+  dV: 2^-8 (2^-8 P^T |dO| + |dV|)        dK: 2^-8 (2^-8 scale |dS|^T |q| + |dK|)
 The table's gradient is fp32 in both: c32 2^-24 times the sum of |dS| of its bucket."""
 import numpy as np
 import torch
@@ -76,6 +78,9 @@ def formula(q, k, v, table, plan, mask=None, scale=None, q_start=0, dout=None, d
     tol["dv"] = back((H * (pd.transpose(2, 3) @ do.abs() + dv.abs()) if half else 0.0) + eq * (1e-30 + (pd.transpose(2, 3) @ do.abs()).max()) * one(dv))
     kk, qq = scale * size @ k.abs(), scale * size.transpose(2, 3) @ q.abs()
     tol["dk"] = back((H * (scale * ds.abs().transpose(2, 3) @ q.abs() + dk.abs()) if half else 0.0) + eq * (1e-30 + qq.max()) * one(dk))
+    vo, ko = pd.transpose(2, 3) @ do.abs(), scale * ds.abs().transpose(2, 3) @ q.abs()
+    tol["dv_split"] = back((H * (H * vo + dv.abs()) if half else 0.0) + eq * (1e-30 + vo.max()) * one(dv))
+    tol["dk_split"] = back((H * (H * ko + dk.abs()) if half else 0.0) + eq * (1e-30 + qq.max()) * one(dk))
     slack = (do.abs() * (out.abs() + pv)).sum(-1, keepdim=True) * (p @ k.abs()) * scale
     tol["dq"] = back((H * (H * scale * ds.abs() @ k.abs() + dq.abs() + H * slack * (1 + H)) if half else 0.0) + eq * (1e-30 + kk.max()) * one(dq))
     dt, da = torch.zeros(plan.num_buckets, heads, dtype=torch.float64), torch.zeros(plan.num_buckets, heads, dtype=torch.float64)

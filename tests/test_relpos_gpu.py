@@ -378,3 +378,16 @@ def test_repeatable_streams_and_capture():
         eager = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(static, eager)), n
+
+
+@pytest.mark.parametrize("height,width,B,D,drop", [(10, 10, 8, 48, 0.0), (10, 10, 3, 16, 0.2), (1, 300, 2, 32, 0.0), (17, 19, 2, 64, 0.0), (9, 11, 4, 128, 0.0)])
+def test_key_gradients_hold_the_weights_twice(height, width, B, D, drop):
+    """bf16: dK and dV carry no rounding of P and dS beyond their own last one, where a sum over many queries nearly cancels too."""
+    plan = RelativePositionBuckets(height, width, 8, 16)
+    n = height * width
+    q, k, v, table, dout = _inputs(B, n, n, 4, D, BF16, plan.num_buckets, 21)
+    mine = [t.cuda().requires_grad_() for t in (q, k, v, table)]
+    want, tol = formula(q, k, v, table, plan, dout=dout, drop=dropout_factors(1234, (B, 4, n, n), drop) if drop else None)
+    grads = torch.autograd.grad(relpos_attention(*mine, plan, dropout_p=drop, seed=1234), mine, dout.cuda())
+    _compare(grads[1], want["dk"], tol["dk_split"], "dk")
+    _compare(grads[2], want["dv"], tol["dv_split"], "dv")
