@@ -59,6 +59,15 @@ void first_derivative_only(const char* name) {
     TORCH_CHECK(!c10::GradMode::is_enabled(), name, " has no second derivative (create_graph=True)");
 }
 
+// A saved tensor as it comes back. Hooks may return the values in another layout (save_on_cpu does so for a view that is not
+// dense), so nothing about addresses, strides or alignment is taken over from the forward; shape, type and device have to be the same.
+Tensor restored(const Tensor& t, at::IntArrayRef shape, at::ScalarType type, at::Device device, const char* name) {
+    TORCH_CHECK(t.defined() && t.sizes() == shape && t.scalar_type() == type && t.device() == device && t.layout() == at::kStrided, name,
+                ": a saved tensor came back from its hooks as ", t.defined() ? c10::str(t.scalar_type(), t.sizes(), " on ", t.device()) : "nothing",
+                " (was ", type, shape, " on ", device, ")");
+    return t;
+}
+
 // ------------------------------------------------------------------------------------------------
 // attention with a relative position bias
 // ------------------------------------------------------------------------------------------------
@@ -67,8 +76,12 @@ struct Attention {
     float scale, pdrop;
     unsigned long long seed;
     const unsigned long long* seed_offset;
-    long long strides[9];
+    at::ScalarType type, mask_type;
+    at::Device device = at::kCPU;
     bool packed, empty;
+
+    std::vector<int64_t> query_shape() const { return packed ? std::vector<int64_t>{B, Lq, 3, heads, D} : std::vector<int64_t>{B, Lq, heads, D}; }
+    std::vector<int64_t> key_shape() const { return {B, Lk, heads, D}; }
 };
 
 // (batch, token, head) strides in elements; one of a dimension of length one does not matter
@@ -102,6 +115,8 @@ struct RelPosAttentionBackward : torch::autograd::Node {
     SavedVariable q, k, v, bias, mask, out, low, stat;
     Tensor order, start;
     std::array<int64_t, 2> table;
+    int64_t offsets;
+    bool masked;
 
     std::string name() const override { return "RelPosAttentionBackward"; }
     void release_variables() override {
@@ -113,30 +128,41 @@ struct RelPosAttentionBackward : torch::autograd::Node {
         first_derivative_only("relpos_attention");
         variable_list got(4);
         if (!grads[0].defined()) return got;
-        const Tensor q_ = q.unpack(), k_ = k.unpack(), v_ = v.unpack();
-        const c10::DeviceGuard guard(q_.device());
-        const auto f32 = q_.options().dtype(at::kFloat);
+        const c10::DeviceGuard guard(a.device);
+        const auto options = at::TensorOptions().device(a.device).dtype(a.type), f32 = options.dtype(at::kFloat);
+        const auto query_shape = a.query_shape(), key_shape = a.key_shape();
         const bool want = task_should_compute_output(3);
         if (a.empty) {
-            got[0] = at::zeros_like(q_);
-            if (!a.packed) got[1] = at::zeros_like(k_), got[2] = at::zeros_like(v_);
+            got[0] = at::zeros(query_shape, options);
+            if (!a.packed) got[1] = at::zeros(key_shape, options), got[2] = at::zeros(key_shape, options);
             if (want) got[3] = at::zeros(table, f32);
             return got;
         }
-        const Tensor bias_ = bias.unpack(), mask_ = mask.unpack(), out_ = out.unpack(shared_from_this()), low_ = low.unpack(), stat_ = stat.unpack();
+        const auto back = [this](const Tensor& t, at::IntArrayRef shape, at::ScalarType type) {
+            return restored(t, shape, type, a.device, "relpos_attention");
+        };
+        const std::array<int64_t, 4> rows = {a.B, a.Lq, a.heads, a.D};
+        Tensor q_ = back(q.unpack(), query_shape, a.type), k_ = k.unpack(), v_ = v.unpack(), mask_ = mask.unpack(), low_ = low.unpack();
+        const Tensor bias_ = dense(back(bias.unpack(), {a.heads, offsets}, at::kFloat));
+        const Tensor stat_ = dense_aligned(back(stat.unpack(), {a.B, a.heads, a.Lq, 2}, at::kFloat));
+        const Tensor out_ = dense_aligned(back(out.unpack(shared_from_this()), rows, a.type));
+        if (a.type == at::kBFloat16) low_ = dense_aligned(back(low_, rows, a.type));
+        if (masked) mask_ = dense(back(mask_, {a.B, a.Lk}, a.mask_type));
         const Tensor dout = dense_aligned(grads[0]);
         const char* in[3];
         char* grad[3];
-        long long gst[9], unused[9];
-        got[0] = at::empty(q_.sizes(), q_.options());
+        long long strides[9], gst[9];
+        got[0] = at::empty(query_shape, options);
         if (a.packed) {
-            packed_rows(q_, in, unused);
+            q_ = dense_aligned(q_);
+            packed_rows(q_, in, strides);
             const char* at[3];
             packed_rows(got[0], at, gst);
             for (int i = 0; i < 3; ++i) grad[i] = const_cast<char*>(at[i]);
         } else {
-            got[1] = at::empty(k_.sizes(), k_.options());
-            got[2] = at::empty(v_.sizes(), v_.options());
+            got[1] = at::empty(key_shape, options);
+            got[2] = at::empty(key_shape, options);
+            q_ = readable(q_, strides), k_ = readable(back(k_, key_shape, a.type), strides + 3), v_ = readable(back(v_, key_shape, a.type), strides + 6);
             const Tensor* of[3] = {&q_, &k_, &v_};
             for (int i = 0; i < 3; ++i) {
                 in[i] = static_cast<const char*>(of[i]->const_data_ptr());
@@ -148,7 +174,7 @@ struct RelPosAttentionBackward : torch::autograd::Node {
         const int dt = dtype_of(q_);
         const long long n = mia_relpos_bwd_ws_floats(dt, a.B, a.heads, a.Lq, a.Lk, a.D, a.height, a.width, want);
         Tensor ws = at::empty({n}, f32);
-        check(mia_relpos_bwd(dt, in[0], in[1], in[2], a.strides, dout.const_data_ptr(), out_.const_data_ptr(), cptr(low_), cfloats(stat_), a.B,
+        check(mia_relpos_bwd(dt, in[0], in[1], in[2], strides, dout.const_data_ptr(), out_.const_data_ptr(), cptr(low_), cfloats(stat_), a.B,
                              a.heads, a.Lq, a.Lk, a.D, cfloats(bias_), a.height, a.width, a.q_start, static_cast<const uint8_t*>(cptr(mask_)), a.scale,
                              a.pdrop, a.seed, a.seed_offset, static_cast<const int*>(cptr(order)), static_cast<const int*>(cptr(start)), a.buckets,
                              floats(ws), n, grad[0], grad[1], grad[2], gst, floats(got[3]), stream_of(q_)),
@@ -176,6 +202,7 @@ Tensor relpos(Tensor q, const Maybe& k_in, const Maybe& v_in, const Tensor& tabl
         a.height = height, a.width = width, a.buckets = buckets, a.q_start = q_start;
         a.scale = (float)scale, a.pdrop = (float)pdrop, a.seed = seed;
         a.seed_offset = reinterpret_cast<const unsigned long long*>(seed_offset);
+        a.type = q.scalar_type(), a.device = q.device();
         a.empty = a.B == 0 || a.Lq == 0 || a.Lk == 0 || a.heads == 0;
         const auto f32 = q.options().dtype(at::kFloat);
         const std::array<int64_t, 4> rows = {a.B, a.Lq, a.heads, a.D};
@@ -184,11 +211,12 @@ Tensor relpos(Tensor q, const Maybe& k_in, const Maybe& v_in, const Tensor& tabl
             out = at::zeros(rows, q.options());
         } else {
             const char* in[3];
+            long long strides[9];
             if (a.packed) {
                 q = dense_aligned(q);
-                packed_rows(q, in, a.strides);
+                packed_rows(q, in, strides);
             } else {
-                q = readable(q, a.strides), k = readable(k, a.strides + 3), v = readable(v, a.strides + 6);
+                q = readable(q, strides), k = readable(k, strides + 3), v = readable(v, strides + 6);
                 const Tensor* of[3] = {&q, &k, &v};
                 for (int i = 0; i < 3; ++i) in[i] = static_cast<const char*>(of[i]->const_data_ptr());
             }
@@ -205,13 +233,14 @@ Tensor relpos(Tensor q, const Maybe& k_in, const Maybe& v_in, const Tensor& tabl
             Tensor ws = n ? at::empty({n}, f32) : Tensor();
             void* stream = stream_of(q);
             check(mia_relpos_bias(cfloats(table), static_cast<const int*>(cptr(index)), height, width, a.heads, a.scale, floats(bias), stream), "mia_relpos_bias");
-            check(mia_relpos_fwd(dt, in[0], in[1], in[2], a.strides, a.B, a.heads, a.Lq, a.Lk, a.D, floats(bias), height, width, q_start,
+            check(mia_relpos_fwd(dt, in[0], in[1], in[2], strides, a.B, a.heads, a.Lq, a.Lk, a.D, floats(bias), height, width, q_start,
                                  static_cast<const uint8_t*>(cptr(mask)), a.scale, a.pdrop, seed, a.seed_offset, floats(ws), n, ptr(out), ptr(low),
                                  floats(stat), stream),
                   "mia_relpos_fwd");
         }
         if (node) {
-            node->a = a;
+            a.mask_type = mask.defined() ? mask.scalar_type() : at::kBool;
+            node->a = a, node->offsets = index.numel(), node->masked = mask.defined();
             node->order = order, node->start = start;
             node->table = {table_in.size(0), table_in.size(1)};
             node->q = SavedVariable(q, false), node->k = SavedVariable(k, false), node->v = SavedVariable(v, false);
@@ -231,6 +260,10 @@ Tensor relpos(Tensor q, const Maybe& k_in, const Maybe& v_in, const Tensor& tabl
 // ------------------------------------------------------------------------------------------------
 struct GatedResidualNormBackward : torch::autograd::Node {
     SavedVariable x, f, stats, parameter[6];   // scale, gate, w1, b1, w2, b2
+    bool has[6];
+    at::ScalarType type;
+    at::Device device = at::kCPU;
+    std::vector<int64_t> shape;
     int images, C, post, pre;
     long long rows;   // of an image
 
@@ -246,17 +279,23 @@ struct GatedResidualNormBackward : torch::autograd::Node {
         variable_list got(8);
         Tensor dy = grads[0], dz = pre ? grads[1] : Tensor();
         if (!dy.defined() && !dz.defined()) return got;
-        const Tensor x_ = x.unpack(), f_ = f.unpack(), stats_ = stats.unpack();
-        Tensor p[6];
-        for (int i = 0; i < 6; ++i) p[i] = parameter[i].unpack();
-        const c10::DeviceGuard guard(x_.device());
-        got[0] = at::empty_like(x_), got[1] = at::empty_like(f_);
+        const c10::DeviceGuard guard(device);
+        const auto options = at::TensorOptions().device(device).dtype(type), f32 = options.dtype(at::kFloat);
+        const auto back = [this](const Tensor& t, at::IntArrayRef of, at::ScalarType as) { return restored(t, of, as, device, "gated_residual_norm"); };
+        const std::vector<int64_t> gate = {images, C}, vector = {C};
+        got[0] = at::empty(shape, options), got[1] = at::empty(shape, options);
         for (int i = 0; i < 6; ++i)
-            if (p[i].defined() && task_should_compute_output(2 + i)) got[2 + i] = rows ? at::empty_like(p[i]) : at::zeros_like(p[i]);
+            if (has[i] && task_should_compute_output(2 + i)) got[2 + i] = rows ? at::empty(i == 1 ? gate : vector, f32) : at::zeros(i == 1 ? gate : vector, f32);
         if (!rows) return got;
+        // aligned, so that the layout of the rows (and with it the order of the sums) does not hang on a hook
+        const Tensor x_ = dense_aligned(back(x.unpack(), shape, type)), f_ = dense_aligned(back(f.unpack(), shape, type));
+        const Tensor stats_ = dense_aligned(back(stats.unpack(), {images * rows, 4}, at::kFloat));
+        Tensor p[6];
+        for (int i = 0; i < 6; ++i)
+            if (has[i]) p[i] = dense_aligned(back(parameter[i].unpack(), i == 1 ? gate : vector, at::kFloat));
         dy = dense(dy), dz = dense(dz);
         const long long n = mia_blocknorm_ws_floats(images, rows, C, p[1].defined());
-        Tensor ws = at::empty({n}, x_.options().dtype(at::kFloat));
+        Tensor ws = at::empty({n}, f32);
         check(mia_blocknorm_bwd(dtype_of(x_), cptr(dy), cptr(dz), cptr(x_), cptr(f_), cfloats(stats_), images, rows, C, cfloats(p[0]), cfloats(p[1]),
                                 post, cfloats(p[2]), cfloats(p[3]), pre, cfloats(p[4]), floats(ws), n, ptr(got[0]), ptr(got[1]), floats(got[2]),
                                 floats(got[3]), floats(got[4]), floats(got[5]), floats(got[6]), floats(got[7]), stream_of(x_)),
@@ -291,8 +330,9 @@ std::tuple<Tensor, Maybe> residual(const Tensor& x_in, const Tensor& f_in, const
                   "mia_blocknorm_fwd");
         if (node) {
             node->images = images, node->rows = rows, node->C = C, node->post = post, node->pre = pre;
+            node->type = x.scalar_type(), node->device = x.device(), node->shape = x.sizes().vec();
             node->x = SavedVariable(x, false), node->f = SavedVariable(f, false), node->stats = SavedVariable(stats, false);
-            for (int i = 0; i < 6; ++i) node->parameter[i] = SavedVariable(p[i], false);
+            for (int i = 0; i < 6; ++i) node->parameter[i] = SavedVariable(p[i], false), node->has[i] = p[i].defined();
         }
     }
     if (node) {

@@ -252,3 +252,67 @@ def test_two_threads_backward():
     for t in threads:
         t.join()
     assert all(torch.equal(a, b) for i in range(2) for a, b in zip(want, got[i]))
+
+
+def _elsewhere(kind):
+    """Saved-tensor hooks that bring the same values back in another layout."""
+    def strided(t):
+        return torch.stack((t, t), -1)[..., 0]
+
+    def unaligned(t):
+        flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view(t.shape)
+
+    def reversed_dims(t):
+        return t.permute(*reversed(range(t.dim()))).contiguous().permute(*reversed(range(t.dim())))
+    if kind in ("cpu", "pinned"):
+        return torch.autograd.graph.save_on_cpu(pin_memory=kind == "pinned")
+    return torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), {"strided": strided, "unaligned": unaligned, "reversed": reversed_dims}[kind])
+
+
+@pytest.mark.parametrize("kind", ["cpu", "pinned", "strided", "unaligned", "reversed"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_saved_tensors_come_back_in_another_layout(dtype, kind):
+    """Views that the kernels read in place (slices of a packed projection, heads first) and every other saved tensor: what a hook
+    returns is read as it lies, not as the forward's tensors lay."""
+    from mia_amd.block_norm import gated_residual_norm
+    from mia_amd.relpos import RelativePositionBuckets, relpos_attention, relpos_self_attention
+    plan = RelativePositionBuckets(5, 9, 8, 16)
+    g = torch.Generator().manual_seed(31)
+    qkv = torch.randn(2, 45, 3, 4, 16, generator=g).to(dtype).cuda().requires_grad_()
+    table = torch.randn(64, 4, generator=g).cuda().requires_grad_()
+    mask = (torch.rand(2, 45, generator=g) < 0.7).cuda()
+    w, s, b = (torch.randn(64, generator=g).cuda().requires_grad_() for _ in range(3))
+    gate = torch.rand(2, 64, generator=g).cuda().requires_grad_()
+    dout = torch.randn(2, 45, 4, 16, generator=g).to(dtype).cuda()
+
+    def sliced():
+        return relpos_attention(*qkv.unbind(2), table, plan, key_mask=mask)
+
+    def heads_first():
+        return relpos_attention(*(t.transpose(1, 2).contiguous().transpose(1, 2) for t in qkv.unbind(2)), table, plan, key_mask=mask)
+
+    def packed():
+        return relpos_self_attention(qkv, table, plan, key_mask=mask)
+
+    def norm():
+        y, z = gated_residual_norm(qkv[:, :, 0].reshape(2, 45, 64), qkv[:, :, 1].reshape(2, 45, 64), scale=s, gate=gate, post="layer", post_weight=w,
+                                   post_bias=b, pre="rms", pre_weight=w)
+        return (y + z).view(2, 45, 4, 16)
+    for run, leaves in ((sliced, (qkv, table)), (heads_first, (qkv, table)), (packed, (qkv, table)), (norm, (qkv, w, s, b, gate))):
+        want = torch.autograd.grad(run(), leaves, dout)
+        with _elsewhere(kind):
+            out = run()
+        got = torch.autograd.grad(out, leaves, dout)
+        assert all(torch.equal(a, c) for a, c in zip(want, got)), run.__name__
+
+
+def test_saved_tensors_that_come_back_wrong_are_refused():
+    run, x, leaves = _block(torch.float32)
+    dout = torch.randn(3, 35, 64, device="cuda")
+    for unpack in (lambda t: t.bfloat16(), lambda t: t.cpu(), lambda t: t[:1], lambda t: t.reshape(-1)[:1]):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            out = run(x)
+        with pytest.raises(RuntimeError, match="came back from its hooks"):
+            torch.autograd.grad(out, leaves, dout)
