@@ -59,6 +59,12 @@ void first_derivative_only(const char* name) {
     TORCH_CHECK(!c10::GradMode::is_enabled(), name, " has no second derivative (create_graph=True)");
 }
 
+// The kernels see values alone: a result would be a constant to forward-mode differentiation.
+template <typename... T>
+void no_tangents(const char* name, const T&... t) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!((t.defined() && t._fw_grad(/*level=*/0).defined()) || ...), name, " has no forward-mode derivative");
+}
+
 // A saved tensor as it comes back. Hooks may return the values in another layout (save_on_cpu does so for a view that is not
 // dense), so nothing about addresses, strides or alignment is taken over from the forward; shape, type and device have to be the same.
 Tensor restored(const Tensor& t, at::IntArrayRef shape, at::ScalarType type, at::Device device, const char* name) {
@@ -188,6 +194,7 @@ Tensor relpos(Tensor q, const Maybe& k_in, const Maybe& v_in, const Tensor& tabl
               const Maybe& mask_in, int height, int width, int buckets, double scale, int q_start, double pdrop, unsigned long long seed,
               unsigned long long seed_offset) {
     Tensor k = or_none(k_in), v = or_none(v_in), mask = or_none(mask_in), out;
+    no_tangents("relpos_attention", q, k, v, table_in);
     std::shared_ptr<RelPosAttentionBackward> node;
     if (recorded(q, k, v, table_in)) {
         node = std::shared_ptr<RelPosAttentionBackward>(new RelPosAttentionBackward(), torch::autograd::deleteNode);
@@ -309,6 +316,7 @@ std::tuple<Tensor, Maybe> residual(const Tensor& x_in, const Tensor& f_in, const
     const Maybe* maybe[6] = {&scale, &gate, &w1, &b1, &w2, &b2};
     Tensor p[6], y, z;
     for (int i = 0; i < 6; ++i) p[i] = or_none(*maybe[i]);
+    no_tangents("gated_residual_norm", x_in, f_in, p[0], p[1], p[2], p[3], p[4], p[5]);
     std::shared_ptr<GatedResidualNormBackward> node;
     if (recorded(x_in, f_in, p[0], p[1], p[2], p[3], p[4], p[5])) {
         node = std::shared_ptr<GatedResidualNormBackward>(new GatedResidualNormBackward(), torch::autograd::deleteNode);
@@ -360,6 +368,7 @@ struct GradTable {
 
     explicit GradTable(const std::vector<Tensor>& grads) {
         for (const Tensor& g : grads) {
+            no_tangents("gradient norm and clipping", g);
             if (!g.is_cuda() || g.device() != grads[0].device())
                 throw std::runtime_error("gradient norm and clipping need their tensors on one MI355X device; there is no CPU path");
             if (g.scalar_type() != at::kFloat && g.scalar_type() != at::kBFloat16)

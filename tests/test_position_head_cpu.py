@@ -80,3 +80,26 @@ def test_plan_of_a_map(height, width):
     n = height * width
     bucket = plan.index.long()[offsets(height, width, n, n, 0)]
     assert torch.equal(ref.relative_position_table[bucket].permute(2, 0, 1), ref.bias(height, width))
+
+
+def _node_calls(shape=(1, 4, 2, 8)):
+    """The operators' C++ entry points on host tensors, past the wrappers' checks: what is refused is refused before any work. Each call
+    takes the tensor that stands in its first place; `others` are its further differentiable places."""
+    import torch
+    from mia_amd._lib import nodes
+    t, index = torch.zeros(shape), torch.zeros(7, dtype=torch.int32)
+    table, w = torch.zeros(3, 2), torch.ones(8)
+    attend = lambda q=t, k=t, v=t, tab=table: nodes().relpos(q, k, v, tab, index, index, index, None, 1, 4, 3, 0.35, 0, 0.0, 0, 0)     # noqa: E731
+    norm = lambda x=t, f=t, s=None, w2=w: nodes().residual(x, f, s, None, None, None, w2, None, 0, 1, 1e-6)        # noqa: E731
+    return [(attend, "q", t), (attend, "k", t), (attend, "v", t), (attend, "tab", table), (norm, "x", t), (norm, "f", t), (norm, "s", w), (norm, "w2", w),
+            (lambda g=t: nodes().grad_norm([g]), "g", t), (lambda g=t: nodes().grad_clip([g], 1.0), "g", t)]
+
+
+@pytest.mark.parametrize("which", range(10))
+def test_forward_mode_is_refused(which):
+    import torch
+    from torch.autograd import forward_ad
+    call, place, t = _node_calls()[which]
+    with forward_ad.dual_level():
+        with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+            call(**{place: forward_ad.make_dual(t, torch.ones_like(t))})

@@ -316,3 +316,20 @@ def test_saved_tensors_that_come_back_wrong_are_refused():
             out = run(x)
         with pytest.raises(RuntimeError, match="came back from its hooks"):
             torch.autograd.grad(out, leaves, dout)
+
+
+def test_forward_mode_is_refused():
+    """A tangent would be lost; tensors without one are taken inside a dual level."""
+    from torch.autograd import forward_ad
+    from mia_amd.optim import clip_grads_, grad_norm
+    run, x, leaves = _block(torch.float32)
+    want = run(x)
+    g = torch.randn(10, device="cuda")
+    with forward_ad.dual_level():
+        assert torch.equal(run(x), want)
+        dual = forward_ad.make_dual(x.detach(), torch.ones_like(x))
+        for call in (lambda: run(dual), lambda: grad_norm([g, forward_ad.make_dual(g, g)]), lambda: clip_grads_([forward_ad.make_dual(g, g)], 1.0)):
+            with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
+                call()
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(run, (x.detach(),), (torch.ones_like(x),))
