@@ -8,6 +8,7 @@
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -15,6 +16,7 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 
 #include "../../include/mia_hip.h"
@@ -63,6 +65,12 @@ void first_derivative_only(const char* name) {
 template <typename... T>
 void no_tangents(const char* name, const T&... t) {
     TORCH_CHECK_NOT_IMPLEMENTED(!((t.defined() && t._fw_grad(/*level=*/0).defined()) || ...), name, " has no forward-mode derivative");
+}
+
+// A tracer sees the allocation of a result and not the kernels that fill it: its program would return memory as it was.
+void not_traced(const char* name) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY), name,
+                " cannot be traced (torch.jit.trace, make_fx, torch.export): its kernels would be missing from the program");
 }
 
 // A saved tensor as it comes back. Hooks may return the values in another layout (save_on_cpu does so for a view that is not
@@ -194,6 +202,7 @@ Tensor relpos(Tensor q, const Maybe& k_in, const Maybe& v_in, const Tensor& tabl
               const Maybe& mask_in, int height, int width, int buckets, double scale, int q_start, double pdrop, unsigned long long seed,
               unsigned long long seed_offset) {
     Tensor k = or_none(k_in), v = or_none(v_in), mask = or_none(mask_in), out;
+    not_traced("relpos_attention");
     no_tangents("relpos_attention", q, k, v, table_in);
     std::shared_ptr<RelPosAttentionBackward> node;
     if (recorded(q, k, v, table_in)) {
@@ -316,6 +325,7 @@ std::tuple<Tensor, Maybe> residual(const Tensor& x_in, const Tensor& f_in, const
     const Maybe* maybe[6] = {&scale, &gate, &w1, &b1, &w2, &b2};
     Tensor p[6], y, z;
     for (int i = 0; i < 6; ++i) p[i] = or_none(*maybe[i]);
+    not_traced("gated_residual_norm");
     no_tangents("gated_residual_norm", x_in, f_in, p[0], p[1], p[2], p[3], p[4], p[5]);
     std::shared_ptr<GatedResidualNormBackward> node;
     if (recorded(x_in, f_in, p[0], p[1], p[2], p[3], p[4], p[5])) {
@@ -367,6 +377,7 @@ struct GradTable {
     Tensor ws, out;   // out: norm and factor
 
     explicit GradTable(const std::vector<Tensor>& grads) {
+        not_traced("gradient norm and clipping");
         for (const Tensor& g : grads) {
             no_tangents("gradient norm and clipping", g);
             if (!g.is_cuda() || g.device() != grads[0].device())

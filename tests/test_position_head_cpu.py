@@ -103,3 +103,19 @@ def test_forward_mode_is_refused(which):
     with forward_ad.dual_level():
         with pytest.raises(NotImplementedError, match="no forward-mode derivative"):
             call(**{place: forward_ad.make_dual(t, torch.ones_like(t))})
+
+
+@pytest.mark.parametrize("which", [0, 4, 8, 9])
+def test_tracing_is_refused(which):
+    """A traced program would hold the allocation of the results and none of the kernels."""
+    import torch
+    from torch.fx.experimental.proxy_tensor import make_fx
+    call, place, t = _node_calls()[which]
+
+    def function(x):
+        out = call(**{place: x})
+        return out[0] if isinstance(out, tuple) else out
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(function, (t,), check_trace=False)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        make_fx(function)(t)

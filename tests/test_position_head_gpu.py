@@ -333,3 +333,18 @@ def test_forward_mode_is_refused():
                 call()
     with pytest.raises(RuntimeError):
         torch.func.jvp(run, (x.detach(),), (torch.ones_like(x),))
+
+
+def test_tracing_is_refused():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from mia_amd.block_norm import gated_residual_norm
+    from mia_amd.optim import clip_grads_
+    from mia_amd.relpos import RelativePositionBuckets, relpos_self_attention
+    plan = RelativePositionBuckets(2, 3, 8, 16)
+    table, w = torch.zeros(64, 2, device="cuda"), torch.ones(8, device="cuda")
+    x = torch.randn(1, 6, 3, 2, 8, device="cuda")
+    for function in (lambda t: relpos_self_attention(t, table, plan), lambda t: gated_residual_norm(t, t, pre_weight=w)[1], lambda t: clip_grads_([t], 1.0)):
+        for trace in (lambda f: torch.jit.trace(f, (x,), check_trace=False), lambda f: make_fx(f)(x)):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                trace(function)
+        assert bool(torch.isfinite(function(x)).all())
