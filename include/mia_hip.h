@@ -250,6 +250,10 @@ int mia_relpos_bwd(int dtype, const void* q, const void* k, const void* v, const
                    long long ws_floats, void* dq, void* dk, void* dv, const long long* grad_strides, float* dtable,
                    void* stream);
 long long mia_relpos_bwd_ws_floats(int dtype, int B, int heads, int Lq, int Lk, int D, int height, int width, int want_bias);
+/* How the kernels of one direction (0 forward, 1 query gradients, 2 key and value gradients) are laid out over a problem, in plan[3]:
+ * 16-wide columns of a wave (0: the forward of few queries), ranges that the walked tokens are split into, and heads of a workgroup
+ * of the forward of few queries (else 0). For tests and sizing: the calls above follow it by themselves. */
+int mia_relpos_plan(int direction, int dtype, int B, int heads, int Lq, int Lk, int D, int* plan);
 
 /* ---- classifier front end: AdaptiveAvgPool2d(1) -> Flatten -> [LayerNorm] -> Dropout (model.py:134-137, :309-311)
  * in_part [B][S][C]: per-image channel sums over H*W (mia_img_colsum). gamma/beta NULL = no LayerNorm. */

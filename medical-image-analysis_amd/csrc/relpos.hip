@@ -1572,6 +1572,16 @@ static RpPlan rp_plan(int what, int dtype, int B, int heads, int Lq, int Lk, int
     return p;
 }
 
+extern "C" int mia_relpos_plan(int direction, int dtype, int B, int heads, int Lq, int Lk, int D, int* plan) {
+    MIA_CHECK_ARG(plan && direction >= RP_FWD && direction <= RP_BWD_KV && (dtype == MIA_F32 || dtype == MIA_BF16), "mia_relpos_plan: bad arguments");
+    MIA_CHECK_ARG(B > 0 && heads > 0 && Lq > 0 && Lk > 0 && D > 0 && D % 8 == 0 && D <= 128, "mia_relpos_plan: bad shape");
+    const RpPlan p = rp_plan(direction, dtype, B, heads, Lq, Lk, D);
+    plan[0] = p.cols;
+    plan[1] = p.splits;
+    plan[2] = p.few;
+    return 0;
+}
+
 template <typename K>
 static int rp_launch(const char* name, K kernel, dim3 grid, size_t lds, const RpArgs& a, hipStream_t s) {
     if (lds > 65536) {

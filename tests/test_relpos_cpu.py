@@ -139,3 +139,27 @@ def test_wrapper_refuses():
         relpos_self_attention(torch.zeros(2, 4, 3, 16), table, plan)
     with pytest.raises(RuntimeError, match="no CPU path"):
         relpos_self_attention(torch.zeros(2, 4, 3, 3, 16), table, plan)
+
+
+def test_every_layout_of_the_kernels_is_tested():
+    from relpos_variants import BF16, F32, FORWARD, KEYS, QUERIES, VARIANTS, layout
+    seen = set()
+    for problem, want in VARIANTS.items():
+        dtype, B, heads, Lq, Lk, D, height, width, q_start = problem
+        assert Lk <= height * width and q_start + Lq <= height * width
+        assert {direction: layout(direction, *problem[:6]) for direction in want} == want, problem
+        seen |= {(direction, dtype, *want[direction]) for direction in want}
+    both = (False, True)
+    assert seen >= {(d, BF16, cols, split, 0) for d in (FORWARD, QUERIES, KEYS) for cols in (1, 2) for split in both}
+    assert seen >= {(d, F32, 1, split, 0) for d in (FORWARD, QUERIES, KEYS) for split in both}
+    assert seen >= {(FORWARD, BF16, 0, split, few) for split in both for few in (1, 2)} | {(FORWARD, F32, 0, split, few) for split in both for few in (1, 4)}
+
+
+def test_plan_entry_refuses():
+    lib, plan = mia_amd.lib(), (ctypes.c_int * 3)()
+    for args in ((3, 0, 1, 1, 5, 5, 16, plan), (-1, 0, 1, 1, 5, 5, 16, plan), (0, 2, 1, 1, 5, 5, 16, plan), (0, 0, 1, 1, 5, 5, 16, None)):
+        with pytest.raises(mia_amd.MiaError, match="bad arguments"):
+            lib.mia_relpos_plan(*args)
+    for args in ((0, 5, 5, 16), (1, 0, 5, 16), (1, 5, 0, 16), (1, 5, 5, 12), (1, 5, 5, 136)):
+        with pytest.raises(mia_amd.MiaError, match="bad shape"):
+            lib.mia_relpos_plan(0, 0, 1, *args, plan)

@@ -391,3 +391,31 @@ def test_key_gradients_hold_the_weights_twice(height, width, B, D, drop):
     grads = torch.autograd.grad(relpos_attention(*mine, plan, dropout_p=drop, seed=1234), mine, dout.cuda())
     _compare(grads[1], want["dk"], tol["dk_split"], "dk")
     _compare(grads[2], want["dv"], tol["dv_split"], "dv")
+
+
+def _variants():
+    from relpos_variants import VARIANTS
+    return [pytest.param(p, id="-".join(map(str, p))) for p in VARIANTS]
+
+
+@pytest.mark.parametrize("problem", _variants())
+def test_every_layout_of_the_kernels(problem):
+    """Each choice of columns, splits and heads of a workgroup, with masks and with dropout (see relpos_variants.py)."""
+    from relpos_variants import VARIANTS, layout
+    dtype, B, heads, Lq, Lk, D, height, width, q_start = problem
+    for direction, want in VARIANTS[problem].items():
+        assert layout(direction, *problem[:6]) == want
+    mask = torch.rand(B, Lk, generator=torch.Generator().manual_seed(22)) < 0.8
+    mask[0] = False
+    if B > 1:
+        mask[1] = torch.arange(Lk) < Lk // 2
+    plan = RelativePositionBuckets(height, width, 16, 64)
+    _check(plan, B=B, heads=heads, Lq=Lq, Lk=Lk, q_start=q_start, D=D, dtype=(F32, BF16)[dtype], mask=mask, drop=0.1 if B * heads * Lq * Lk < 1 << 23 else 0.0)
+    if B * heads * Lq * Lk < 1 << 22:
+        _check(plan, B=B, heads=heads, Lq=Lq, Lk=Lk, q_start=q_start, D=D, dtype=(F32, BF16)[dtype])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_bias_gradient_over_more_than_1024_key_blocks(dtype):
+    _check(RelativePositionBuckets(1, 65800, 32, 128), B=1, heads=1, Lq=70, Lk=65700, q_start=65700, D=16, dtype=dtype)
+    _check(RelativePositionBuckets(256, 257, 16, 64), B=1, heads=1, Lq=70, Lk=65700, q_start=30000, D=8, dtype=dtype)
