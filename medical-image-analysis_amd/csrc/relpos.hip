@@ -276,7 +276,7 @@ enum { RP_FWD, RP_BWD_Q, RP_BWD_KV };
 // 4, 8 heads of 64: dK/dV 140 -> 103 us, forward unchanged).
 constexpr int rp_waves(int what, bool half, int DP, int cols) {
     if (what == RP_FWD)
-        return half ? (cols == 1 ? (DP <= 32 ? 4 : DP <= 64 ? 3 : 2) : (DP <= 16 ? 3 : 2)) : (DP <= 32 ? 4 : DP <= 64 ? 3 : 2);
+        return half ? (cols == 1 ? (DP <= 32 ? 4 : DP <= 64 ? 3 : 2) : 2) : (DP <= 32 ? 4 : DP <= 64 ? 3 : 2);
     if (what == RP_BWD_Q) return half ? (cols == 1 ? (DP <= 32 ? 4 : DP <= 64 ? 3 : 2) : (DP <= 32 ? 3 : 2)) : (DP <= 32 ? 4 : DP <= 96 ? 2 : 1);
     return half ? (cols == 1 ? (DP <= 32 ? 4 : DP <= 64 ? 3 : 2) : (DP <= 16 ? 3 : 2)) : (DP <= 16 ? 4 : DP <= 32 ? 3 : DP <= 64 ? 2 : 1);
 }
@@ -1523,8 +1523,8 @@ static size_t rp_es(int dtype) { return dtype == MIA_BF16 ? 2 : 4; }
 
 // How the kernels are laid out over a problem: the pair with the lowest estimate of
 //   cols: 16-wide columns of a wave, so 64 * cols queries (keys) of a workgroup. Two serve more products with every operand read from
-//     LDS, but a round of them is 1.85 times as long (about twice with short heads, whose two-column kernels have half as many
-//     waves a SIMD). fp32 and wide heads keep one: their operands do not fit.
+//     LDS, but a round of them is 1.85 times as long (1.95 backward with heads of up to 32, whose two-column kernels have half as
+//     many waves a SIMD; forward 2.1, so such heads keep one). fp32 and wide heads keep one: their operands do not fit.
 //   splits: ranges of the tokens a workgroup walks, of at least four rounds, joined afterwards.
 // The kernels are bound by issue, so what counts is the busiest of the 256 CUs: ceil(workgroups * splits / 256) of them, for
 // ceil(rounds / splits) rounds each; a workgroup alone on its CU takes 1.25 times its share, and joining about 3 rounds plus what the
@@ -1536,6 +1536,7 @@ static size_t rp_es(int dtype) { return dtype == MIA_BF16 ? 2 : 4; }
 // waves read neighbouring heads, whose rows are one piece of memory, in ranges that make about 2048 waves; else the waves share one
 // head's keys, four chunks each, which is what a second workgroup and the joining would cost.
 #define RP_FEW_WAVES 2048
+constexpr bool rp_two_columns(int what, int DP) { return what == RP_FWD ? DP > 32 && DP <= 96 : DP <= 64; }
 struct RpPlan {
     int cols, splits, few;
 };
@@ -1543,7 +1544,7 @@ static RpPlan rp_plan(int what, int dtype, int B, int heads, int Lq, int Lk, int
     const int DP = rp_dp(D), owned = what == RP_BWD_KV ? Lk : Lq, walked = what == RP_BWD_KV ? Lq : Lk;
     const int round = what == RP_BWD_KV ? RP_TILE : rp_stage(dtype, DP);
     const long long rounds = (walked + round - 1) / round, most = rounds / 4 < 1 ? 1 : rounds / 4 < 64 ? rounds / 4 : 64;
-    const int max_cols = dtype == MIA_F32 || DP > (what == RP_FWD ? 96 : 64) || owned <= 64 ? 1 : 2;
+    const int max_cols = dtype == MIA_F32 || owned <= 64 || !rp_two_columns(what, DP) ? 1 : 2;
     RpPlan p = {1, 1, 0};
     if (what == RP_FWD && Lq <= RP_FEW) {
         const int keys = rp_few_keys(dtype, DP);
@@ -1561,7 +1562,7 @@ static RpPlan rp_plan(int what, int dtype, int B, int heads, int Lq, int Lk, int
     double best = 1e300;
     for (int cols = 1; cols <= max_cols; ++cols) {
         const long long wgs = (long long)B * heads * ((owned + 64 * cols - 1) / (64 * cols));
-        const double length = cols == 1 ? 1.0 : DP > 32 ? 1.85 : what == RP_FWD ? 2.1 : 1.95;
+        const double length = cols == 1 ? 1.0 : DP > 32 ? 1.85 : 1.95;
         for (long long s = 1; s <= most; ++s) {
             const long long busiest = (wgs * s + 255) / 256, walk = (rounds + s - 1) / s;
             double t = length * walk * (busiest == 1 ? 1.25 : (double)busiest);
@@ -1593,7 +1594,6 @@ static int rp_launch(const char* name, K kernel, dim3 grid, size_t lds, const Rp
     return 0;
 }
 
-// cols: 16-wide columns of a wave
 template <typename T, int DP>
 static int rp_few(const char* name, dim3 grid, const RpArgs& a, hipStream_t s) {
     MIA_LAUNCH((relpos_few_kernel<T, DP>), grid, dim3(256), 0, s, a);
@@ -1605,14 +1605,15 @@ static int rp_few(const char* name, dim3 grid, const RpArgs& a, hipStream_t s) {
     return 0;
 }
 
+// COLS: 16-wide columns of a wave
 template <typename T, int DP, int COLS>
 static int rp_run(int what, const char* name, dim3 grid, size_t lds, const RpArgs& a, hipStream_t s) {
-    if constexpr (COLS == 1 || DP <= 96) {
+    if constexpr (COLS == 1 || rp_two_columns(RP_FWD, DP)) {
         if (what == RP_FWD) return rp_launch(name, relpos_fwd_kernel<T, DP, COLS>, grid, lds, a, s);
     }
-    if constexpr (COLS == 1 || DP <= 64) {
+    if constexpr (COLS == 1 || rp_two_columns(RP_BWD_Q, DP)) {
         if (what == RP_BWD_Q) return rp_launch(name, relpos_bwd_q_kernel<T, DP, COLS>, grid, lds, a, s);
-        return rp_launch(name, relpos_bwd_kv_kernel<T, DP, COLS>, grid, lds, a, s);
+        if (what == RP_BWD_KV) return rp_launch(name, relpos_bwd_kv_kernel<T, DP, COLS>, grid, lds, a, s);
     }
     mia_set_error("%s: dispatch failed", name);
     return -1;
