@@ -12,8 +12,8 @@
 //
 // Matrix cores: S^T = K Q^T with keys as rows leaves a lane of v_mfma_f32_16x16x* four consecutive keys of ONE query: the
 // softmax runs down registers plus two lane exchanges, and the four values are already the B operand of O^T = V^T P^T (V^T
-// read from the row-major tile by the transposing LDS read). fp32 runs the same code on 16x16x4. No L x L array exists in
-// memory; the backward recomputes P from the row statistics, once with queries as columns (dQ) and once with keys as
+// read from the row-major tile by the transposing LDS read). fp32 runs the same code on 16x16x4. Scores and weights never
+// exist in memory (the table's gradient needs rows of offsets, see rp_slab_ld); the backward recomputes P from the row statistics, once with queries as columns (dQ) and once with keys as
 // columns (dK, dV, dtable). P and dS become bf16 only as operands of bf16 products, as two numbers each (what the first
 // rounding took off is the second); statistics, D and the bias gradient stay fp32.
 //
@@ -1761,9 +1761,12 @@ extern "C" int mia_relpos_fwd(int dtype, const void* q, const void* k, const voi
     return rp_join<RP_FWD>("mia_relpos_fwd", dtype, a, s);
 }
 
-// floats of one slab row, and key blocks of one (image, head)
-static int rp_slab_ld(const RpArgs& a, int tokens, int cols) {
-    return rp_span(a, a.Lq, tokens) + rp_span(a, 64 * cols, tokens) + 1;
+// Floats of one slab row: the offsets between the keys of a block and the queries of a split's range. A map's offsets span about
+// twice its tokens, so the rows of an (image, head) are L^2 / 32 floats on a map with blocks of 64 keys, L^2 / 128 on a sequence
+// with blocks of 128, and the ranges' ends (75x75, 4 heads of 32: 18 MB; 127 with room for all queries in every range's row).
+static int rp_slab_ld(const RpArgs& a, int tokens, const RpPlan& p) {
+    const int qtiles = (a.Lq + RP_TILE - 1) / RP_TILE, range = RP_TILE * ((qtiles + p.splits - 1) / p.splits);
+    return rp_span(a, range < a.Lq ? range : a.Lq, tokens) + rp_span(a, 64 * p.cols, tokens) + 1;
 }
 
 // The backward's workspace: D of every row | the bias gradient per offset | slab rows | partial results (those of dQ are
@@ -1779,7 +1782,7 @@ static RpWs rp_bwd_ws(int dtype, int B, int heads, int Lq, int Lk, int D, int he
     RpWs w;
     w.per_off = (bh * Lq + 3) / 4 * 4;
     w.slab = w.per_off + (want_bias ? (long long)heads * a.n_off : 0);
-    w.part = w.slab + (want_bias ? bh * ((Lk + kt - 1) / kt) * kv.splits * rp_slab_ld(a, height * width, kv.cols) : 0);
+    w.part = w.slab + (want_bias ? bh * ((Lk + kt - 1) / kt) * kv.splits * rp_slab_ld(a, height * width, kv) : 0);
     w.part = (w.part + 3) / 4 * 4;
     const long long pq = rp_part_floats(RP_BWD_Q, q, B, heads, Lq, Lk, D), pk = rp_part_floats(RP_BWD_KV, kv, B, heads, Lq, Lk, D);
     w.total = w.part + (pq > pk ? pq : pk);
@@ -1839,7 +1842,7 @@ extern "C" int mia_relpos_bwd(int dtype, const void* q, const void* k, const voi
     a.splits = kp.splits;
     float* per_off = ws + w.per_off;
     if (dtable) {
-        a.slab_ld = rp_slab_ld(a, tokens, kp.cols);
+        a.slab_ld = rp_slab_ld(a, tokens, kp);
         a.slab = ws + w.slab;
     }
     const size_t kv_lds = 2 * (tile + 256) + 5 * RP_TILE * 4 + (size_t)ring * (dtable ? 4 + 4 * 8 : 4);

@@ -1,5 +1,6 @@
-"""Multi-head attention with a learned relative position bias, on the gfx950 kernels of csrc/relpos.hip: no limit on the
-number of tokens, masked keys, few queries against many keys, gradients of everything including the bias table."""
+"""Multi-head attention with a learned relative position bias, on the gfx950 kernels of csrc/relpos.hip: maps of up to 2 ** 22
+tokens and series of up to 2 ** 26, masked keys, few queries against many keys, gradients of everything including the bias table
+(whose backward holds up to L * L / 32 floats an image and head on a map of L tokens, L * L / 64 on a series)."""
 import math
 
 import numpy as np

@@ -163,3 +163,19 @@ def test_plan_entry_refuses():
     for args in ((0, 5, 5, 16), (1, 0, 5, 16), (1, 5, 0, 16), (1, 5, 5, 12), (1, 5, 5, 136)):
         with pytest.raises(mia_amd.MiaError, match="bad shape"):
             lib.mia_relpos_plan(0, 0, 1, *args, plan)
+
+
+@pytest.mark.parametrize("dtype,B,heads,height,width,D", [(1, 1, 4, 75, 75, 32), (0, 1, 4, 75, 75, 32), (1, 1, 4, 38, 38, 64), (1, 4, 8, 38, 38, 64), (0, 1, 2, 128, 128, 64),
+                                                          (1, 1, 4, 1, 4096, 64), (1, 128, 8, 10, 10, 48), (0, 1, 1, 700, 2, 16)])
+def test_workspace_of_the_bias_gradient(dtype, B, heads, height, width, D):
+    """A key block keeps room for the offsets that its queries reach, not once more for every range that its walk is split into:
+    what the ranges add is their ends alone."""
+    lib, plan, L = mia_amd.lib(), (ctypes.c_int * 3)(), height * width
+    lib.mia_relpos_plan(2, dtype, B, heads, L, L, D, plan)
+    cols, splits = plan[0], plan[1]
+    span = lambda n: n - 1 + (-(-(n - 1) // width) * (width - 1) if height > 1 else 0)     # noqa: E731  (offsets between n tokens)
+    blocks = -(-L // (64 * cols))
+    rows = blocks * (span(L) + splits * (span(128) + span(64 * cols) + 2))
+    n_off = (2 * height - 1) * (2 * width - 1)
+    want = lambda table: lib.mia_relpos_bwd_ws_floats(dtype, B, heads, L, L, D, height, width, table)      # noqa: E731
+    assert want(1) - want(0) <= heads * n_off + B * heads * rows + 4
