@@ -15,7 +15,7 @@
 // read from the row-major tile by the transposing LDS read). fp32 runs the same code on 16x16x4. Scores and weights never
 // exist in memory (the table's gradient needs rows of offsets, see rp_slab_ld); the backward recomputes P from the row statistics, once with queries as columns (dQ) and once with keys as
 // columns (dK, dV, dtable). P and dS become bf16 only as operands of bf16 products, as two numbers each (what the first
-// rounding took off is the second); statistics, D and the bias gradient stay fp32.
+// rounding took off is the second); statistics and D stay fp32, the bias gradient is added up in double.
 //
 // D is needed to fp32 accuracy because the rows of dS sum to zero and a bucket's gradient is what is left of many terms. The
 // output a bf16 caller holds is too coarse for it: the forward keeps what its rounding took off beside it, the dQ kernel starts from
@@ -1422,7 +1422,8 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
 
 // ------------------------------------------------------------------------------------------------
 // bias gradient: offsets over images and key blocks, then buckets over their offsets (the offsets of bucket k are
-// order[start[k]] .. order[start[k + 1] - 1]). Fixed order everywhere.
+// order[start[k]] .. order[start[k + 1] - 1]). Fixed order everywhere; in double, because a bucket's gradient is what is left of many
+// terms of both signs: only a slab row and the result are fp32.
 // ------------------------------------------------------------------------------------------------
 // Slab rows are [image][head][key block][query range]; the offsets that a row covers depend on the last two alone. A workgroup: 64
 // * PER offsets, 16 waves that share the rows where there are at least 16 of them (PER = 4: a row's four loads are in flight
@@ -1430,14 +1431,14 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
 // that reach the workgroup's offsets. 75x75 map, 4 heads, 704 rows: 11 us, 18 to 20 with PER = 1 (31 with every row tested by every
 // wave); 38x38, 8 heads, 23 rows, 4 images: 5.5 us, 7.7 with PER = 1.
 template <int PER>
-__global__ __launch_bounds__(1024) void relpos_offsets_kernel(RpArgs a, int ktiles, int kt, float* __restrict__ per_off) {
-    __shared__ float sm[16][64 * PER];
+__global__ __launch_bounds__(1024) void relpos_offsets_kernel(RpArgs a, int ktiles, int kt, double* __restrict__ per_off) {
+    __shared__ double sm[16][64 * PER];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), o0 = blockIdx.x * 64 * PER, h = blockIdx.y;
     const int rows = ktiles * a.splits, qtiles = (a.Lq + RP_TILE - 1) / RP_TILE;
     const size_t image = (size_t)a.heads * rows * a.slab_ld;
-    float v[PER];
+    double v[PER];
 #pragma unroll
-    for (int u = 0; u < PER; ++u) v[u] = 0.f;
+    for (int u = 0; u < PER; ++u) v[u] = 0.0;
     for (int first = 0; first < rows; first += 1024) {
         const int r = first + (PER == 4 ? lane * 16 + wave : lane), kb = (int)((unsigned)r / (unsigned)a.splits), sp = r - kb * a.splits, k0 = kb * kt;
         int lo = 0, hi = -1;
@@ -1459,7 +1460,7 @@ __global__ __launch_bounds__(1024) void relpos_offsets_kernel(RpArgs a, int ktil
 #pragma unroll
                     for (int u = 0; u < 4; ++u) x[u] = p[at[u]];
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) v[u] += at[u] == o0 + u * 64 + lane - from ? x[u] : 0.f;
+                    for (int u = 0; u < 4; ++u) v[u] += (double)(at[u] == o0 + u * 64 + lane - from ? x[u] : 0.f);
                 }
             } else {
                 const int o = o0 + lane;
@@ -1470,11 +1471,11 @@ __global__ __launch_bounds__(1024) void relpos_offsets_kernel(RpArgs a, int ktil
                     float x[4];
 #pragma unroll
                     for (int u = 0; u < 4; ++u) x[u] = p[(b + u * 16) * image];
-                    if (in) v[0] += (x[0] + x[1]) + (x[2] + x[3]);
+                    if (in) v[0] += ((double)x[0] + (double)x[1]) + ((double)x[2] + (double)x[3]);
                 }
                 for (; b < a.B; b += 16) {
                     const float x = p[b * image];
-                    if (in) v[0] += x;
+                    if (in) v[0] += (double)x;
                 }
             }
         }
@@ -1483,22 +1484,23 @@ __global__ __launch_bounds__(1024) void relpos_offsets_kernel(RpArgs a, int ktil
     for (int u = 0; u < PER; ++u) sm[wave][u * 64 + lane] = v[u];
     __syncthreads();
     if ((int)threadIdx.x >= 64 * PER || o0 + (int)threadIdx.x >= a.n_off) return;
-    float total = sm[0][threadIdx.x];
+    double total = sm[0][threadIdx.x];
     for (int w = 1; w < 16; ++w) total += sm[w][threadIdx.x];
     per_off[(size_t)h * a.n_off + o0 + threadIdx.x] = total;
 }
 
-__global__ __launch_bounds__(256) void relpos_buckets_kernel(const float* __restrict__ per_off, int n_off, int heads,
+__global__ __launch_bounds__(256) void relpos_buckets_kernel(const double* __restrict__ per_off, int n_off, int heads,
                                                              const int* __restrict__ order, const int* __restrict__ start,
                                                              float* __restrict__ dtable) {
-    __shared__ float sm[4];
+    __shared__ double sm[4];
     const int k = blockIdx.x, h = blockIdx.y;
-    float v = 0.f;
+    double v = 0.0;
     for (int i = start[k] + threadIdx.x; i < start[k + 1]; i += 256) v += per_off[(size_t)h * n_off + order[i]];
-    v = wave_sum(v);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     if ((threadIdx.x & 63) == 0) sm[threadIdx.x >> 6] = v;
     __syncthreads();
-    if (threadIdx.x == 0) dtable[(size_t)k * heads + h] = (sm[0] + sm[1]) + (sm[2] + sm[3]);
+    if (threadIdx.x == 0) dtable[(size_t)k * heads + h] = (float)((sm[0] + sm[1]) + (sm[2] + sm[3]));
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1769,7 +1771,7 @@ static int rp_slab_ld(const RpArgs& a, int tokens, const RpPlan& p) {
     return rp_span(a, range < a.Lq ? range : a.Lq, tokens) + rp_span(a, 64 * p.cols, tokens) + 1;
 }
 
-// The backward's workspace: D of every row | the bias gradient per offset | slab rows | partial results (those of dQ are
+// The backward's workspace: D of every row | the bias gradient per offset (doubles) | slab rows | partial results (those of dQ are
 // joined before the dK / dV kernel writes its own over them)
 struct RpWs {
     long long per_off, slab, part, total;
@@ -1781,7 +1783,7 @@ static RpWs rp_bwd_ws(int dtype, int B, int heads, int Lq, int Lk, int D, int he
     const long long bh = (long long)B * heads, kt = 64 * kv.cols;
     RpWs w;
     w.per_off = (bh * Lq + 3) / 4 * 4;
-    w.slab = w.per_off + (want_bias ? (long long)heads * a.n_off : 0);
+    w.slab = w.per_off + (want_bias ? 2ll * heads * a.n_off : 0);
     w.part = w.slab + (want_bias ? bh * ((Lk + kt - 1) / kt) * kv.splits * rp_slab_ld(a, height * width, kv) : 0);
     w.part = (w.part + 3) / 4 * 4;
     const long long pq = rp_part_floats(RP_BWD_Q, q, B, heads, Lq, Lk, D), pk = rp_part_floats(RP_BWD_KV, kv, B, heads, Lq, Lk, D);
@@ -1840,7 +1842,7 @@ extern "C" int mia_relpos_bwd(int dtype, const void* q, const void* k, const voi
     MIA_CHECK_ARG(ring <= RP_RING_MAX, "mia_relpos_bwd: ring of %d offsets", ring);
     a.acc_mask = ring - 1;
     a.splits = kp.splits;
-    float* per_off = ws + w.per_off;
+    double* per_off = reinterpret_cast<double*>(ws + w.per_off);
     if (dtable) {
         a.slab_ld = rp_slab_ld(a, tokens, kp);
         a.slab = ws + w.slab;

@@ -419,3 +419,28 @@ def test_every_layout_of_the_kernels(problem):
 def test_bias_gradient_over_more_than_1024_key_blocks(dtype):
     _check(RelativePositionBuckets(1, 65800, 32, 128), B=1, heads=1, Lq=70, Lk=65700, q_start=65700, D=16, dtype=dtype)
     _check(RelativePositionBuckets(256, 257, 16, 64), B=1, heads=1, Lq=70, Lk=65700, q_start=30000, D=8, dtype=dtype)
+
+
+@pytest.mark.parametrize("height,width,Lq", [(1, 64, 64), (8, 8, 64), (1, 1088, 64), (32, 34, 64)])
+def test_bias_gradient_is_added_up_exactly(height, width, Lq):
+    """With equal scores over a power of two of keys every weight is exact, and with small whole numbers in v and dout so are dS
+    (multiples of 2^-12) and the sum of an offset over a tile. What is left is the addition over images, tiles and offsets, whose
+    terms do not cancel here (odd dx against even) and need more than 24 bits: it may cost the result's own rounding, 2^-24."""
+    index = torch.arange((2 * height - 1) * (2 * width - 1)) % (2 * width - 1) % 2      # whether dx is even
+    plan = RelativePositionBuckets.from_index(height, width, index)
+    B, L, g = 100, height * width, torch.Generator().manual_seed(23)
+    keep = torch.arange(L) >= L - 64            # 64 keys that exist: weights of 1/64
+    sign = 1.0 - 2.0 * (torch.arange(L) % 2)
+    v = torch.randint(-3, 4, (B, L, 2, 8), generator=g).float()
+    v[..., 0] = 7.0 * sign[None, :, None]
+    dout = torch.randint(-3, 4, (B, Lq, 2, 8), generator=g).float()
+    dout[..., 0] = 7.0 * sign[None, :Lq, None]
+    q, k = torch.zeros(B, Lq, 2, 8), torch.randn(B, L, 2, 8, generator=g)
+    table = torch.zeros(2, 2)
+    mask = keep.expand(B, L)
+    want, _ = formula(q, k, v, table, plan, mask, dout=dout)
+    assert float(want["dtable"].abs().min()) * 2 ** 12 > 2 ** 25
+    t = table.cuda().requires_grad_()
+    out = relpos_attention(q.cuda(), k.cuda(), v.cuda(), t, plan, key_mask=mask.cuda())
+    (got,) = torch.autograd.grad(out, t, dout.cuda())
+    _compare(got, want["dtable"], 2.0 ** -24 * want["dtable"].abs() + 1e-9, "dtable")
