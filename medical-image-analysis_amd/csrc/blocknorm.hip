@@ -532,6 +532,7 @@ extern "C" int mia_blocknorm_fwd(int dtype, const void* x, const void* f, int im
                                  void* stream) {
     if (bn_checks("mia_blocknorm_fwd", dtype, images, rows_per_image, C, gate, post, pre, eps)) return -1;
     MIA_CHECK_ARG(x && f && y && (!pre || z), "mia_blocknorm_fwd: null");
+    MIA_CHECK_ARG(((uintptr_t)stats & 15) == 0, "mia_blocknorm_fwd: stats must start at a multiple of 16 bytes");
     MIA_CHECK_ARG(!post == !post_w && !pre == !pre_w && (post || !post_b) && (pre || !pre_b),
                   "mia_blocknorm_fwd: a norm comes with its weight, and only then with a bias");
     BNormArgs a = {};
@@ -553,6 +554,7 @@ extern "C" int mia_blocknorm_bwd(int dtype, const void* dy, const void* dz, cons
                                  float* dpost_b, float* dpre_w, float* dpre_b, void* stream) {
     if (bn_checks("mia_blocknorm_bwd", dtype, images, rows_per_image, C, gate, post, pre, 0.f)) return -1;
     MIA_CHECK_ARG((dy || dz) && x && f && stats && ws && dx && df, "mia_blocknorm_bwd: null");
+    MIA_CHECK_ARG((((uintptr_t)ws | (uintptr_t)stats) & 15) == 0, "mia_blocknorm_bwd: stats and the workspace must start at multiples of 16 bytes");
     MIA_CHECK_ARG(!post == !post_w && !pre == !pre_w && (post || !post_b) && (pre || !dz),
                   "mia_blocknorm_bwd: a norm comes with its weight, and only then with a gradient");
     MIA_CHECK_ARG(ws_floats >= mia_blocknorm_ws_floats(images, rows_per_image, C, gate != nullptr),

@@ -64,3 +64,14 @@ def test_wrapper_refuses():
         gated_residual_norm(torch.zeros(1, 8200), torch.zeros(1, 8200), pre=None)
     with pytest.raises(ValueError, match="two dimensions"):
         gated_residual_norm(torch.zeros(16), torch.zeros(16), pre=None, gate=torch.ones(16, 16))
+
+
+def test_scratch_alignment_is_checked():
+    """Statistics are read and written 16 bytes at a time."""
+    lib, odd = mia_amd.lib(), ctypes.c_void_p(4104)
+    need = lib.mia_blocknorm_ws_floats(2, 3, 16, 1)
+    with pytest.raises(mia_amd.MiaError, match="16 bytes"):
+        lib.mia_blocknorm_fwd(0, P, P, 2, 3, 16, None, None, 0, None, None, 1, P, None, 1e-6, P, P, odd, None)
+    for ws, stats in ((odd, P), (P, odd)):
+        with pytest.raises(mia_amd.MiaError, match="16 bytes"):
+            lib.mia_blocknorm_bwd(0, P, P, P, P, stats, 2, 3, 16, None, None, 0, None, None, 1, P, ws, need, P, P, None, None, None, None, None, None, None)
