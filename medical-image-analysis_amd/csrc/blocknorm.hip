@@ -20,7 +20,7 @@
 // waiting out every load (32 images of 1444 rows of 1024 bf16 channels, two RMS norms: forward 91 -> 73 us, backward 164 -> 131;
 // now 65, 5.8 TB/s, and 125, 4.5 TB/s). Long batches of rows are bound by HBM, short ones (a head's 100 tokens) by latency.
 // The backward keeps its column sums in registers over all rows of a workgroup and leaves one slab row; two small kernels add
-// the slab up in a fixed order (no atomics).
+// the slab up in double, in a fixed order (no atomics).
 #include "common.h"
 
 enum { BNORM_NONE = 0, BNORM_RMS = 1, BNORM_LAYER = 2 };
@@ -392,16 +392,16 @@ __global__ __launch_bounds__(WG) void blocknorm_bwd_kernel(BNormArgs a) {
 // grid (groups, ceil(C / 64)), 16 row lanes x 64 columns.
 __global__ __launch_bounds__(1024) void blocknorm_fold_kernel(const float* __restrict__ slab, int rows, int per, int C,
                                                               const float* __restrict__ scale, const float* __restrict__ w1,
-                                                              const float* __restrict__ b1, float* __restrict__ sums,
+                                                              const float* __restrict__ b1, double* __restrict__ sums,
                                                               float* __restrict__ dgate) {
-    __shared__ float sm[16][4][64];
+    __shared__ double sm[16][4][64];
     const int col = threadIdx.x & 63, g = threadIdx.x >> 6, c = blockIdx.y * 64 + col;
     const int r0 = blockIdx.x * per, r1 = min(rows, r0 + per);
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    double v[4] = {0.0, 0.0, 0.0, 0.0};
     if (c < C)
         for (int r = r0 + g; r < r1; r += 16)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] += slab[((size_t)r * 4 + k) * C + c];
+            for (int k = 0; k < 4; ++k) v[k] += (double)slab[((size_t)r * 4 + k) * C + c];
 #pragma unroll
     for (int k = 0; k < 4; ++k) sm[g][k][col] = v[k];
     __syncthreads();
@@ -411,25 +411,26 @@ __global__ __launch_bounds__(1024) void blocknorm_fold_kernel(const float* __res
         for (int w = 1; w < 16; ++w) v[k] += sm[w][k][col];
 #pragma unroll
     for (int k = 0; k < 4; ++k) sums[((size_t)blockIdx.x * 4 + k) * C + c] = v[k];
-    if (dgate) dgate[(size_t)blockIdx.x * C + c] = (scale ? scale[c] : 1.f) * ((w1 ? w1[c] : 1.f) * v[0] + (b1 ? b1[c] : 0.f) * v[1]);
+    if (dgate) dgate[(size_t)blockIdx.x * C + c] = (float)((scale ? scale[c] : 1.f) * ((w1 ? w1[c] : 1.f) * v[0] + (b1 ? b1[c] : 0.f) * v[1]));
 }
 
-// parameter gradients from the group sums; gate (nullable): [groups][C]
-__global__ __launch_bounds__(1024) void blocknorm_params_kernel(const float* __restrict__ sums, int groups, int C,
+// parameter gradients from the group sums (S = double) or from the slab's rows themselves (float); gate (nullable): [groups][C]
+template <typename S>
+__global__ __launch_bounds__(1024) void blocknorm_params_kernel(const S* __restrict__ sums, int groups, int C,
                                                                 const float* __restrict__ gate, const float* __restrict__ scale,
                                                                 const float* __restrict__ w1, const float* __restrict__ b1,
                                                                 float* dscale, float* dw1, float* db1, float* dw2, float* db2) {
-    __shared__ float sm[16][4][64];
+    __shared__ double sm[16][4][64];
     const int col = threadIdx.x & 63, g = threadIdx.x >> 6, c = blockIdx.x * 64 + col;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    double v[4] = {0.0, 0.0, 0.0, 0.0};
     if (c < C)
         for (int n = g; n < groups; n += 16) {
-            const float* p = sums + (size_t)n * 4 * C + c;
-            const float gt = gate ? gate[(size_t)n * C + c] : 1.f;
-            v[0] = fmaf(gt, p[0], v[0]);
-            v[1] = fmaf(gt, p[C], v[1]);
-            v[2] += p[2 * (size_t)C];
-            v[3] += p[3 * (size_t)C];
+            const S* p = sums + (size_t)n * 4 * C + c;
+            const double gt = gate ? gate[(size_t)n * C + c] : 1.f;
+            v[0] = fma(gt, (double)p[0], v[0]);
+            v[1] = fma(gt, (double)p[C], v[1]);
+            v[2] += (double)p[2 * (size_t)C];
+            v[3] += (double)p[3 * (size_t)C];
         }
 #pragma unroll
     for (int k = 0; k < 4; ++k) sm[g][k][col] = v[k];
@@ -438,12 +439,12 @@ __global__ __launch_bounds__(1024) void blocknorm_params_kernel(const float* __r
 #pragma unroll
     for (int k = 0; k < 4; ++k)
         for (int w = 1; w < 16; ++w) v[k] += sm[w][k][col];
-    const float sc = scale ? scale[c] : 1.f;
-    if (dscale) dscale[c] = (w1 ? w1[c] : 1.f) * v[0] + (b1 ? b1[c] : 0.f) * v[1];
-    if (dw1) dw1[c] = sc * v[0];
-    if (db1) db1[c] = sc * v[1];
-    if (dw2) dw2[c] = v[2];
-    if (db2) db2[c] = v[3];
+    const double sc = scale ? scale[c] : 1.f;
+    if (dscale) dscale[c] = (float)((w1 ? w1[c] : 1.f) * v[0] + (b1 ? b1[c] : 0.f) * v[1]);
+    if (dw1) dw1[c] = (float)(sc * v[0]);
+    if (db1) db1[c] = (float)(sc * v[1]);
+    if (dw2) dw2[c] = (float)v[2];
+    if (db2) db2[c] = (float)v[3];
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -505,7 +506,7 @@ static int bn_groups(int gated, int N, int S) { return gated ? N : (N * S + 15) 
 
 extern "C" long long mia_blocknorm_ws_floats(int images, long long rows_per_image, int C, int gated) {
     const int S = bn_splits(false, MIA_F32, gated ? images : 1, gated ? rows_per_image : rows_per_image * images, C), N = gated ? images : 1;
-    return ((long long)N * S + bn_groups(gated, N, S)) * 4 * C;
+    return ((long long)N * S + 2ll * bn_groups(gated, N, S)) * 4 * C;   // slab rows | group sums (doubles)
 }
 
 static int bn_checks(const char* name, int dtype, int images, long long rows, int C, const float* gate, int post, int pre, float eps) {
@@ -574,14 +575,17 @@ extern "C" int mia_blocknorm_bwd(int dtype, const void* dy, const void* dz, cons
     const int rows = a.N * a.S;
     const bool fold = gate || rows > 64;
     const int groups = fold ? bn_groups(gate != nullptr, a.N, a.S) : rows;
-    float* sums = fold ? ws + (size_t)rows * 4 * C : ws;
     if (fold) {
+        double* sums = reinterpret_cast<double*>(ws + (size_t)rows * 4 * C);
         MIA_LAUNCH(blocknorm_fold_kernel, dim3(groups, cdiv(C, 64)), dim3(1024), 0, s, ws, rows, gate ? a.S : 16, C, scale, post_w,
                    post_b, sums, gate ? dgate : nullptr);
         MIA_CHECK_LAUNCH("mia_blocknorm_bwd");
+        MIA_LAUNCH(blocknorm_params_kernel<double>, dim3(cdiv(C, 64)), dim3(1024), 0, s, sums, groups, C, gate, scale, post_w, post_b, dscale,
+                   dpost_w, dpost_b, dpre_w, dpre_b);
+    } else {
+        MIA_LAUNCH(blocknorm_params_kernel<float>, dim3(cdiv(C, 64)), dim3(1024), 0, s, ws, groups, C, gate, scale, post_w, post_b, dscale,
+                   dpost_w, dpost_b, dpre_w, dpre_b);
     }
-    MIA_LAUNCH(blocknorm_params_kernel, dim3(cdiv(C, 64)), dim3(1024), 0, s, sums, groups, C, gate, scale, post_w, post_b, dscale,
-               dpost_w, dpost_b, dpre_w, dpre_b);
     MIA_CHECK_LAUNCH("mia_blocknorm_bwd");
     return 0;
 }

@@ -67,7 +67,7 @@ def test_wrapper_refuses():
 
 
 def test_scratch_alignment_is_checked():
-    """Statistics are read and written 16 bytes at a time."""
+    """Statistics are read and written 16 bytes at a time, the workspace holds doubles behind its rows."""
     lib, odd = mia_amd.lib(), ctypes.c_void_p(4104)
     need = lib.mia_blocknorm_ws_floats(2, 3, 16, 1)
     with pytest.raises(mia_amd.MiaError, match="16 bytes"):

@@ -233,3 +233,23 @@ def test_repeatable_streams_and_capture():
         eager = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(static, eager)), k
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("shape", [(1, 361, 2304), (128, 100, 384), (3, 40, 64), (300, 7, 136), (2, 5000, 1024)])
+def test_column_sums_are_added_up_exactly(shape, gated):
+    """Without norms the gradient of the scale is a plain sum of dy * f over the rows (of the gate, over its image's). Whole numbers of up to 2^9
+    leave the few rows of a workgroup exact (63 rows of products below 2^18), the sum over workgroups needs more than 24 bits: it may
+    cost the result's own rounding, 2^-24."""
+    g = torch.Generator().manual_seed(8)
+    C, rows = shape[-1], shape[0] * shape[1]
+    f, dy = (torch.randint(300, 512, shape, generator=g).float() for _ in range(2))
+    scale = torch.ones(C).cuda().requires_grad_()
+    gate = torch.ones(shape[0], C).cuda().requires_grad_() if gated else None
+    y, _ = gated_residual_norm(torch.zeros(shape).cuda(), f.cuda(), scale=scale, gate=gate, pre=None)
+    per_image = (f.double() * dy.double()).sum(1)
+    got = torch.autograd.grad(y, [scale] + [gate] * gated, dy.cuda())
+    _close(got[0], per_image.sum(0), 2.0 ** -24 * per_image.sum(0).abs(), "dscale")
+    if gated:
+        _close(got[1], per_image, 2.0 ** -24 * per_image.abs(), "dgate")
+    assert float(per_image.sum(0).min()) > 2 ** 23 or rows < 200
