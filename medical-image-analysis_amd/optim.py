@@ -17,6 +17,22 @@ def _dense(g):
     return nodes().all_dense([g])
 
 
+_update_check = None
+
+
+def _update_ready(params):
+    """Whether AdamW's kernel can take every parameter and gradient as it is. Attribute by attribute in Python that is a fifth of a
+    step of 22 parameters; it is left to the step's own loop (False) where the C++ module is not built, which nothing else
+    in the optimizer needs."""
+    global _update_check
+    if _update_check is None:
+        try:
+            _update_check = nodes().update_ready
+        except ImportError:
+            _update_check = lambda params: False        # noqa: E731
+    return _update_check(params)
+
+
 def _check_max_norm(max_norm):
     max_norm = float(max_norm)
     if not max_norm >= 0:
@@ -136,8 +152,7 @@ class AdamW(torch.optim.Optimizer):
             ps = [p for p in group["params"] if p.grad is not None]
             if not ps:
                 continue
-            # attribute by attribute in Python the check is a fifth of a step of 22 parameters
-            for p in (() if nodes().update_ready(ps) else ps):
+            for p in (() if _update_ready(ps) else ps):
                 if (not p.is_cuda or not p.grad.is_cuda or p.dtype != torch.float32 or p.grad.dtype != torch.float32
                         or not p.is_contiguous() or p.grad.is_sparse):
                     raise RuntimeError("mia_amd.optim.AdamW needs contiguous fp32 parameters on an MI355X device")

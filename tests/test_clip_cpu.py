@@ -69,3 +69,25 @@ def test_dense_layouts():
     assert optim._dense(t) and optim._dense(t.to(memory_format=torch.channels_last)) and optim._dense(t.permute(3, 1, 0, 2))
     assert optim._dense(t[:, :1, :1, :1].contiguous()) and optim._dense(torch.zeros(())) and optim._dense(t[1:])
     assert not optim._dense(t[:, 1:]) and not optim._dense(t[..., ::2]) and not optim._dense(torch.zeros(3, 1).expand(3, 4))
+
+
+@pytest.fixture
+def without_the_module(monkeypatch):
+    """As where _mia_autograd is missing or was built against another torch."""
+    import mia_amd._lib as _lib
+    from mia_amd import _proto
+    monkeypatch.setattr(_lib, "_nodes", None)
+    monkeypatch.setattr(_proto, "autograd_digest", lambda: "another")
+    monkeypatch.setattr(optim, "_update_check", None, raising=False)
+
+
+def test_adamw_does_not_need_the_autograd_module(without_the_module):
+    """A step gets as far as the check of its parameters; the clipping functions say what is missing."""
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.ones(4)
+    for kw in ({}, {"max_grad_norm": 1.0}):
+        for _ in range(2):
+            with pytest.raises(RuntimeError, match="contiguous fp32 parameters on an MI355X device"):
+                optim.AdamW([p], **kw).step()
+    with pytest.raises(ImportError, match="another header or another torch"):
+        optim.clip_grad_norm_([p], 1.0)

@@ -210,3 +210,21 @@ def test_captured_training_step_with_clipping():
         assert torch.equal(got, loss) and torch.equal(opt_e.grad_norm, opt_g.grad_norm) and float(opt_e.grad_norm) > 0.5
         for p, q in zip(model.parameters(), other.parameters()):
             assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("max_grad_norm", [None, 0.5])
+def test_adamw_without_the_autograd_module(monkeypatch, max_grad_norm):
+    """The optimizer's own check of its parameters: the same steps, and a transposed gradient made contiguous."""
+    import mia_amd._lib as _lib
+    from mia_amd import _proto, optim
+    a, b = _params(24, (70, 4000)), _params(24, (70, 4000))
+    for ps in (a, b):
+        ps.append(torch.nn.Parameter(torch.ones(6, 5, device="cuda")))
+        ps[-1].grad = torch.arange(30.0, device="cuda").view(5, 6).t()
+    first, second = AdamW(a, max_grad_norm=max_grad_norm), AdamW(b, max_grad_norm=max_grad_norm)
+    first.step()
+    monkeypatch.setattr(_lib, "_nodes", None)
+    monkeypatch.setattr(_proto, "autograd_digest", lambda: "another")
+    monkeypatch.setattr(optim, "_update_check", None)
+    second.step()
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
