@@ -119,3 +119,20 @@ def test_tracing_is_refused(which):
         torch.jit.trace(function, (t,), check_trace=False)
     with pytest.raises(RuntimeError, match="cannot be traced"):
         make_fx(function)(t)
+
+
+def test_another_torch_makes_the_module_stale(monkeypatch):
+    """The build that an ImportError asks for compiles the module where its digest is another one, though no file is newer."""
+    import importlib.util
+    import os
+    import torch
+    spec = importlib.util.spec_from_file_location("mia_build_again", os.path.join(os.path.dirname(mia_amd.__file__), "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    made = []
+    monkeypatch.setattr(build.subprocess, "check_call", lambda cmd, *a, **k: made.append(cmd))
+    monkeypatch.setattr(build.os.path, "getmtime", lambda path: 0.0)
+    assert build.build_autograd(verbose=False) == build.autograd_module_path() and not made
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + ".another")
+    build.build_autograd(verbose=False)
+    assert len(made) == 1 and build.autograd_module_path() in made[0]
