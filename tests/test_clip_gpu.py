@@ -228,3 +228,66 @@ def test_adamw_without_the_autograd_module(monkeypatch, max_grad_norm):
     monkeypatch.setattr(optim, "_update_check", None)
     second.step()
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def _rank(rank, port, q):
+    try:
+        import copy
+        import faulthandler
+        import os
+        import torch.distributed as dist
+        faulthandler.dump_traceback_later(100, exit=True)
+        os.environ.update(MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+        dist.init_process_group("gloo", rank=rank, world_size=2)
+        from mia_amd.ddp import GradReducer
+        torch.manual_seed(3)
+        net = torch.nn.Sequential(torch.nn.Linear(20, 30), torch.nn.Tanh(), torch.nn.Linear(30, 5))
+        data = [torch.randn(8, 20) * (1 + 3 * r) for r in range(2)]
+        ref = copy.deepcopy(net).double()
+        (0.5 * sum(ref(x.double()).square().sum() for x in data)).backward()      # the mean of the ranks' gradients
+        want = math.sqrt(sum(float(p.grad.square().sum()) for p in ref.parameters()))
+        own = copy.deepcopy(net).double()
+        own(data[rank].double()).square().sum().backward()
+        alone = math.sqrt(sum(float(p.grad.square().sum()) for p in own.parameters()))
+        net.cuda()
+        red = GradReducer(net.parameters(), bucket_bytes=1 << 10)
+        opt = AdamW(net.parameters(), lr=1e-3, max_grad_norm=0.5)
+        red.zero_grad()
+        net(data[rank].cuda()).square().sum().backward()
+        red.finish()
+        opt.step()
+        inside = float(opt.grad_norm)
+        got = float(clip_grad_norm_(net.parameters(), 0.5))
+        after = _norm64([p.grad for p in net.parameters()])
+        dist.destroy_process_group()
+        q.put((rank, want, alone, inside, got, after, [p.detach().cpu().numpy() for p in net.parameters()]))
+    except Exception:
+        import traceback
+        q.put((rank, traceback.format_exc()[-1500:]))
+
+
+def test_norm_of_exchanged_gradients():
+    """Behind GradReducer the norm is that of the averaged gradients, the same on both ranks, and so is the step. (fp32 gradients of two
+    small layers: a few sums of at most 30 terms, 100 * 2^-24 of the norm.)"""
+    import socket
+    import torch.multiprocessing as mp
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    ranks = [ctx.Process(target=_rank, args=(r, port, q)) for r in range(2)]
+    for p in ranks:
+        p.start()
+    try:
+        res = sorted((q.get(timeout=110) for _ in ranks), key=lambda r: r[0])
+    finally:
+        for p in ranks:
+            p.join(timeout=20)
+            if p.is_alive():
+                p.kill()
+    assert all(len(r) > 2 for r in res), [r[1] for r in res if len(r) == 2]
+    for _, want, alone, inside, got, after, _ in res:
+        assert abs(inside - want) <= 100 * 2.0 ** -24 * want and inside == got and abs(alone - want) > 0.1 * want and want > 0.5
+        assert abs(after - 0.5 * want / (want + 1e-6)) < 1e-6
+    assert res[0][3] == res[1][3] and all((a == b).all() for a, b in zip(res[0][-1], res[1][-1]))
