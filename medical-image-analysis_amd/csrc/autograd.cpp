@@ -421,11 +421,16 @@ Tensor grad_clip(const std::vector<Tensor>& grads, double max_norm) {
             throw py::value_error("clip_grads_ scales in place and needs dense tensors (got strides " + c10::str(g.strides()) + " for " + c10::str(g.sizes()) + ")");
     const c10::OptionalDeviceGuard guard(at::device_of(grads[0]));
     GradTable t(grads);
-    std::vector<const void*> each;
-    for (int i = 0; i < t.count(); ++i)
-        if (t.sizes[i]) each.push_back(t.at[i]);
+    std::vector<std::pair<const char*, const char*>> each;   // first and last byte; in this order any overlap shows between neighbours
+    for (int i = 0; i < t.count(); ++i) {
+        const char* p = static_cast<const char*>(t.at[i]);
+        if (t.sizes[i]) each.emplace_back(p, p + t.sizes[i] * grads[i].element_size() - 1);
+    }
     std::sort(each.begin(), each.end());
-    if (std::adjacent_find(each.begin(), each.end()) != each.end()) throw py::value_error("a tensor is listed twice: it would be scaled twice");
+    for (size_t i = 1; i < each.size(); ++i)
+        if (each[i].first <= each[i - 1].second)
+            throw py::value_error(each[i] == each[i - 1] ? "a tensor is listed twice: it would be scaled twice"
+                                                         : "two tensors overlap: their common elements would be scaled twice");
     check(mia_grad_clip(t.count(), t.at.data(), t.dtypes.data(), t.sizes.data(), max_norm, static_cast<double*>(ptr(t.ws)), t.ws.numel(), floats(t.out),
                         stream_of(t.ws)),
           "mia_grad_clip");

@@ -50,7 +50,7 @@ def grad_norm(grads):
 def clip_grads_(grads, max_norm):
     """Scales the tensors in place so that their global norm is at most max_norm and returns the norm they had (0-d fp32
     device tensor): g *= min(1, max_norm / (norm + 1e-6)), as torch.nn.utils.clip_grad_norm_ does. No host
-    synchronisation; the tensors must not overlap; may be captured into a HIP graph. A norm that is infinite or NaN makes the
+    synchronisation; tensors that overlap are refused; may be captured into a HIP graph. A norm that is infinite or NaN makes the
     gradients zero, NaN or both, as there: look at the returned norm where that can happen."""
     max_norm = _check_max_norm(max_norm)
     grads = list(grads)

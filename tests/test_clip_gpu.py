@@ -291,3 +291,15 @@ def test_norm_of_exchanged_gradients():
         assert abs(inside - want) <= 100 * 2.0 ** -24 * want and inside == got and abs(alone - want) > 0.1 * want and want > 0.5
         assert abs(after - 0.5 * want / (want + 1e-6)) < 1e-6
     assert res[0][3] == res[1][3] and all((a == b).all() for a, b in zip(res[0][-1], res[1][-1]))
+
+
+def test_overlapping_gradients_are_refused():
+    """Their common elements would be scaled twice, by workgroups that race; neighbours in one buffer are fine."""
+    flat = torch.randn(1000, device="cuda")
+    keep = flat.clone()
+    for a, b in ((flat[:600], flat[599:]), (flat, flat[10:20]), (flat[300:], flat[:301]), (flat.view(10, 100)[2:4], flat[250:260])):
+        with pytest.raises(ValueError, match="overlap"):
+            clip_grads_([a, torch.zeros(3, device="cuda"), b], 0.1)
+    assert torch.equal(flat, keep)
+    want = _norm64([flat])
+    assert abs(float(clip_grads_([flat[600:], flat[:600], flat[5:5]], 1e9)) - want) <= 2.0 ** -23 * want
