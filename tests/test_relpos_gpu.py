@@ -444,3 +444,24 @@ def test_bias_gradient_is_added_up_exactly(height, width, Lq):
     out = relpos_attention(q.cuda(), k.cuda(), v.cuda(), t, plan, key_mask=mask.cuda())
     (got,) = torch.autograd.grad(out, t, dout.cuda())
     _compare(got, want["dtable"], 2.0 ** -24 * want["dtable"].abs() + 1e-9, "dtable")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("Lq", [3, 70])
+def test_shared_heads_and_broadcast_inputs(Lq, dtype):
+    """Keys and values shared by the heads, by the batch, queries shared by the tokens (strides of zero): read where they lie, and their
+    gradients are the sums over what shares them. (Such a sum of n rounded gradients is off by n of their bounds and its own rounding.)"""
+    plan = RelativePositionBuckets(6, 15, 8, 16)
+    q, k, v, table, dout = _inputs(2, Lq, 90, 4, 24, dtype, plan.num_buckets, 24)
+    for dims in ((2,), (0,), (0, 2), (0, 1)):
+        one = [t[tuple(slice(0, 1) if d in dims else slice(None) for d in range(4))] for t in (q, k, v)]
+        wide = [t.expand(2, n, 4, 24) for t, n in zip(one, (Lq, 90, 90))]
+        want, tol = formula(*wide, table, plan, q_start=90 - Lq, dout=dout)
+        mine = [t.cuda().requires_grad_() for t in one]
+        out = relpos_attention(*(t.expand(2, n, 4, 24) for t, n in zip(mine, (Lq, 90, 90))), table.cuda(), plan, q_start=90 - Lq)
+        _compare(out.detach(), want["out"], tol["out"], "out")
+        for name, t, got in zip(("dq", "dk", "dv"), mine, torch.autograd.grad(out, mine, dout.cuda())):
+            total, slack = (x.sum(dims, keepdim=True) for x in (want[name], tol[name]))
+            size = want[name].abs().sum(dims, keepdim=True)
+            n = 2 * 4 * 90
+            _compare(got, total, slack + (2.0 ** -8 * total.abs() if dtype == BF16 else 0.0) + n * 2.0 ** -24 * size, name)
