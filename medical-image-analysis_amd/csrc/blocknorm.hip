@@ -414,17 +414,18 @@ __global__ __launch_bounds__(1024) void blocknorm_fold_kernel(const float* __res
     if (dgate) dgate[(size_t)blockIdx.x * C + c] = (float)((scale ? scale[c] : 1.f) * ((w1 ? w1[c] : 1.f) * v[0] + (b1 ? b1[c] : 0.f) * v[1]));
 }
 
-// parameter gradients from the group sums (S = double) or from the slab's rows themselves (float); gate (nullable): [groups][C]
+// Parameter gradients from the group sums (S = double) or from the slab's rows themselves (float); gate (nullable): [groups][C].
+// 64 row lanes x 16 columns: few rounds of loads, each of which waits for memory.
 template <typename S>
 __global__ __launch_bounds__(1024) void blocknorm_params_kernel(const S* __restrict__ sums, int groups, int C,
                                                                 const float* __restrict__ gate, const float* __restrict__ scale,
                                                                 const float* __restrict__ w1, const float* __restrict__ b1,
                                                                 float* dscale, float* dw1, float* db1, float* dw2, float* db2) {
-    __shared__ double sm[16][4][64];
-    const int col = threadIdx.x & 63, g = threadIdx.x >> 6, c = blockIdx.x * 64 + col;
+    __shared__ double sm[64][4][16];
+    const int col = threadIdx.x & 15, g = threadIdx.x >> 4, c = blockIdx.x * 16 + col;
     double v[4] = {0.0, 0.0, 0.0, 0.0};
     if (c < C)
-        for (int n = g; n < groups; n += 16) {
+        for (int n = g; n < groups; n += 64) {
             const S* p = sums + (size_t)n * 4 * C + c;
             const double gt = gate ? gate[(size_t)n * C + c] : 1.f;
             v[0] = fma(gt, (double)p[0], v[0]);
@@ -435,10 +436,16 @@ __global__ __launch_bounds__(1024) void blocknorm_params_kernel(const S* __restr
 #pragma unroll
     for (int k = 0; k < 4; ++k) sm[g][k][col] = v[k];
     __syncthreads();
+    if (threadIdx.x < 64) {   // one sum a thread; only it reads and writes its column of sm[..][g]
+        double t = sm[0][g][col];
+#pragma unroll 8
+        for (int w = 1; w < 64; ++w) t += sm[w][g][col];
+        sm[0][g][col] = t;
+    }
+    __syncthreads();
     if (g != 0 || c >= C) return;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        for (int w = 1; w < 16; ++w) v[k] += sm[w][k][col];
+    for (int k = 0; k < 4; ++k) v[k] = sm[0][k][col];
     const double sc = scale ? scale[c] : 1.f;
     if (dscale) dscale[c] = (float)((w1 ? w1[c] : 1.f) * v[0] + (b1 ? b1[c] : 0.f) * v[1]);
     if (dw1) dw1[c] = (float)(sc * v[0]);
@@ -580,10 +587,10 @@ extern "C" int mia_blocknorm_bwd(int dtype, const void* dy, const void* dz, cons
         MIA_LAUNCH(blocknorm_fold_kernel, dim3(groups, cdiv(C, 64)), dim3(1024), 0, s, ws, rows, gate ? a.S : 16, C, scale, post_w,
                    post_b, sums, gate ? dgate : nullptr);
         MIA_CHECK_LAUNCH("mia_blocknorm_bwd");
-        MIA_LAUNCH(blocknorm_params_kernel<double>, dim3(cdiv(C, 64)), dim3(1024), 0, s, sums, groups, C, gate, scale, post_w, post_b, dscale,
+        MIA_LAUNCH(blocknorm_params_kernel<double>, dim3(cdiv(C, 16)), dim3(1024), 0, s, sums, groups, C, gate, scale, post_w, post_b, dscale,
                    dpost_w, dpost_b, dpre_w, dpre_b);
     } else {
-        MIA_LAUNCH(blocknorm_params_kernel<float>, dim3(cdiv(C, 64)), dim3(1024), 0, s, ws, groups, C, gate, scale, post_w, post_b, dscale,
+        MIA_LAUNCH(blocknorm_params_kernel<float>, dim3(cdiv(C, 16)), dim3(1024), 0, s, ws, groups, C, gate, scale, post_w, post_b, dscale,
                    dpost_w, dpost_b, dpre_w, dpre_b);
     }
     MIA_CHECK_LAUNCH("mia_blocknorm_bwd");
