@@ -254,6 +254,7 @@ __global__ __launch_bounds__(WG) void blocknorm_bwd_kernel(BNormArgs a) {
     // The threads of a row of 1024 have 128 registers each: with eight channels they neither request rows ahead nor keep the
     // parameters, but read those again (from L2) where a row needs them (2048 rows of 8192, two RMS norms: 169 -> 97 us in
     // bf16, 251 -> 167 us in fp32). Single elements spill either way (353 us, 517 us so).
+    // (dy and dz were one tensor there; with two of them 182 us in fp32, 374 for rows of 8190 in single elements.)
     constexpr bool SLIM = TPR == 1024 && V > 1 && R * V == 8;
     float mul[R * V], add[R * V], w2[R * V];
     auto load_w2 = [&]() { bn_param<V, R, TPR>(a.w2, 1.f, lane, a.C, w2); };

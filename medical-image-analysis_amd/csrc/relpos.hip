@@ -271,9 +271,9 @@ __device__ __forceinline__ void rp_lds_add(double* p, float v) {
 }
 
 enum { RP_FWD, RP_BWD_Q, RP_BWD_KV };
-// Waves a SIMD has room for: the most that leave a kernel with at most a few registers in scratch (36 bytes at most). Asking for two
+// Waves a SIMD has room for: the most that leave a kernel with at most a few registers in scratch (48 bytes at most). Asking for two
 // already keeps the compiler from spreading over the accumulation registers, whose moves cost issue slots (38x38 maps, batch
-// 4, 8 heads of 64: dK/dV 140 -> 103 us, forward unchanged).
+// 4, 8 heads of 64: dK/dV 140 -> 103 us, 110 since its weights are two numbers, forward unchanged).
 constexpr int rp_waves(int what, bool half, int DP, int cols) {
     if (what == RP_FWD)
         return half ? (cols == 1 ? (DP <= 32 ? 4 : DP <= 64 ? 3 : 2) : 2) : (DP <= 32 ? 4 : DP <= 64 ? 3 : 2);
@@ -1428,8 +1428,8 @@ __global__ __launch_bounds__(256, rp_waves(RP_BWD_KV, sizeof(T) == 2, DP, KB)) v
 // Slab rows are [image][head][key block][query range]; the offsets that a row covers depend on the last two alone. A workgroup: 64
 // * PER offsets, 16 waves that share the rows where there are at least 16 of them (PER = 4: a row's four loads are in flight
 // together), else the images (PER = 1, four images in flight). A lane works out what one row covers, a ballot finds the rows
-// that reach the workgroup's offsets. 75x75 map, 4 heads, 704 rows: 11 us, 18 to 20 with PER = 1 (31 with every row tested by every
-// wave); 38x38, 8 heads, 23 rows, 4 images: 5.5 us, 7.7 with PER = 1.
+// that reach the workgroup's offsets. 75x75 map, 4 heads, 704 rows: 12 us in double (11 in fp32; there 18 to 20 with PER = 1, 31 with every
+// row tested by every wave); 38x38, 8 heads, 23 rows, 4 images: 5.7 us (5.5 in fp32, 7.7 with PER = 1).
 template <int PER>
 __global__ __launch_bounds__(1024) void relpos_offsets_kernel(RpArgs a, int ktiles, int kt, double* __restrict__ per_off) {
     __shared__ double sm[16][64 * PER];
