@@ -333,13 +333,14 @@ int mia_gather_slices(const void* vol, int elem_bytes, long long n_slices, long 
  *      the tokens without either, model.py:167-168; its only norm is the classifier's, model.py:136) ---------------------
  * u = norm1(f) (f where post = 0), y = x + scale * gate * u, z = norm2(y) (not formed where pre = 0). x, f, y, z
  * [images * rows_per_image, C] in dtype, C <= 8192; scale [C], gate [images][C] nullable; post / pre: 0 none, 1 RMS norm,
- * 2 layer norm, each with a weight [C] and a nullable bias [C]; all parameters fp32. stats (nullable): [rows][4] fp32, kept
- * for the backward pass. z is formed from y before y is rounded to dtype. */
+ * 2 layer norm, each with a weight [C] and a nullable bias [C]; all parameters fp32. stats (nullable): [rows][4] fp32 at a
+ * multiple of 16 bytes, kept for the backward pass. z is formed from y before y is rounded to dtype. */
 int mia_blocknorm_fwd(int dtype, const void* x, const void* f, int images, long long rows_per_image, int C,
                       const float* scale, const float* gate, int post, const float* post_w, const float* post_b, int pre,
                       const float* pre_w, const float* pre_b, float eps, void* y, void* z, float* stats, void* stream);
 /* dy, dz: gradients of y and z (one of them may be NULL = zero). dx, df like x; the parameter gradients (each nullable) are
- * fp32, summed in a fixed order. ws: mia_blocknorm_ws_floats(images, rows_per_image, C, gate != NULL) floats. */
+ * fp32, summed in a fixed order. ws: mia_blocknorm_ws_floats(images, rows_per_image, C, gate != NULL) floats
+ * at a multiple of 16 bytes. */
 int mia_blocknorm_bwd(int dtype, const void* dy, const void* dz, const void* x, const void* f, const float* stats, int images,
                       long long rows_per_image, int C, const float* scale, const float* gate, int post, const float* post_w,
                       const float* post_b, int pre, const float* pre_w, float* ws, long long ws_floats, void* dx, void* df,

@@ -20,7 +20,7 @@ def gated_residual_norm(x, f, scale=None, gate=None, post=None, post_weight=None
     [x.shape[0], C] (one row per image, broadcast over its tokens) are optional; post and pre name the norms, "rms" or
     "layer", each with a weight [C] and optionally a bias [C] (population variance over C, eps added to it). Parameters and
     gate are fp32. All arithmetic is fp32: z is formed from y before y is rounded to the tensors' type. Returns (y, z);
-    differentiable in every tensor. C <= 8192."""
+    differentiable (once, backward) in every tensor. C <= 8192."""
     if post not in _KINDS or pre not in _KINDS:
         raise ValueError(f"norms are 'rms', 'layer' or None (got post={post!r}, pre={pre!r})")
     dtype, shape = x.dtype, x.shape

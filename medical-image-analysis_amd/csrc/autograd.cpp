@@ -309,12 +309,13 @@ struct GatedResidualNormBackward : torch::autograd::Node {
         for (int i = 0; i < 6; ++i)
             if (has[i] && task_should_compute_output(2 + i)) got[2 + i] = rows ? at::empty(i == 1 ? gate : vector, f32) : at::zeros(i == 1 ? gate : vector, f32);
         if (!rows) return got;
-        // aligned, so that the layout of the rows (and with it the order of the sums) does not hang on a hook
-        const Tensor x_ = dense_aligned(back(x.unpack(), shape, type)), f_ = dense_aligned(back(f.unpack(), shape, type));
+        // rows that can be read 16 bytes at a time are: their layout, and with it the order of the sums, does not hang on a hook
+        const auto rows_of = C % (type == at::kBFloat16 ? 8 : 4) ? dense : dense_aligned;
+        const Tensor x_ = rows_of(back(x.unpack(), shape, type)), f_ = rows_of(back(f.unpack(), shape, type));
         const Tensor stats_ = dense_aligned(back(stats.unpack(), {images * rows, 4}, at::kFloat));
         Tensor p[6];
         for (int i = 0; i < 6; ++i)
-            if (has[i]) p[i] = dense_aligned(back(parameter[i].unpack(), i == 1 ? gate : vector, at::kFloat));
+            if (has[i]) p[i] = rows_of(back(parameter[i].unpack(), i == 1 ? gate : vector, at::kFloat));
         dy = dense(dy), dz = dense(dz);
         const long long n = mia_blocknorm_ws_floats(images, rows, C, p[1].defined());
         Tensor ws = at::empty({n}, f32);

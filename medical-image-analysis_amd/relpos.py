@@ -117,8 +117,8 @@ def relpos_attention(q, k, v, table, buckets, key_mask=None, scale=None, q_start
     key j is at token j, query i at token q_start + i (a new token against a series: q_start = Lk - 1). table: fp32
     [buckets.num_buckets, heads]. key_mask: bool [B, Lk], false = the key does not exist (what its rows hold is never read into a
     result); a query without any key gives zeros. scale defaults to 1/sqrt(D). dropout_p drops attention weights with the
-    counter-based mask of the library's other dropouts. Returns [B, Lq, heads, D]; differentiable in q, k, v and table, the
-    same bits every time."""
+    counter-based mask of the library's other dropouts. Returns [B, Lq, heads, D]; differentiable (once, backward) in q, k, v and table,
+    the same bits every time."""
     for what, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4:
             raise ValueError(f"relpos_attention: {what} must be [batch, tokens, heads, D] (got {tuple(t.shape)})")
