@@ -348,3 +348,26 @@ def test_tracing_is_refused():
             with pytest.raises(RuntimeError, match="cannot be traced"):
                 trace(function)
         assert bool(torch.isfinite(function(x)).all())
+
+
+def test_plans_built_in_inference_mode_serve_training():
+    """A head's first map may come under inference_mode; its plan, also copied and pickled with the head, is then used in training."""
+    import io
+    torch.manual_seed(4)
+    head = MultiHeadAttentionClassifier(64, 4, 3, 0.0, relative_position_buckets=8, residual_norm="rms").cuda()
+    with torch.no_grad():
+        head.relative_position_table.normal_()
+    x = torch.randn(2, 5, 6, 64, device="cuda")
+    with torch.inference_mode():
+        want = head.eval()(x)
+    buffer = io.BytesIO()
+    torch.save(head, buffer)
+    buffer.seek(0)
+    grads = []
+    for other in (head, copy.deepcopy(head), torch.load(buffer, weights_only=False)):
+        assert torch.equal(other.eval()(x), want)
+        loss = other.train()(x).square().sum()
+        grads.append(torch.autograd.grad(loss, list(other.parameters()), allow_unused=True))
+    for g in grads[1:]:
+        assert all((a is None and b is None) or torch.equal(a, b) for a, b in zip(grads[0], g))
+    assert all(g is not None for g in grads[0])
